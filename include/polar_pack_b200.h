@@ -386,6 +386,117 @@ PP_API int pp_swiglu_rows(const void* gate_up, int64_t ldg, int64_t I, void* y, 
                           const uint32_t* wait_flags, int wait_world, const uint32_t* wait_epoch, int* wait_status,
                           void* stream);
 
+/* ------------------------------------------------------- 8-bit KV cache --
+ * Keys and values of one layer for `batch` sequences in 8 bits, with one FP32
+ * scale for each block of 64 positions and head; no counterpart in the
+ * reference, whose models keep the FP16 cache of Hugging Face's generate
+ * (polar_inference.py:224-229).  Contiguous arrays, [0] keys and [1] values:
+ *   codes   uint8 [batch][kv_heads][capacity][head_dim]
+ *   scales  float [batch][kv_heads][capacity / 64]
+ *   tail    FP16  [batch][kv_heads][64][head_dim]
+ * A stored value is (code - 128) * scale, with scale = max|x| / 127 over the
+ * block and head and code = 128 + round(x / scale), ties to even (NaN counts
+ * as 0, infinities as +-65504).  The block that holds a sequence's last token
+ * is read from the FP16 tail; its codes are written by the call that completes
+ * it, so the cache does not depend on how its tokens were split into calls.
+ * capacity is a multiple of 64, head_dim 64 or 128, all arrays 16-byte aligned.
+ * Lengths, positions and counts are int32 in device memory, one per sequence;
+ * the caller advances them.  A sequence that would pass the capacity (or its
+ * rotation tables) sets *status (device int, may be NULL) to 5, is not written
+ * and gets zero outputs.  Nothing at or past a sequence's length is used.
+ * Rotation (optional, all NULL for none): FP16 tables cos_t / sin_t
+ * [rope_len][head_dim] and rope_pos [batch], the rotation position of the
+ * call's first row (it may differ from the cache position after evictions);
+ * rounded as in pp_decode_attention.  Strides are those of (sequence, token,
+ * head), multiples of 8 elements; rows are contiguous and 16-byte aligned.
+ */
+#define PP_KV8_BLOCK 64
+#define PP_KV8_MAX_BATCH 4096
+
+typedef struct pp_kv8_cache {
+  void* codes[2];
+  float* scales[2];
+  void* tail[2];
+  int64_t batch, kv_heads, capacity, head_dim;
+} pp_kv8_cache;
+
+/* Appends rows i < counts[b] (NULL: all n) of k, v (batch, n, kv_heads) at
+ * positions pos[b] + i.  A negative position marks an unused sequence. */
+PP_API int pp_kv8_append(const pp_kv8_cache* cache, const void* k, const int64_t k_strides[3], const void* v,
+                         const int64_t v_strides[3], int64_t n, const int* pos, const int* counts, const void* cos_t,
+                         const void* sin_t, const int* rope_pos, int64_t rope_len, int* status, void* stream);
+
+/* The stored values of positions start[b] (NULL: 0) .. start[b] + count - 1 as
+ * FP16, k and v contiguous (batch, count, kv_heads, head_dim); zeros outside
+ * 0 .. lens[b] - 1. */
+PP_API int pp_kv8_restore(const pp_kv8_cache* cache, const int* lens, const int* start, int64_t count, void* k, void* v,
+                          int* status, void* stream);
+
+/* Causal grouped-query attention of n query tokens per sequence:
+ *   out[b][i][h] = softmax(scale * q[b][i][h] k^T) v
+ * over positions 0 .. lens[b] - counts[b] + i of kv head h / (nq / kv_heads):
+ * the queries are the last counts[b] (NULL: n) of the sequence's lens[b]
+ * tokens, appended before.  Rows i >= counts[b], and rows that attend nothing,
+ * are zero.  At most 16 query heads per kv head.  FP32 scores, softmax and
+ * sums. */
+PP_API int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64_t nq, int weights,
+                                            size_t* bytes);
+
+PP_API int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[3], int64_t n, int64_t nq,
+                            const int* lens, const int* counts, float scale, void* out, const int64_t out_strides[3],
+                            const void* cos_t, const void* sin_t, const int* rope_pos, int64_t rope_len, void* workspace,
+                            size_t workspace_bytes, int* status, void* stream);
+
+/* The single-token form: appends one token per sequence at pos[b] (as
+ * pp_kv8_append) and attends to positions 0 .. pos[b] (as pp_kv8_attention).
+ * weights (optional, NULL: none): float [batch][kv_heads][capacity];
+ * weights[b][g][t] += sum of head group g's softmax weights at position t.
+ * Strides are those of (sequence, head).  Calls at the same position rewrite
+ * the same token. */
+PP_API int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[2], int64_t nq, const void* k,
+                         const int64_t k_strides[2], const void* v, const int64_t v_strides[2], const int* pos,
+                         float scale, float* weights, void* out, const int64_t out_strides[2], const void* cos_t,
+                         const void* sin_t, const int* rope_pos, int64_t rope_len, void* workspace,
+                         size_t workspace_bytes, int* status, void* stream);
+
+/* Eviction by accumulated attention weight into another cache (same
+ * sequences, heads and head_dim; any capacity of at least keep).  Of each
+ * sequence and kv head that holds more than keep tokens, the first sinks and
+ * the last recent stay, and those of the others with the largest weights
+ * (float [batch][kv_heads][capacity]; equal weights by the lower position,
+ * NaN above every number), in their order.  The new cache is what appending
+ * the kept tokens' restored values to an empty one gives, except that a block
+ * which is one whole coded block of the old cache is copied unchanged.
+ * into_weights ([batch][kv_heads][into->capacity]) receives the kept tokens'
+ * weights, zero past them; new_lens[b] = min(lens[b], keep); kept
+ * [batch][kv_heads][keep] the old positions, -1 past new_lens[b]. */
+PP_API int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int* lens, const float* weights,
+                        float* into_weights, int* new_lens, int* kept, int64_t keep, int64_t sinks, int64_t recent,
+                        int* status, void* stream);
+
+/* -------------------------------------------------------------- scoring --
+ * For each of `rows` rows of logits (row stride ldx elements, contiguous rows
+ * of vocab values, any alignment):
+ *   logprob = x[token] - ln sum e^x      (FP32)
+ *   entropy = -sum p ln p, p = softmax(x), terms with p = 0 left out
+ *   top_ids / top_logprobs [rows][top]: the top largest logits, largest first,
+ *     equal ones by the lower index, NaN before every number, with their log
+ *     probabilities (top <= 32 and <= vocab)
+ * What the reference's perplexity tools take from whole logits
+ * (measure_ppl.py:40-65, measure_quad_ppl.py:57-85).  A negative token asks
+ * for no score (logprob 0); a token past the vocabulary gets NaN and sets
+ * *status (device int, may be NULL) to 4.  A row whose logits are all -inf has
+ * logprob and top_logprobs -inf and entropy 0; one with a NaN or +inf has
+ * entropy NaN.  dtype: PP_F16, PP_BF16 or PP_F32. */
+#define PP_F16 0
+#define PP_BF16 1
+#define PP_F32 2
+#define PP_LOGPROBS_MAX_TOP 32
+
+PP_API int pp_token_logprobs(const void* logits, int dtype, int64_t ldx, int64_t rows, int64_t vocab, const int* tokens,
+                             int64_t top, float* logprob, float* entropy, int* top_ids, float* top_logprobs, int* status,
+                             void* stream);
+
 /* ------------------------------------------------------------------ dual --
  * Kernel-layout fused dequant GEMM, the drop-in for `polar_dual_bitpacked`
  * (reference polar_kernels.py:98-115, kernel 30-95):

@@ -44,7 +44,16 @@ class QuadLinearDesc(ctypes.Structure):
 PER_MODEL_X = 1
 
 
+class Kv8CacheDesc(ctypes.Structure):
+    """``pp_kv8_cache``: the arrays of one layer's 8-bit KV cache."""
+    _fields_ = [("codes", ctypes.c_void_p * 2), ("scales", ctypes.c_void_p * 2), ("tail", ctypes.c_void_p * 2),
+                ("batch", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("capacity", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64)]
+
+
 _DESC_P = ctypes.POINTER(QuadLinearDesc)
+_KV8_P = ctypes.POINTER(Kv8CacheDesc)
+_I64_P = ctypes.POINTER(_i64)
 
 _SIGNATURES = {
     "pp_last_error": ([], ctypes.c_char_p),
@@ -101,6 +110,20 @@ _SIGNATURES = {
                              _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p], _int),
     "pp_swiglu_rows": ([_c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p,
                         _c_void_p], _int),
+    "pp_kv8_append": ([_KV8_P, _c_void_p, _I64_P, _c_void_p, _I64_P, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                       _c_void_p, _i64, _c_void_p, _c_void_p], _int),
+    "pp_kv8_restore": ([_KV8_P, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p], _int),
+    "pp_kv8_attention_workspace_bytes": ([_KV8_P, _i64, _i64, _int, ctypes.POINTER(_size_t)], _int),
+    "pp_kv8_attention": ([_KV8_P, _c_void_p, _I64_P, _i64, _i64, _c_void_p, _c_void_p, ctypes.c_float, _c_void_p,
+                          _I64_P, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _size_t, _c_void_p, _c_void_p],
+                         _int),
+    "pp_kv8_decode": ([_KV8_P, _c_void_p, _I64_P, _i64, _c_void_p, _I64_P, _c_void_p, _I64_P, _c_void_p,
+                       ctypes.c_float, _c_void_p, _c_void_p, _I64_P, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p,
+                       _size_t, _c_void_p, _c_void_p], _int),
+    "pp_kv8_evict": ([_KV8_P, _KV8_P, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64,
+                      _c_void_p, _c_void_p], _int),
+    "pp_token_logprobs": ([_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+                           _c_void_p, _c_void_p, _c_void_p], _int),
     "pp_dual_gemm_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_size_t)], _int),
     "pp_dual_gemm": ([_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p,
                       _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,

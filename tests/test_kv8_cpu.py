@@ -1,0 +1,67 @@
+"""Argument checks of the 8-bit KV cache and scoring entry points (no GPU: every
+refusal happens on the host, before anything is enqueued)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from polar_pack_b200 import _lib
+    return _lib
+
+
+def _cache(lib, **kw):
+    p = ctypes.c_void_p * 2
+    d = dict(codes=p(256, 512), scales=p(256, 512), tail=p(256, 512), batch=2, kv_heads=2, capacity=128, head_dim=128)
+    d.update(kw)
+    return ctypes.byref(lib.Kv8CacheDesc(**d))
+
+
+S3 = (ctypes.c_int64 * 3)(1024, 256, 128)
+S2 = (ctypes.c_int64 * 2)(256, 128)
+
+
+@pytest.mark.parametrize("bad", [dict(batch=0), dict(batch=4097), dict(kv_heads=0), dict(capacity=100),
+                                 dict(capacity=0), dict(head_dim=96), dict(codes=(ctypes.c_void_p * 2)(0, 256)),
+                                 dict(tail=(ctypes.c_void_p * 2)(264, 256)),
+                                 dict(scales=(ctypes.c_void_p * 2)(256, 0))])
+def test_descriptor(lib, bad):
+    L, c = lib.load(), _cache(lib, **bad)
+    rcs = [L.pp_kv8_append(c, 256, S3, 256, S3, 1, 256, None, None, None, None, 0, None, None),
+           L.pp_kv8_restore(c, 256, None, 1, 256, 256, None, None),
+           L.pp_kv8_attention(c, 256, S3, 1, 4, 256, None, 1.0, 256, S3, None, None, None, 0, 256, 1 << 30, None, None),
+           L.pp_kv8_decode(c, 256, S2, 4, 256, S2, 256, S2, 256, 1.0, None, 256, S2, None, None, None, 0, 256, 1 << 30,
+                           None, None),
+           L.pp_kv8_evict(c, _cache(lib), 256, 256, 512, 256, 256, 64, 0, 0, None, None),
+           L.pp_kv8_attention_workspace_bytes(c, 1, 4, 0, ctypes.byref(ctypes.c_size_t()))]
+    assert rcs == [lib.PP_ERR_INVALID] * 6
+
+
+def test_arguments(lib):
+    L, c = lib.load(), _cache(lib)
+    odd = (ctypes.c_int64 * 3)(1024, 256, 100)
+    bad = [L.pp_kv8_append(c, None, S3, 256, S3, 1, 256, None, None, None, None, 0, None, None),
+           L.pp_kv8_append(c, 256, S3, 264, S3, 1, 256, None, None, None, None, 0, None, None),
+           L.pp_kv8_append(c, 256, odd, 256, S3, 1, 256, None, None, None, None, 0, None, None),
+           L.pp_kv8_append(c, 256, S3, 256, S3, -1, 256, None, None, None, None, 0, None, None),
+           L.pp_kv8_append(c, 256, S3, 256, S3, 1, 256, None, 256, None, 256, 10, None, None),    # half a rotation
+           L.pp_kv8_restore(c, None, None, 1, 256, 256, None, None),
+           L.pp_kv8_restore(c, 256, None, 1, 256, 8, None, None),
+           L.pp_kv8_attention(c, 256, S3, 1, 5, 256, None, 1.0, 256, S3, None, None, None, 0, 256, 1 << 30, None, None),
+           L.pp_kv8_attention(c, 256, S3, 1, 40, 256, None, 1.0, 256, S3, None, None, None, 0, 256, 1 << 30, None, None),
+           L.pp_kv8_attention(c, 256, S3, 70000, 4, 256, None, 1.0, 256, S3, None, None, None, 0, 256, 1 << 30, None,
+                              None),
+           L.pp_kv8_attention(c, 256, odd, 1, 4, 256, None, 1.0, 256, S3, None, None, None, 0, 256, 1 << 30, None, None),
+           L.pp_kv8_evict(c, c, 256, 256, 512, 256, 256, 64, 0, 0, None, None),
+           L.pp_kv8_evict(c, _cache(lib, kv_heads=1), 256, 256, 512, 256, 256, 64, 0, 0, None, None)]
+    assert bad == [lib.PP_ERR_INVALID] * len(bad)
+    assert L.pp_kv8_append(c, 256, S3, 256, S3, 0, 256, None, None, None, None, 0, None, None) == 0
+    for args in ((9, 100, 1, 0), (0, 0, 1, 0), (0, 100, 1, 33), (0, 5, 1, 6), (2, 100, 1, -1), (2, 100, -1, 0)):
+        dtype, vocab, rows, top = args
+        assert L.pp_token_logprobs(256, dtype, 100, rows, vocab, 256, top, 256, 256, 256, 256, None,
+                                   None) == lib.PP_ERR_INVALID
+    assert L.pp_token_logprobs(257, 0, 100, 1, 100, 256, 0, 256, 256, 256, 256, None, None) == lib.PP_ERR_INVALID
+    assert L.pp_token_logprobs(256, 0, 100, 0, 100, 256, 0, 256, 256, 256, 256, None, None) == 0
