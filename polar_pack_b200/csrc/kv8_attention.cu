@@ -3,6 +3,7 @@
 //   s_t = scale * q . k_t,  p = softmax(s) over t <= the query's position,
 //   out = sum_t p_t v_t     (FP32 throughout, rounded once)
 #include "kv8.cuh"
+#include "kv8_decode.cuh"
 
 namespace pp {
 namespace {
@@ -17,12 +18,10 @@ struct AttnParams {
   __half* out;
   int64_t ldob, ldot, ldoh;
   const int* lens;
-  int extra;            // tokens beyond lens: 1 after a fused append, else 0
   const int* counts;
   int n, nq;
   float scale;
   Kv8Rope rope;
-  float* weights;       // [batch][kv head][cap] += the group's probabilities (n == 1), or NULL
   int* status;
 };
 
@@ -36,7 +35,7 @@ __global__ void __launch_bounds__(kTile) kv8_attention_kernel(const AttnParams p
   pdl_wait();
   const int i = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int group = p.nq / p.c.nkv;
-  const int len = p.lens[b] + p.extra;
+  const int len = p.lens[b];
   const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
   const int end = len - cnt + i + 1;  // positions attended
   bool ok = len <= p.c.cap;
@@ -131,14 +130,105 @@ __global__ void __launch_bounds__(kTile) kv8_attention_kernel(const AttnParams p
   }
   if (tid < HD)
     for (int h = 0; h < group; ++h) out[h * p.ldoh + tid] = __float2half_rn(acc[h] / sum[h]);
-  if (p.weights) {
-    for (int t = tid; t < end; t += kTile) {
-      float s[kMaxGroup], w = 0.f;
-      scores(t, s);
-      for (int h = 0; h < group; ++h) w += expf(s[h] * p.scale - mx[h]) / sum[h];
-      p.weights[p.c.head(b, kvh) * p.c.cap + t] += w;
-    }
+}
+
+// How a call with `rows` query rows per kv head runs on kv8_decode_kernel:
+// tiles of 8 rows while one is enough, else of 16.
+constexpr int kDecodeRows = 64;
+
+struct DecodePlan {
+  int nt, tiles, ctas;
+  size_t cnt, part, lse, scores, bytes;  // workspace offsets
+};
+
+DecodePlan plan_decode(const Kv8Cache& c, int64_t n, int64_t nq, bool weights, int ctas) {
+  DecodePlan d{};
+  const int64_t rows = n * (nq / c.nkv);
+  d.nt = rows <= 8 ? 1 : 2;
+  d.tiles = (int)cdiv(rows, 8 * d.nt);
+  d.ctas = ctas;
+  d.part = align_up((size_t)ctas * sizeof(int), 256);  // the counters' place must not depend on the call
+  d.lse = align_up(d.part + (size_t)ctas * 2 * kv8_part_floats(d.nt, c.hd) * sizeof(float), 256);
+  d.scores = align_up(d.lse + (weights ? (size_t)c.batch * nq * sizeof(float) : 0), 256);
+  d.bytes = d.scores + (weights ? (size_t)c.batch * nq * c.cap * sizeof(float) : 0);
+  return d;
+}
+
+bool g_attr[4][64];
+int g_limit[4][64];
+
+template <int NT, int HD>
+int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
+  constexpr int kv = (NT - 1) * 2 + (HD == 128);
+  using S = Kv8DecodeSmem<NT, HD>;
+  auto kern = kv8_decode_kernel<NT, HD>;
+  int lim = 0;
+  if (int rc = ensure_smem_attr(kern, g_attr[kv], g_limit[kv], &lim)) return rc;
+  const int smem = S::bytes(p.c.batch);
+  if (smem > lim) {
+    set_error("kv8_decode_kernel: %d bytes of shared memory needed, %d available", smem, lim);
+    return PP_ERR_CUDA;
   }
+  CUtensorMap tm[2];
+  const uint64_t rows = (uint64_t)p.c.batch * p.c.nkv * p.c.cap;
+  for (int w = 0; w < 2; ++w)
+    if (int rc = encode_tmap_2d(&tm[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.c.codes[w], HD, rows, HD, HD, kDecUnit,
+                                HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+      return rc;
+  return launch_kernel("kv8_decode_kernel", launch_overlap(), kern, dim3((unsigned)ctas), dim3(kDecWarps * 32),
+                       (size_t)smem, s, p, tm[0], tm[1]);
+}
+
+// Query and output rows, heads and sizes, checked.  Sets *empty for a call
+// without work.
+int check_rows(const char* who, const Kv8Cache& c, const void* q, const int64_t* qs, int64_t n, int64_t nq,
+               const int* lens, const void* out, const int64_t* os, const int* status, bool* empty) {
+  const bool heads = nq >= 1 && nq % c.nkv == 0 && nq / c.nkv <= kMaxGroup;
+  *empty = n == 0 && heads;
+  if (*empty) return PP_OK;
+  if (!q || !qs || !lens || !out || !os || !status || n < 0 || n > 65535 || !heads) {
+    set_error("%s: queries, lengths, outputs and a status word are required, at most 65535 tokens, query heads a "
+              "multiple of the kv heads (at most %d for each)", who, kMaxGroup);
+    return PP_ERR_INVALID;
+  }
+  for (int i = 0; i < 3; ++i)
+    if (!aligned(q, 16) || !aligned(out, 16) || qs[i] % 8 || os[i] % 8) {
+      set_error("%s: query and output rows must be 16-byte aligned", who);
+      return PP_ERR_INVALID;
+    }
+  if ((int64_t)c.batch * c.nkv * c.cap > INT32_MAX) {
+    set_error("%s: sequences x heads x capacity must stay below 2^31", who);
+    return PP_ERR_INVALID;
+  }
+  return PP_OK;
+}
+
+int run_decode(const char* who, Kv8DecodeParams& p, float* weights, void* workspace, size_t workspace_bytes,
+               cudaStream_t s) {
+  const int ctas = device_sm_count(current_device());
+  if (ctas < 1) {
+    set_error("%s: no current CUDA device", who);
+    return PP_ERR_CUDA;
+  }
+  const DecodePlan d = plan_decode(p.c, p.n, p.nq, weights != nullptr, ctas);
+  if (!workspace || workspace_bytes < d.bytes || !aligned(workspace, 256)) {
+    set_error("%s: workspace of %zu bytes (256-byte aligned, zero-filled) required", who, d.bytes);
+    return PP_ERR_WORKSPACE;
+  }
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  p.tiles = d.tiles;
+  p.cnt = reinterpret_cast<int*>(ws);
+  p.part = reinterpret_cast<float*>(ws + d.part);
+  if (weights) {
+    p.lse = reinterpret_cast<float*>(ws + d.lse);
+    p.scores = reinterpret_cast<float*>(ws + d.scores);
+  }
+  const int rc = p.c.hd == 128 ? (d.nt == 1 ? launch_decode<1, 128>(p, ctas, s) : launch_decode<2, 128>(p, ctas, s))
+                               : (d.nt == 1 ? launch_decode<1, 64>(p, ctas, s) : launch_decode<2, 64>(p, ctas, s));
+  if (rc || !weights) return rc;
+  const Kv8WeightsParams w{p.scores, p.lse, weights, p.lens, p.rope, p.extra, p.nq, p.c.nkv, p.c.cap};
+  return launch_kernel("kv8_weights_kernel", launch_overlap(), kv8_weights_kernel,
+                       dim3((unsigned)cdiv(p.c.cap, 256), (unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(256), 0, s, w);
 }
 
 }  // namespace
@@ -149,58 +239,57 @@ extern "C" {
 int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64_t nq, int weights, size_t* bytes) {
   pp::Kv8Cache c{};
   if (int rc = pp::kv8_cache("pp_kv8_attention_workspace_bytes", cache, &c)) return rc;
-  if (!bytes || n < 0 || nq < 1) {
+  if (!bytes || n < 0 || nq < 1 || nq % c.nkv) {
     pp::set_error("pp_kv8_attention_workspace_bytes: invalid arguments");
     return PP_ERR_INVALID;
   }
   *bytes = 0;
-  return PP_OK;
-}
-
-static int kv8_run(const char* who, pp::AttnParams& p, const void* q, const int64_t* qs, int64_t n, int64_t nq,
-                   const int* lens, float scale, void* out, const int64_t* os, void* stream) {
-  const bool heads = nq >= 1 && nq % p.c.nkv == 0 && nq / p.c.nkv <= pp::kMaxGroup;
-  if (n == 0 && heads) return PP_OK;
-  if (!q || !qs || !lens || !out || !os || n < 0 || n > 65535 || !heads) {
-    pp::set_error("%s: queries, lengths and outputs are required, at most 65535 tokens, query heads a multiple of the kv "
-                  "heads (at most %d for each)", who, pp::kMaxGroup);
-    return PP_ERR_INVALID;
-  }
-  for (int i = 0; i < 3; ++i)
-    if (!pp::aligned(q, 16) || !pp::aligned(out, 16) || qs[i] % 8 || os[i] % 8) {
-      pp::set_error("%s: query and output rows must be 16-byte aligned", who);
-      return PP_ERR_INVALID;
+  if (n > 0 && n * (nq / c.nkv) <= pp::kDecodeRows) {
+    const int ctas = pp::device_sm_count(pp::current_device());
+    if (ctas < 1) {
+      pp::set_error("pp_kv8_attention_workspace_bytes: no current CUDA device");
+      return PP_ERR_CUDA;
     }
-  p.q = reinterpret_cast<const __half*>(q);
-  p.ldqb = qs[0];
-  p.ldqt = qs[1];
-  p.ldqh = qs[2];
-  p.out = reinterpret_cast<__half*>(out);
-  p.ldob = os[0];
-  p.ldot = os[1];
-  p.ldoh = os[2];
-  p.lens = lens;
-  p.n = (int)n;
-  p.nq = (int)nq;
-  p.scale = scale;
-  return pp::launch_kernel("kv8_attention_kernel", pp::launch_overlap(),
-                           p.c.hd == 128 ? pp::kv8_attention_kernel<128> : pp::kv8_attention_kernel<64>,
-                           dim3((unsigned)n, (unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kTile), 0,
-                           reinterpret_cast<cudaStream_t>(stream), p);
+    *bytes = pp::plan_decode(c, n, nq, weights != 0, ctas).bytes;
+  }
+  return PP_OK;
 }
 
 int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[3], int64_t n, int64_t nq,
                      const int* lens, const int* counts, float scale, void* out, const int64_t out_strides[3],
                      const void* cos_t, const void* sin_t, const int* rope_pos, int64_t rope_len, void* workspace,
                      size_t workspace_bytes, int* status, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
-  pp::AttnParams p{};
+  pp::Kv8DecodeParams p{};
   if (int rc = pp::kv8_cache("pp_kv8_attention", cache, &p.c)) return rc;
   if (int rc = pp::kv8_rope("pp_kv8_attention", cos_t, sin_t, rope_pos, rope_len, &p.rope)) return rc;
-  p.counts = counts;
-  p.status = status;
-  return kv8_run("pp_kv8_attention", p, q, q_strides, n, nq, lens, scale, out, out_strides, stream);
+  bool empty = false;
+  if (int rc = pp::check_rows("pp_kv8_attention", p.c, q, q_strides, n, nq, lens, out, out_strides, status, &empty))
+    return rc;
+  if (empty) return PP_OK;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (n * (nq / p.c.nkv) <= pp::kDecodeRows) {
+    p.q = reinterpret_cast<const __half*>(q);
+    p.ldqb = q_strides[0];
+    p.ldqt = q_strides[1];
+    p.ldqh = q_strides[2];
+    p.out = reinterpret_cast<__half*>(out);
+    p.ldob = out_strides[0];
+    p.ldot = out_strides[1];
+    p.ldoh = out_strides[2];
+    p.lens = lens;
+    p.counts = counts;
+    p.n = (int)n;
+    p.nq = (int)nq;
+    p.scale2 = scale * 1.44269504088896341f;
+    p.status = status;
+    return pp::run_decode("pp_kv8_attention", p, nullptr, workspace, workspace_bytes, s);
+  }
+  pp::AttnParams a{p.c,     reinterpret_cast<const __half*>(q),
+                   q_strides[0], q_strides[1], q_strides[2], reinterpret_cast<__half*>(out),
+                   out_strides[0], out_strides[1], out_strides[2], lens, counts, (int)n, (int)nq, scale, p.rope, status};
+  return pp::launch_kernel("kv8_attention_kernel", pp::launch_overlap(),
+                           p.c.hd == 128 ? pp::kv8_attention_kernel<128> : pp::kv8_attention_kernel<64>,
+                           dim3((unsigned)n, (unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kTile), 0, s, a);
 }
 
 int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[2], int64_t nq, const void* k,
@@ -208,23 +297,40 @@ int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t q_stri
                   float* weights, void* out, const int64_t out_strides[2], const void* cos_t, const void* sin_t,
                   const int* rope_pos, int64_t rope_len, void* workspace, size_t workspace_bytes, int* status,
                   void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
-  pp::AttnParams p{};
+  pp::Kv8DecodeParams p{};
   if (int rc = pp::kv8_cache("pp_kv8_decode", cache, &p.c)) return rc;
   if (int rc = pp::kv8_rope("pp_kv8_decode", cos_t, sin_t, rope_pos, rope_len, &p.rope)) return rc;
-  if (!q_strides || !k_strides || !v_strides || !out_strides) {
-    pp::set_error("pp_kv8_decode: strides are required");
+  if (!q_strides || !k || !k_strides || !v || !v_strides || !out_strides) {
+    pp::set_error("pp_kv8_decode: keys, values and strides are required");
     return PP_ERR_INVALID;
   }
-  const int64_t ks[3] = {k_strides[0], 0, k_strides[1]}, vs[3] = {v_strides[0], 0, v_strides[1]};
-  if (int rc = pp_kv8_append(cache, k, ks, v, vs, 1, pos, nullptr, cos_t, sin_t, rope_pos, rope_len, status, stream))
-    return rc;
-  p.extra = 1;
-  p.weights = weights;
-  p.status = status;
   const int64_t qs[3] = {q_strides[0], 0, q_strides[1]}, os[3] = {out_strides[0], 0, out_strides[1]};
-  return kv8_run("pp_kv8_decode", p, q, qs, 1, nq, pos, scale, out, os, stream);
+  bool empty = false;
+  if (int rc = pp::check_rows("pp_kv8_decode", p.c, q, qs, 1, nq, pos, out, os, status, &empty)) return rc;
+  const void* x[2] = {k, v};
+  const int64_t* st[2] = {k_strides, v_strides};
+  for (int w = 0; w < 2; ++w) {
+    if (!pp::aligned(x[w], 16) || st[w][0] % 8 || st[w][1] % 8) {
+      pp::set_error("pp_kv8_decode: rows must be 16-byte aligned");
+      return PP_ERR_INVALID;
+    }
+    p.x[w] = reinterpret_cast<const __half*>(x[w]);
+    p.ldxb[w] = st[w][0];
+    p.ldxh[w] = st[w][1];
+  }
+  p.q = reinterpret_cast<const __half*>(q);
+  p.ldqb = qs[0];
+  p.ldqh = qs[2];
+  p.out = reinterpret_cast<__half*>(out);
+  p.ldob = os[0];
+  p.ldoh = os[2];
+  p.lens = pos;
+  p.extra = 1;
+  p.n = 1;
+  p.nq = (int)nq;
+  p.scale2 = scale * 1.44269504088896341f;
+  p.status = status;
+  return pp::run_decode("pp_kv8_decode", p, weights, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,772 @@
+// Decode attention over the 8-bit KV cache: few query rows per kv head, any
+// cache length (kv8_attention.cu launches it).
+//
+// Mathematics.  With S = scale * s_k (q . (c_k - 128)) for the codes c_k of a
+// block, out = sum_blocks s_v (P (c_v - 128)) / sum P, P = exp(S - m): the
+// codes enter the products as the exact FP16 integers -128..127 and the block
+// scales are applied in FP32 beside them.  P is rounded to FP16 relative to its
+// own unit's maximum m (2^-11 of values up to 1), everything else is FP32.
+//
+// Bound: the cache's bytes at long lengths, latency at short ones.  Work is
+// counted in units, 32 positions of codes or 16 FP16 rows of the tail, over
+// all (sequence, kv head, row tile) segments in a row, and each CTA takes an
+// equal share of them, so ragged batches balance; where the segments divide
+// the GPU nearly evenly, no share spans two of them.  The shares come from the
+// lengths in device memory.  A warp has a ring of units that arrive by
+// swizzled TMA boxes, two in flight; keys are the A operand of m16n8k16 (16
+// positions x 8 rows), read by ldmatrix with the four dimensions of a lane's
+// word as its k elements, values by transposed ldmatrix, whose word holds two
+// dimensions at two positions: both orders cost nothing, since the queries and
+// the outputs take the same permutation.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace pp {
+
+constexpr int kDecWarps = 8;
+constexpr int kDecSlots = 2;   // units in flight per warp: 128 KB per SM at head_dim 128
+constexpr int kDecUnit = 32;   // positions of a coded unit
+constexpr int kDecTailUnit = 16;
+
+struct Kv8DecodeParams {
+  Kv8Cache c;
+  const __half* q;
+  int64_t ldqb, ldqt, ldqh;
+  __half* out;
+  int64_t ldob, ldot, ldoh;
+  const int* lens;
+  int extra;                 // 1: the call's own token follows the lens[b] of the cache
+  const int* counts;
+  int n, nq, tiles;          // query tokens, query heads, row tiles per kv head
+  float scale2;              // scale * log2(e)
+  Kv8Rope rope;
+  const __half* x[2];        // the token's key and value rows (extra == 1)
+  int64_t ldxb[2], ldxh[2];
+  int* cnt;                  // [ctas] arrivals at the segment whose units begin in that CTA, zero between launches
+  float* part;               // [ctas][2] partial results
+  float* lse;                // [batch][nq] log2 of the softmax sums (scores != NULL)
+  float* scores;             // [batch][nq][cap] log2-scaled scores, or NULL
+  int* status;
+};
+
+template <int NT, int HD>
+struct Kv8DecodeSmem {
+  static constexpr int kSide = kDecUnit * HD;                    // a unit's keys or values
+  static constexpr int kSlot = 2 * kSide;
+  static constexpr int kRing = kDecWarps * kDecSlots * kSlot;
+  static constexpr int kMerge = kRing;                           // half the warps' results
+  static constexpr int kMergeWarp = (HD / 16 * NT * 4 + NT * 4) * 32 * 4;
+  static constexpr int kQ = kMerge + kDecWarps / 2 * kMergeWarp; // query rows, then the token's key and value
+  static constexpr int kQRow = HD * 2 + 32;  // conflict-free 8-byte reads of eight rows
+  static constexpr int kNew = kQ + NT * 8 * kQRow;
+  static constexpr int kBar = kNew + 2 * HD * 2;
+  static constexpr int kLens = kBar + kDecWarps * kDecSlots * 8; // lengths, then unit prefix
+  static constexpr int bytes(int batch) { return kLens + (2 * batch + 2) * 4; }
+};
+
+// Floats of one partial result: NT * 8 rows of HD sums, then maxima and sums.
+__host__ __device__ constexpr int kv8_part_floats(int nt, int hd) { return nt * 8 * (hd + 2); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Two codes of a word as FP16 integers code - 128: the byte in the low half of
+// 0x6400 is 1024 + code, exactly.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+  return h2u(__hsub2(u2h(__byte_perm(w, 0x64646464u, SEL)), __float2half2_rn(1152.f)));
+}
+
+// Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte or
+// 64-byte rows, as the tensor maps of launch_decode order them).
+template <int HD>
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return HD == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// One warp's running result: NT tiles of 8 rows (the columns of its mma
+// accumulators).  A lane holds rows 2 (lane & 3) + j of a tile; o[i][nt][j]
+// and o[i][nt][2 + j] are dimensions 16 i + 2 (lane >> 2) and the next.
+template <int NT, int HD>
+struct Kv8Acc {
+  float o[HD / 16][NT][4];
+  float m[NT][2], l[NT][2];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[nt][j] = -INFINITY;
+        l[nt][j] = 0.f;
+      }
+  }
+
+  // Moves the reference of row (nt, j) to `to`.
+  __device__ __forceinline__ void rebase(int nt, int j, float to) {
+    const float f = m[nt][j] == -INFINITY ? 0.f : ex2(m[nt][j] - to);
+    m[nt][j] = to;
+    l[nt][j] *= f;
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      o[i][nt][j] *= f;
+      o[i][nt][2 + j] *= f;
+    }
+  }
+};
+
+// Scores s[mt] (16 positions each, log2-scaled, masked) to probabilities
+// relative to the unit's maximum.  Gives each row's factor that brings the
+// unit's sums to the running reference, which moves only when the maximum
+// outgrows it by 2^8, so most units rescale nothing; and P^T as B operands.
+template <int NT, int HD, int MT>
+__device__ __forceinline__ void kv8_softmax(Kv8Acc<NT, HD>& a, float (&s)[MT][NT][4], float (&gain)[NT][2],
+                                            uint32_t (&pb)[MT][NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float mu[2];
+    bool grow = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float m = s[0][nt][j];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) m = fmaxf(m, fmaxf(s[mt][nt][j], s[mt][nt][2 + j]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      mu[j] = m;
+      grow |= m > a.m[nt][j] + 8.f;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (mu[j] > a.m[nt][j] + 8.f) a.rebase(nt, j, mu[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float base = mu[j] == -INFINITY ? 0.f : mu[j];
+      gain[nt][j] = mu[j] == -INFINITY ? 0.f : ex2(mu[j] - a.m[nt][j]);
+      float sum = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e = ex2(s[mt][nt][2 * h + j] - base);
+          s[mt][nt][2 * h + j] = e;
+          sum += e;
+        }
+      a.l[nt][j] = fmaf(sum, gain[nt][j], a.l[nt][j]);
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pb[mt][nt][h] = transpose8(h2u(__floats2half2_rn(s[mt][nt][2 * h], s[mt][nt][2 * h + 1])));
+  }
+}
+
+// What a CTA knows of the launch's work: effective lengths and unit counts.
+struct Kv8Work {
+  const int* len;   // [batch], 0 for sequences without work
+  const int* pre;   // [batch + 1] units before each sequence, all heads and tiles
+  int batch, per_seq;  // segments per sequence: kv heads x row tiles
+  __device__ __forceinline__ static int units(int len) {
+    if (len <= 0) return 0;
+    const int last = kv8_last_block(len);
+    return last * (kKvBlock / kDecUnit) + (len - last * kKvBlock + kDecTailUnit - 1) / kDecTailUnit;
+  }
+};
+
+// Where a unit index falls: sequence, segment of the sequence, unit.
+struct Kv8Cursor {
+  int b, seg, u, U;
+  __device__ __forceinline__ void seek(const Kv8Work& w, int idx) {
+    int lo = 0, hi = w.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (w.pre[mid] <= idx) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    U = Kv8Work::units(w.len[b]);
+    seg = (idx - w.pre[b]) / U;
+    u = idx - w.pre[b] - seg * U;
+  }
+  // idx must stay below the total.
+  __device__ __forceinline__ void advance(const Kv8Work& w, int by) {
+    u += by;
+    while (u >= U) {
+      u -= U;
+      if (++seg == w.per_seq) {
+        seg = 0;
+        do ++b;
+        while (w.pre[b + 1] == w.pre[b]);
+        U = Kv8Work::units(w.len[b]);
+      }
+    }
+  }
+};
+
+// The blocks of the cache that a token completes, and the token's own row in
+// the tail: nothing that attends in this launch reads either.
+template <int HD>
+__device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const int* s_len, float* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int items = p.c.batch * p.c.nkv * 2;
+  const int cta = gridDim.x - 1 - blockIdx.x;  // idle CTAs of short launches come first
+  auto row8 = [&](int w, int b, int h, int d0) {
+    Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
+    return kv8_load8(p.x[w] + b * p.ldxb[w] + h * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
+  };
+  for (int i = cta * kDecWarps + warp; i < items; i += gridDim.x * kDecWarps) {
+    const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
+    if (len > 0 && lane < HD / 8)
+      *reinterpret_cast<uint4*>(p.c.tail_row(w, b, h, (len - 1) % kKvBlock) + 8 * lane) = row8(w, b, h, 8 * lane);
+  }
+  constexpr int kThreads = kDecWarps * 32, kVecs = kKvBlock * HD / 8 / kThreads;
+  for (int i = cta; i < items; i += gridDim.x) {
+    const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
+    if (len <= 0 || len % kKvBlock) continue;  // the same for the whole CTA
+    uint4 v[kVecs];
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
+      v[k] = r == kKvBlock - 1 ? row8(w, b, h, d0)
+                               : *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
+      m = fmaxf(m, kv8_amax8(v[k]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __syncthreads();
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    for (int k = 0; k < kDecWarps; ++k) m = fmaxf(m, red[k]);
+    const float scale = kv8_scale(m);
+    const int block = len / kKvBlock - 1;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
+      *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[k], scale);
+    }
+    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = scale;
+  }
+}
+
+template <int NT, int HD>
+__global__ void __launch_bounds__(kDecWarps * 32, 1)
+    kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv) {
+  using S = Kv8DecodeSmem<NT, HD>;
+  constexpr int kThreads = kDecWarps * 32;
+  __shared__ float red[kDecWarps];
+  __shared__ int s_flag, s_max;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
+  const uint32_t ring = base + warp * kDecSlots * S::kSlot, bars = base + S::kBar + warp * kDecSlots * 8;
+  int* s_len = reinterpret_cast<int*>(pp_smem + S::kLens);
+  int* s_pre = s_len + p.c.batch;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kDecSlots; ++i) mbar_init(bars + 8 * i, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  if (tid == 0) s_max = 0;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // lengths and the units before each sequence
+  const int group = p.nq / p.c.nkv;
+  for (int b = tid; b < p.c.batch; b += kThreads) {
+    int len = p.lens[b] + p.extra;
+    const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    bool ok = len <= p.c.cap;
+    if (p.rope.cos && len > 0 && cnt > 0) {
+      const int r = p.rope.pos[b];
+      ok = ok && r >= 0 && r <= p.rope.len - cnt;
+    }
+    if (!ok && blockIdx.x == 0 && p.status) atomicExch(p.status, 5);
+    s_len[b] = ok && cnt > 0 ? max(len, 0) : 0;
+  }
+  __syncthreads();
+  const Kv8Work work{s_len, s_pre, p.c.batch, p.c.nkv * p.tiles};
+  if (warp == 0) {
+    int sum = 0, mx = 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += 32) {
+      const int u = b0 + lane < p.c.batch ? Kv8Work::units(s_len[b0 + lane]) : 0;
+      mx = max(mx, u);
+      int x = u * work.per_seq;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (b0 + lane < p.c.batch) s_pre[b0 + lane + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) {
+      s_pre[0] = 0;
+      s_max = mx;
+    }
+  }
+  __syncthreads();
+
+  // rows without work
+  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x)
+    if (s_len[b] == 0)
+      for (int e = tid; e < p.n * p.nq * (HD / 8); e += kThreads) {
+        const int d0 = e % (HD / 8) * 8, h = e / (HD / 8) % p.nq, i = e / (HD / 8) / p.nq;
+        *reinterpret_cast<uint4*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d0) = make_uint4(0, 0, 0, 0);
+      }
+
+  // this CTA's share [a, z) of the units
+  const int total = s_pre[p.c.batch], ctas = gridDim.x;
+  const int per = max(kDecWarps, (total + ctas - 1) / ctas);
+  const int each = ctas / (p.c.batch * work.per_seq);           // CTAs per segment, if every one got as many
+  const bool aligned = each > 0 && (s_max + each - 1) / each <= per + per / 4;
+  auto pieces = [&](int U) { return min(each, (U + kDecWarps - 1) / kDecWarps); };
+  int a = 0, z = 0;
+  if (aligned) {
+    const int b = blockIdx.x / each / work.per_seq, j = blockIdx.x % each;
+    if (b < p.c.batch) {
+      const int U = Kv8Work::units(s_len[b]), k = pieces(U);
+      if (j < k) {
+        const int s0 = s_pre[b] + blockIdx.x / each % work.per_seq * U;
+        a = s0 + (int)((int64_t)U * j / k);
+        z = s0 + (int)((int64_t)U * (j + 1) / k);
+      }
+    }
+  } else {
+    a = min((int64_t)total, (int64_t)blockIdx.x * per);
+    z = min((int64_t)total, (int64_t)a + per);
+  }
+
+  // the ring's producer runs ahead over the warp's coded units
+  Kv8Cursor ahead{};
+  int ahead_idx = a + warp, issued = 0;
+  if (ahead_idx < z) ahead.seek(work, ahead_idx);
+  auto is_coded = [&](const Kv8Cursor& c) { return c.u < kv8_last_block(s_len[c.b]) * (kKvBlock / kDecUnit); };
+  bool fine = true;
+  auto issue_one = [&]() {
+    while (ahead_idx < z && !is_coded(ahead)) {
+      ahead_idx += kDecWarps;
+      if (ahead_idx < z) ahead.advance(work, kDecWarps);
+    }
+    if (ahead_idx >= z || !fine) return;
+    if (lane == 0) {
+      const int slot = issued % kDecSlots;
+      const uint32_t dst = ring + slot * S::kSlot;
+      const int y = (int)(p.c.head(ahead.b, ahead.seg / p.tiles) * p.c.cap) + ahead.u * kDecUnit;
+      mbar_expect_tx(bars + 8 * slot, S::kSlot);
+      tma_load_2d(dst, &tk, 0, y, bars + 8 * slot);
+      tma_load_2d(dst + S::kSide, &tv, 0, y, bars + 8 * slot);
+    }
+    ++issued;
+    ahead_idx += kDecWarps;
+    if (ahead_idx < z) ahead.advance(work, kDecWarps);
+  };
+#pragma unroll
+  for (int i = 0; i < kDecSlots; ++i) issue_one();
+
+  Kv8Cursor cur{};
+  int idx = a + warp, used = 0;
+  if (idx < z) cur.seek(work, idx);
+  Kv8Cursor seg{};  // the segment at hand, the same for all warps
+  if (a < z) seg.seek(work, a);
+  for (int at = a; at < z;) {
+    const int b = seg.b, kvh = seg.seg / p.tiles, tile = seg.seg % p.tiles;
+    const int seg0 = at - seg.u, seg1 = seg0 + seg.U, end = min(z, seg1);
+    const int len = s_len[b], last = kv8_last_block(len);
+    const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    const int row0 = tile * NT * 8, rows = min(NT * 8, p.n * group - row0);
+
+    // the tile's query rows (padding rows are zero) and the token, as FP16
+    for (int e = tid; e < NT * 8 * (HD / 8); e += kThreads) {
+      const int r = e / (HD / 8), d0 = e % (HD / 8) * 8;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int i = (row0 + r) / group, h = kvh * group + (row0 + r) % group;
+        if (i < cnt)
+          x = kv8_load8(p.q + b * p.ldqb + i * p.ldqt + h * p.ldqh, d0, HD, p.rope, p.rope.cos ? p.rope.pos[b] + i : 0);
+      }
+      uint2* dst = reinterpret_cast<uint2*>(pp_smem + S::kQ + r * S::kQRow + d0 * 2);
+      dst[0] = make_uint2(x.x, x.y);
+      dst[1] = make_uint2(x.z, x.w);
+    }
+    if (p.extra && tid < 2 * (HD / 8)) {
+      const int w = tid / (HD / 8), d0 = tid % (HD / 8) * 8;
+      const Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
+      *reinterpret_cast<uint4*>(pp_smem + S::kNew + w * HD * 2 + d0 * 2) =
+          kv8_load8(p.x[w] + b * p.ldxb[w] + kvh * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
+    }
+    __syncthreads();
+    uint32_t qb[NT][HD / 16][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint2 v = lds_u2(base + S::kQ + (nt * 8 + g) * S::kQRow + (16 * k + 4 * t4) * 2);
+        qb[nt][k][0] = v.x;
+        qb[nt][k][1] = v.y;
+      }
+    // first position that row (nt, j) does not attend
+    int stop[NT][2];
+    int min_stop = len;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = nt * 8 + 2 * t4 + j, i = (row0 + r) / group;
+        stop[nt][j] = r >= rows ? len : i < cnt ? len - cnt + i + 1 : 0;  // padding rows are zero queries
+        min_stop = min(min_stop, stop[nt][j]);
+      }
+
+    Kv8Acc<NT, HD> acc;
+    acc.clear();
+    float* score_rows = p.scores ? p.scores + ((int64_t)b * p.nq + kvh * group) * p.c.cap : nullptr;
+    for (; idx < end; idx += kDecWarps) {
+      float gain[NT][2];
+      if (is_coded(cur)) {
+        const int t0 = cur.u * kDecUnit;
+        const float ks = *p.c.scale(0, b, kvh, t0 / kKvBlock) * p.scale2, vs = *p.c.scale(1, b, kvh, t0 / kKvBlock);
+        const int slot = used % kDecSlots;
+        const uint32_t kt = ring + slot * S::kSlot, vt = kt + S::kSide;
+        if (fine) {
+          fine = mbar_wait_bounded(bars + 8 * slot, (used / kDecSlots) & 1, p.status);
+          ++used;
+        }
+        float s[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < HD / 16; k += 2) {
+            uint32_t r[4];
+            ldsm4(r, kt + tile_off<HD>(16 * mt + (lane & 15), k + (lane >> 4)));
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+              const uint32_t a0 = codes2<0x4140>(r[2 * kk]), a1 = codes2<0x4140>(r[2 * kk + 1]);
+              const uint32_t a2 = codes2<0x4342>(r[2 * kk]), a3 = codes2<0x4342>(r[2 * kk + 1]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_16816(s[mt][nt], a0, a1, a2, a3, qb[nt][k + kk][0], qb[nt][k + kk][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[mt][nt][e] *= ks;
+              if (t0 + kDecUnit > min_stop && t0 + 16 * mt + g + 8 * (e >> 1) >= stop[nt][e & 1])
+                s[mt][nt][e] = -INFINITY;
+            }
+        if (score_rows) {
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int h = nt * 8 + 2 * t4 + (e & 1);
+                if (h < rows) score_rows[(int64_t)h * p.c.cap + t0 + 16 * mt + g + 8 * (e >> 1)] = s[mt][nt][e];
+              }
+        }
+        uint32_t pb[2][NT][2];
+        kv8_softmax<NT, HD, 2>(acc, s, gain, pb);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) gain[nt][j] *= vs;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i += 2) {
+          float u[2][NT][4];
+#pragma unroll
+          for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) u[ii][nt][e] = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            uint32_t r[4];
+            ldsm4_t(r, vt + tile_off<HD>(16 * mt + (lane & 15), i + (lane >> 4)));
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii) {
+              const uint32_t a0 = codes2<0x4240>(r[2 * ii]), a1 = codes2<0x4341>(r[2 * ii]);
+              const uint32_t a2 = codes2<0x4240>(r[2 * ii + 1]), a3 = codes2<0x4341>(r[2 * ii + 1]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_16816(u[ii][nt], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+            }
+          }
+#pragma unroll
+          for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc.o[i + ii][nt][e] = fmaf(u[ii][nt][e], gain[nt][e & 1], acc.o[i + ii][nt][e]);
+        }
+        __syncwarp();  // the slot's rows are in registers
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        issue_one();
+      } else {
+        // 16 FP16 rows of the tail, straight from memory; rows past the end are zero
+        const int t0 = last * kKvBlock + (cur.u - last * (kKvBlock / kDecUnit)) * kDecTailUnit;
+        auto row = [&](int w, int t) -> const __half* {
+          if (p.extra && t == len - 1) return reinterpret_cast<const __half*>(pp_smem + S::kNew + w * HD * 2);
+          return t < len ? p.c.tail_row(w, b, kvh, t % kKvBlock) : nullptr;
+        };
+        float s[1][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][nt][e] = 0.f;
+        {
+          const __half *k0 = row(0, t0 + g), *k1 = row(0, t0 + g + 8);
+          uint2 x[HD / 16], y[HD / 16];
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            x[k] = k0 ? *reinterpret_cast<const uint2*>(k0 + 16 * k + 4 * t4) : make_uint2(0, 0);
+            y[k] = k1 ? *reinterpret_cast<const uint2*>(k1 + 16 * k + 4 * t4) : make_uint2(0, 0);
+          }
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + g + 8 * (e >> 1), h = nt * 8 + 2 * t4 + (e & 1);
+            s[0][nt][e] = t < stop[nt][e & 1] ? s[0][nt][e] * p.scale2 : -INFINITY;
+            if (score_rows && h < rows && t < len) score_rows[(int64_t)h * p.c.cap + t] = s[0][nt][e];
+          }
+        uint32_t pb[1][NT][2];
+        kv8_softmax<NT, HD, 1>(acc, s, gain, pb);
+        const __half *v0 = row(1, t0 + 2 * t4), *v1 = row(1, t0 + 2 * t4 + 1);
+        const __half *v2 = row(1, t0 + 2 * t4 + 8), *v3 = row(1, t0 + 2 * t4 + 9);
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const int d = 16 * i + 2 * g;
+          const uint32_t x0 = v0 ? ld_u32(v0 + d) : 0u, x1 = v1 ? ld_u32(v1 + d) : 0u;
+          const uint32_t x2 = v2 ? ld_u32(v2 + d) : 0u, x3 = v3 ? ld_u32(v3 + d) : 0u;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float u[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816(u, lo_pair(x0, x1), hi_pair(x0, x1), lo_pair(x2, x3), hi_pair(x2, x3), pb[0][nt][0], pb[0][nt][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc.o[i][nt][e] = fmaf(u[e], gain[nt][e & 1], acc.o[i][nt][e]);
+          }
+        }
+      }
+      if (idx + kDecWarps < z) cur.advance(work, kDecWarps);
+    }
+
+    // the warps' results, halves pairwise: lanes hold the same rows and dimensions
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float l = acc.l[nt][j];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        acc.l[nt][j] = l;
+      }
+#pragma unroll
+    for (int half = kDecWarps / 2; half > 0; half >>= 1) {
+      float* area = reinterpret_cast<float*>(pp_smem + S::kMerge + (warp % half) * S::kMergeWarp) + lane;
+      if (warp >= half && warp < 2 * half) {
+        float* f = area;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e, f += 32) *f = acc.o[i][nt][e];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j, f += 64) {
+            f[0] = acc.m[nt][j];
+            f[32] = acc.l[nt][j];
+          }
+      }
+      __syncthreads();
+      if (warp < half) {
+        float fa[NT][2];
+        const float* f = area + HD / 16 * NT * 4 * 32;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j, f += 64) {
+            const float m2 = f[0], l2 = f[32];
+            if (m2 > acc.m[nt][j]) acc.rebase(nt, j, m2);
+            fa[nt][j] = m2 == -INFINITY ? 0.f : ex2(m2 - acc.m[nt][j]);
+            acc.l[nt][j] = m2 == -INFINITY ? acc.l[nt][j] + l2 : fmaf(l2, fa[nt][j], acc.l[nt][j]);
+          }
+        f = area;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e, f += 32) acc.o[i][nt][e] = fmaf(*f, fa[nt][e & 1], acc.o[i][nt][e]);
+      }
+      __syncthreads();
+    }
+
+    const int segment = b * work.per_seq + seg.seg;
+    auto store = [&](int r, int d, float x, float y) {  // two dimensions of row r
+      const int i = (row0 + r) / group, h = kvh * group + (row0 + r) % group;
+      *reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d) = __floats2half2_rn(x, y);
+    };
+    if (at == seg0 && end == seg1) {
+      if (warp == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = nt * 8 + 2 * t4 + j;
+            if (r >= rows) continue;
+            const float l = acc.l[nt][j], inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+              store(r, 16 * i + 2 * g, acc.o[i][nt][j] * inv, acc.o[i][nt][2 + j] * inv);
+            if (p.scores && g == 0) p.lse[b * p.nq + kvh * group + r] = acc.m[nt][j] + log2f(l);
+          }
+      }
+    } else {
+      constexpr int kPart = kv8_part_floats(NT, HD);
+      if (warp == 0) {
+        float* rec = p.part + ((int64_t)blockIdx.x * 2 + (a >= seg0 ? 0 : 1)) * kPart;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = nt * 8 + 2 * t4 + j;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+              *reinterpret_cast<float2*>(rec + r * HD + 16 * i + 2 * g) =
+                  make_float2(acc.o[i][nt][j], acc.o[i][nt][2 + j]);
+            if (g == 0)
+              *reinterpret_cast<float2*>(rec + NT * 8 * HD + 2 * r) = make_float2(acc.m[nt][j], acc.l[nt][j]);
+          }
+        __threadfence();
+        __syncwarp();
+      }
+      // the last CTA of the segment to arrive adds up the partials in order
+      const int first = aligned ? segment * each : seg0 / per;
+      const int contrib = aligned ? pieces(seg.U) : (seg1 - 1) / per - first + 1;
+      if (tid == 0) {
+        const int n = atomicAdd(p.cnt + first, 1);  // at most one segment goes on past a CTA's share
+        s_flag = n == contrib - 1;
+        if (s_flag) {
+          p.cnt[first] = 0;
+          __threadfence();
+        }
+      }
+      __syncthreads();
+      if (s_flag) {
+        auto rec = [&](int k) {
+          return p.part + ((int64_t)(first + k) * 2 + (aligned || (first + k) * (int64_t)per >= seg0 ? 0 : 1)) * kPart;
+        };
+        for (int e = tid; e < rows * (HD / 4); e += kThreads) {
+          const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+          float m = -INFINITY;
+#pragma unroll 4
+          for (int k = 0; k < contrib; ++k) m = fmaxf(m, __ldcg(rec(k) + NT * 8 * HD + 2 * r));
+          float l = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int k = 0; k < contrib; ++k) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec(k) + NT * 8 * HD + 2 * r));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec(k) + r * HD + d));
+            const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - m);  // a NaN in an empty row's sums stays one
+            l = fmaf(ml.y, f, l);
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
+            o.z = fmaf(x.z, f, o.z);
+            o.w = fmaf(x.w, f, o.w);
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          store(r, d, o.x * inv, o.y * inv);
+          store(r, d + 2, o.z * inv, o.w * inv);
+          if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
+        }
+      }
+      __syncthreads();
+    }
+    at = end;
+    if (at < z) seg.advance(work, seg.U - seg.u);
+  }
+  if (!fine)  // a copy did not arrive in time (status 1): leave none in flight
+    for (; used < issued; ++used) mbar_wait_bounded(bars + 8 * (used % kDecSlots), (used / kDecSlots) & 1, p.status);
+  if (p.extra) kv8_store_token<HD>(p, s_len, red);
+}
+
+// weights[b][g][t] += sum of the group's exp2(score - lse).
+struct Kv8WeightsParams {
+  const float* scores;
+  const float* lse;
+  float* weights;
+  const int* lens;
+  const Kv8Rope rope;
+  int extra, nq, nkv, cap;
+};
+
+__global__ void __launch_bounds__(256) kv8_weights_kernel(const Kv8WeightsParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.z, kvh = blockIdx.y, group = p.nq / p.nkv;
+  const int len = p.lens[b] + p.extra;
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (len > p.cap || t >= len) return;
+  if (p.rope.cos && (p.rope.pos[b] < 0 || p.rope.pos[b] >= p.rope.len)) return;
+  const float* s = p.scores + ((int64_t)b * p.nq + kvh * group) * p.cap + t;
+  const float* l = p.lse + b * p.nq + kvh * group;
+  float w = 0.f;
+#pragma unroll 4
+  for (int h = 0; h < group; ++h) w += ex2(s[(int64_t)h * p.cap] - l[h]);
+  p.weights[((int64_t)b * p.nkv + kvh) * p.cap + t] += w;
+}
+
+}  // namespace pp

@@ -98,6 +98,25 @@ class KV8Cache:
 
 
 _strides: dict = {}
+_scratch: dict = {}
+_scratch_kept: list = []
+
+
+def _workspace(cache: KV8Cache, nbytes: int) -> torch.Tensor:
+    """Zero-filled scratch of the attention calls, one per (device, stream); the
+    kernels leave its counters at zero.  An outgrown buffer is kept, since a
+    captured graph may refer to it.  A capture that needs a new one gets its
+    own, whose fill is part of the graph."""
+    key = (cache.device.index, _lib.stream_handle(cache.device))
+    buf = _scratch.get(key)
+    if buf is None or buf.numel() < nbytes:
+        new = torch.zeros(max(nbytes, 1 << 20) * 5 // 4, dtype=torch.uint8, device=cache.device)
+        if torch.cuda.is_current_stream_capturing():
+            return new
+        if buf is not None:
+            _scratch_kept.append(buf)
+        buf = _scratch[key] = new
+    return buf
 
 
 def _c_strides(*s: int):
@@ -217,7 +236,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, counts: 
     shape = (cache.batch, n, nq, cache.head_dim)
     q = _rows(q, "q", shape, cache)
     out = _output(out, shape, cache)
-    ws = _lib.workspace(cache.device, cache.workspace_bytes(n, nq, False))
+    ws = _workspace(cache, cache.workspace_bytes(n, nq, False))
     _call(cache, "pp_kv8_attention", q.data_ptr(), _c_strides(*q.stride()[:3]), n, nq, _ints(lens, "lens", cache),
           _ints(counts, "counts", cache), 1 / math.sqrt(cache.head_dim) if scale is None else scale, out.data_ptr(),
           _c_strides(*out.stride()[:3]), *_rope(rope, cache), ws.data_ptr(), ws.numel())
@@ -242,7 +261,7 @@ def kv8_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV8Cach
     q = _rows(q, "q", (b, nq, hd), cache)
     k, v = _rows(k, "k", (b, cache.kv_heads, hd), cache), _rows(v, "v", (b, cache.kv_heads, hd), cache)
     out = _output(out, (b, nq, hd), cache)
-    ws = _lib.workspace(cache.device, cache.workspace_bytes(1, nq, weights is not None))
+    ws = _workspace(cache, cache.workspace_bytes(1, nq, weights is not None))
     _call(cache, "pp_kv8_decode", q.data_ptr(), _c_strides(*q.stride()[:2]), nq, k.data_ptr(),
           _c_strides(*k.stride()[:2]), v.data_ptr(), _c_strides(*v.stride()[:2]), _ints(pos, "pos", cache),
           1 / math.sqrt(hd) if scale is None else scale, _weights(weights, "weights", cache), out.data_ptr(),
