@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kTile) kv8_attention_kernel(const AttnParams p
 // How a call with `rows` query rows per kv head runs on kv8_decode_kernel:
 // tiles of 8 rows while one is enough, else of 16.
 constexpr int kDecodeRows = 64;
+constexpr int kDecodeBatch = 512;
 
 struct DecodePlan {
   int nt, tiles, ctas;
@@ -172,10 +173,10 @@ int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
   CUtensorMap tm[2];
   const uint64_t rows = (uint64_t)p.c.batch * p.c.nkv * p.c.cap;
   for (int w = 0; w < 2; ++w)
-    if (int rc = encode_tmap_2d(&tm[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.c.codes[w], HD, rows, HD, HD, kDecUnit,
+    if (int rc = encode_tmap_2d(&tm[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.c.codes[w], HD, rows, HD, HD, kKvBlock,
                                 HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return rc;
-  return launch_kernel("kv8_decode_kernel", launch_overlap(), kern, dim3((unsigned)ctas), dim3(kDecWarps * 32),
+  return launch_kernel("kv8_decode_kernel", launch_overlap(), kern, dim3((unsigned)ctas), dim3(kv8_warps(NT) * 32),
                        (size_t)smem, s, p, tm[0], tm[1]);
 }
 
@@ -223,12 +224,35 @@ int run_decode(const char* who, Kv8DecodeParams& p, float* weights, void* worksp
     p.lse = reinterpret_cast<float*>(ws + d.lse);
     p.scores = reinterpret_cast<float*>(ws + d.scores);
   }
-  const int rc = p.c.hd == 128 ? (d.nt == 1 ? launch_decode<1, 128>(p, ctas, s) : launch_decode<2, 128>(p, ctas, s))
-                               : (d.nt == 1 ? launch_decode<1, 64>(p, ctas, s) : launch_decode<2, 64>(p, ctas, s));
-  if (rc || !weights) return rc;
-  const Kv8WeightsParams w{p.scores, p.lse, weights, p.lens, p.rope, p.extra, p.nq, p.c.nkv, p.c.cap};
+  // a launch keeps its sequences' lengths in shared memory: larger batches go in parts
+  const Kv8DecodeParams all = p;
+  for (int b0 = 0; b0 < all.c.batch; b0 += kDecodeBatch) {
+    const int64_t heads = (int64_t)b0 * all.c.nkv;
+    p.c.batch = all.c.batch - b0 < kDecodeBatch ? all.c.batch - b0 : kDecodeBatch;
+    for (int w = 0; w < 2; ++w) {
+      p.c.codes[w] = all.c.codes[w] + heads * all.c.cap * all.c.hd;
+      p.c.scales[w] = all.c.scales[w] + heads * (all.c.cap / kKvBlock);
+      p.c.tail[w] = all.c.tail[w] + heads * kKvBlock * all.c.hd;
+      p.x[w] = all.x[w] ? all.x[w] + b0 * all.ldxb[w] : nullptr;
+    }
+    p.q = all.q + b0 * all.ldqb;
+    p.out = all.out + b0 * all.ldob;
+    p.lens = all.lens + b0;
+    p.counts = all.counts ? all.counts + b0 : nullptr;
+    p.rope.pos = all.rope.pos ? all.rope.pos + b0 : nullptr;
+    if (weights) {
+      p.lse = all.lse + (int64_t)b0 * all.nq;
+      p.scores = all.scores + (int64_t)b0 * all.nq * all.c.cap;
+    }
+    if (int rc = p.c.hd == 128 ? (d.nt == 1 ? launch_decode<1, 128>(p, ctas, s) : launch_decode<2, 128>(p, ctas, s))
+                               : (d.nt == 1 ? launch_decode<1, 64>(p, ctas, s) : launch_decode<2, 64>(p, ctas, s)))
+      return rc;
+  }
+  if (!weights) return PP_OK;
+  const Kv8WeightsParams w{all.scores, all.lse, weights, all.lens, all.rope, all.extra, all.nq, all.c.nkv, all.c.cap};
   return launch_kernel("kv8_weights_kernel", launch_overlap(), kv8_weights_kernel,
-                       dim3((unsigned)cdiv(p.c.cap, 256), (unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(256), 0, s, w);
+                       dim3((unsigned)cdiv(all.c.cap, 256), (unsigned)all.c.nkv, (unsigned)all.c.batch), dim3(256), 0, s,
+                       w);
 }
 
 }  // namespace

@@ -8,26 +8,28 @@
 // own unit's maximum m (2^-11 of values up to 1), everything else is FP32.
 //
 // Bound: the cache's bytes at long lengths, latency at short ones.  Work is
-// counted in units, 32 positions of codes or 16 FP16 rows of the tail, over
-// all (sequence, kv head, row tile) segments in a row, and each CTA takes an
-// equal share of them, so ragged batches balance; where the segments divide
-// the GPU nearly evenly, no share spans two of them.  The shares come from the
-// lengths in device memory.  A warp has a ring of units that arrive by
-// swizzled TMA boxes, two in flight; keys are the A operand of m16n8k16 (16
-// positions x 8 rows), read by ldmatrix with the four dimensions of a lane's
-// word as its k elements, values by transposed ldmatrix, whose word holds two
-// dimensions at two positions: both orders cost nothing, since the queries and
-// the outputs take the same permutation.
+// counted in units, a block of codes or 16 FP16 rows of the tail, over all
+// (sequence, kv head, row tile) segments in a row, and each CTA takes an equal
+// share of them, so ragged batches balance; where the segments divide the GPU
+// nearly evenly, no share spans two of them.  The shares come from the lengths
+// in device memory.  A warp holds one block, keys and values apart, each
+// arriving by a swizzled TMA box; the next block's keys are on their way while
+// it works on the values, and the other way round.  Keys are the A operand of
+// m16n8k16 (16 positions x 8 rows), read by ldmatrix with the four dimensions
+// of a lane's word as its k elements, values by transposed ldmatrix, whose
+// word holds two dimensions at two positions: both orders cost nothing, since
+// the queries and the outputs take the same permutation.
 #pragma once
 
 #include "kv8.cuh"
 
 namespace pp {
 
-constexpr int kDecWarps = 8;
-constexpr int kDecSlots = 2;   // units in flight per warp: 128 KB per SM at head_dim 128
-constexpr int kDecUnit = 32;   // positions of a coded unit
-constexpr int kDecTailUnit = 16;
+constexpr int kDecTailUnit = 16;  // FP16 rows of a tail unit; a coded unit is a block
+
+// Warps of a CTA (one CTA per SM): 12 while a row tile is 8 rows, 8 warps with
+// twice the accumulators for 16 rows.
+constexpr int kv8_warps(int nt) { return nt == 1 ? 12 : 8; }
 
 struct Kv8DecodeParams {
   Kv8Cache c;
@@ -52,16 +54,17 @@ struct Kv8DecodeParams {
 
 template <int NT, int HD>
 struct Kv8DecodeSmem {
-  static constexpr int kSide = kDecUnit * HD;                    // a unit's keys or values
-  static constexpr int kSlot = 2 * kSide;
-  static constexpr int kRing = kDecWarps * kDecSlots * kSlot;
-  static constexpr int kMerge = kRing;                           // half the warps' results
-  static constexpr int kMergeWarp = (HD / 16 * NT * 4 + NT * 4) * 32 * 4;
-  static constexpr int kQ = kMerge + kDecWarps / 2 * kMergeWarp; // query rows, then the token's key and value
-  static constexpr int kQRow = HD * 2 + 32;  // conflict-free 8-byte reads of eight rows
+  static constexpr int kWarps = kv8_warps(NT);
+  static constexpr int kSlot = kKvBlock * HD;                    // a block's keys or values
+  static constexpr int kRounds = NT == 1 ? 2 : 1;                // the warps' results are added up in as many parts
+  static constexpr int kPart = HD / 16 / kRounds * NT * 4;       // floats a lane contributes to one
+  static constexpr int kMerge = kWarps * 2 * kSlot;
+  static constexpr int kMl = kMerge + kWarps * kPart * 32 * 4;   // each warp's row maxima and sums
+  static constexpr int kQ = kMl + kWarps * NT * 8 * 8;           // query rows, then the token's key and value
+  static constexpr int kQRow = HD * 2 + 32;                      // conflict-free 8-byte reads of eight rows
   static constexpr int kNew = kQ + NT * 8 * kQRow;
   static constexpr int kBar = kNew + 2 * HD * 2;
-  static constexpr int kLens = kBar + kDecWarps * kDecSlots * 8; // lengths, then unit prefix
+  static constexpr int kLens = kBar + kWarps * 2 * 8;            // lengths, then unit prefix
   static constexpr int bytes(int batch) { return kLens + (2 * batch + 2) * 4; }
 };
 
@@ -92,6 +95,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// D = A B + 0.
+__device__ __forceinline__ void mma_16816_0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Two codes of a word as FP16 integers code - 128: the byte in the low half of
 // 0x6400 is 1024 + code, exactly.
 template <int SEL>
@@ -100,7 +112,8 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 }
 
 // Byte offset of 16-byte chunk c of row r in a swizzled tile (128-byte or
-// 64-byte rows, as the tensor maps of launch_decode order them).
+// 64-byte rows, as the tensor maps of launch_decode order them).  For an even
+// k, chunk k + c (c = 0, 1) lies at the offset of chunk c xor 16 k.
 template <int HD>
 __device__ __forceinline__ uint32_t tile_off(int r, int c) {
   return HD == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
@@ -201,7 +214,7 @@ struct Kv8Work {
   __device__ __forceinline__ static int units(int len) {
     if (len <= 0) return 0;
     const int last = kv8_last_block(len);
-    return last * (kKvBlock / kDecUnit) + (len - last * kKvBlock + kDecTailUnit - 1) / kDecTailUnit;
+    return last + (len - last * kKvBlock + kDecTailUnit - 1) / kDecTailUnit;
   }
 };
 
@@ -220,24 +233,20 @@ struct Kv8Cursor {
     seg = (idx - w.pre[b]) / U;
     u = idx - w.pre[b] - seg * U;
   }
-  // idx must stay below the total.
-  __device__ __forceinline__ void advance(const Kv8Work& w, int by) {
-    u += by;
-    while (u >= U) {
-      u -= U;
-      if (++seg == w.per_seq) {
-        seg = 0;
-        do ++b;
-        while (w.pre[b + 1] == w.pre[b]);
-        U = Kv8Work::units(w.len[b]);
-      }
-    }
+  // To the start of the next segment, which must exist.
+  __device__ __forceinline__ void next(const Kv8Work& w) {
+    u = 0;
+    if (++seg < w.per_seq) return;
+    seg = 0;
+    do ++b;
+    while (w.pre[b + 1] == w.pre[b]);
+    U = Kv8Work::units(w.len[b]);
   }
 };
 
 // The blocks of the cache that a token completes, and the token's own row in
 // the tail: nothing that attends in this launch reads either.
-template <int HD>
+template <int HD, int WARPS>
 __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const int* s_len, float* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int items = p.c.batch * p.c.nkv * 2;
@@ -246,12 +255,12 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
     Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
     return kv8_load8(p.x[w] + b * p.ldxb[w] + h * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
   };
-  for (int i = cta * kDecWarps + warp; i < items; i += gridDim.x * kDecWarps) {
+  for (int i = cta * WARPS + warp; i < items; i += gridDim.x * WARPS) {
     const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
     if (len > 0 && lane < HD / 8)
       *reinterpret_cast<uint4*>(p.c.tail_row(w, b, h, (len - 1) % kKvBlock) + 8 * lane) = row8(w, b, h, 8 * lane);
   }
-  constexpr int kThreads = kDecWarps * 32, kVecs = kKvBlock * HD / 8 / kThreads;
+  constexpr int kThreads = WARPS * 32, kItems = kKvBlock * HD / 8, kVecs = (kItems + kThreads - 1) / kThreads;
   for (int i = cta; i < items; i += gridDim.x) {
     const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
     if (len <= 0 || len % kKvBlock) continue;  // the same for the whole CTA
@@ -260,8 +269,9 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      v[k] = r == kKvBlock - 1 ? row8(w, b, h, d0)
-                               : *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
+      v[k] = e >= kItems ? make_uint4(0, 0, 0, 0)
+             : r == kKvBlock - 1 ? row8(w, b, h, d0)
+                                 : *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
       m = fmaxf(m, kv8_amax8(v[k]));
     }
 #pragma unroll
@@ -269,53 +279,54 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
     __syncthreads();
     if (lane == 0) red[warp] = m;
     __syncthreads();
-    for (int k = 0; k < kDecWarps; ++k) m = fmaxf(m, red[k]);
+    for (int k = 0; k < WARPS; ++k) m = fmaxf(m, red[k]);
     const float scale = kv8_scale(m);
     const int block = len / kKvBlock - 1;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[k], scale);
+      if (e < kItems)
+        *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[k], scale);
     }
     if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = scale;
   }
 }
 
 template <int NT, int HD>
-__global__ void __launch_bounds__(kDecWarps * 32, 1)
+__global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
   using S = Kv8DecodeSmem<NT, HD>;
-  constexpr int kThreads = kDecWarps * 32;
-  __shared__ float red[kDecWarps];
+  constexpr int kWarps = S::kWarps, kThreads = kWarps * 32, kPartFloats = kv8_part_floats(NT, HD);
+  __shared__ float red[kWarps];
   __shared__ int s_flag, s_max;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
-  const uint32_t ring = base + warp * kDecSlots * S::kSlot, bars = base + S::kBar + warp * kDecSlots * 8;
+  const uint32_t k_slot = base + warp * 2 * S::kSlot, v_slot = k_slot + S::kSlot;
+  const uint32_t k_bar = base + S::kBar + warp * 16, v_bar = k_bar + 8;
   int* s_len = reinterpret_cast<int*>(pp_smem + S::kLens);
   int* s_pre = s_len + p.c.batch;
   if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < kDecSlots; ++i) mbar_init(bars + 8 * i, 1);
+    mbar_init(k_bar, 1);
+    mbar_init(v_bar, 1);
     fence_mbar_init();
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
   }
-  if (tid == 0) s_max = 0;
   pdl_launch_dependents();
   pdl_wait();
 
   // lengths and the units before each sequence
   const int group = p.nq / p.c.nkv;
   for (int b = tid; b < p.c.batch; b += kThreads) {
-    int len = p.lens[b] + p.extra;
+    const int len = p.lens[b] + p.extra;
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
     bool ok = len <= p.c.cap;
     if (p.rope.cos && len > 0 && cnt > 0) {
       const int r = p.rope.pos[b];
       ok = ok && r >= 0 && r <= p.rope.len - cnt;
     }
-    if (!ok && blockIdx.x == 0 && p.status) atomicExch(p.status, 5);
+    if (!ok && blockIdx.x == 0) atomicExch(p.status, 5);
     s_len[b] = ok && cnt > 0 ? max(len, 0) : 0;
   }
   __syncthreads();
@@ -342,27 +353,19 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
   }
   __syncthreads();
 
-  // rows without work
-  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x)
-    if (s_len[b] == 0)
-      for (int e = tid; e < p.n * p.nq * (HD / 8); e += kThreads) {
-        const int d0 = e % (HD / 8) * 8, h = e / (HD / 8) % p.nq, i = e / (HD / 8) / p.nq;
-        *reinterpret_cast<uint4*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d0) = make_uint4(0, 0, 0, 0);
-      }
-
   // this CTA's share [a, z) of the units
   const int total = s_pre[p.c.batch], ctas = gridDim.x;
-  const int per = max(kDecWarps, (total + ctas - 1) / ctas);
-  const int each = ctas / (p.c.batch * work.per_seq);           // CTAs per segment, if every one got as many
+  const int per = max(kWarps, (total + ctas - 1) / ctas);
+  const int each = ctas / (p.c.batch * work.per_seq);  // CTAs per segment, if every one got as many
   const bool aligned = each > 0 && (s_max + each - 1) / each <= per + per / 4;
-  auto pieces = [&](int U) { return min(each, (U + kDecWarps - 1) / kDecWarps); };
+  auto pieces = [&](int U) { return min(each, (U + kWarps - 1) / kWarps); };
   int a = 0, z = 0;
   if (aligned) {
-    const int b = blockIdx.x / each / work.per_seq, j = blockIdx.x % each;
+    const int s = blockIdx.x / each, b = s / work.per_seq, j = blockIdx.x % each;
     if (b < p.c.batch) {
       const int U = Kv8Work::units(s_len[b]), k = pieces(U);
       if (j < k) {
-        const int s0 = s_pre[b] + blockIdx.x / each % work.per_seq * U;
+        const int s0 = s_pre[b] + s % work.per_seq * U;
         a = s0 + (int)((int64_t)U * j / k);
         z = s0 + (int)((int64_t)U * (j + 1) / k);
       }
@@ -372,42 +375,45 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
     z = min((int64_t)total, (int64_t)a + per);
   }
 
-  // the ring's producer runs ahead over the warp's coded units
-  Kv8Cursor ahead{};
-  int ahead_idx = a + warp, issued = 0;
-  if (ahead_idx < z) ahead.seek(work, ahead_idx);
-  auto is_coded = [&](const Kv8Cursor& c) { return c.u < kv8_last_block(s_len[c.b]) * (kKvBlock / kDecUnit); };
+  // Warp w takes units a + w, a + w + kWarps, ... of the share.
   bool fine = true;
-  auto issue_one = [&]() {
-    while (ahead_idx < z && !is_coded(ahead)) {
-      ahead_idx += kDecWarps;
-      if (ahead_idx < z) ahead.advance(work, kDecWarps);
+  auto load = [&](const CUtensorMap* tm, uint32_t dst, uint32_t bar, int row) {
+    if (lane == 0 && fine) {
+      mbar_expect_tx(bar, S::kSlot);
+      tma_load_2d(dst, tm, 0, row, bar);
     }
-    if (ahead_idx >= z || !fine) return;
-    if (lane == 0) {
-      const int slot = issued % kDecSlots;
-      const uint32_t dst = ring + slot * S::kSlot;
-      const int y = (int)(p.c.head(ahead.b, ahead.seg / p.tiles) * p.c.cap) + ahead.u * kDecUnit;
-      mbar_expect_tx(bars + 8 * slot, S::kSlot);
-      tma_load_2d(dst, &tk, 0, y, bars + 8 * slot);
-      tma_load_2d(dst + S::kSide, &tv, 0, y, bars + 8 * slot);
-    }
-    ++issued;
-    ahead_idx += kDecWarps;
-    if (ahead_idx < z) ahead.advance(work, kDecWarps);
   };
-#pragma unroll
-  for (int i = 0; i < kDecSlots; ++i) issue_one();
+  int idx = a + warp, phase = 0;
+  Kv8Cursor seg{};
+  int seg_row = 0;  // the segment's first row of the tensor maps
+  auto enter = [&](int from, int to) {  // starts the warp's first block of the segment of units [from, to)
+    const int tile_head = p.tiles == 1 ? seg.seg : seg.seg / p.tiles;
+    seg_row = (int)(p.c.head(seg.b, tile_head) * p.c.cap);
+    const int u = idx - from;
+    if (idx < min(z, to) && u < kv8_last_block(s_len[seg.b])) {
+      load(&tk, k_slot, k_bar, seg_row + u * kKvBlock);
+      load(&tv, v_slot, v_bar, seg_row + u * kKvBlock);
+    }
+  };
+  if (a < z) {
+    seg.seek(work, a);
+    enter(a - seg.u, a - seg.u + seg.U);
+  }
 
-  Kv8Cursor cur{};
-  int idx = a + warp, used = 0;
-  if (idx < z) cur.seek(work, idx);
-  Kv8Cursor seg{};  // the segment at hand, the same for all warps
-  if (a < z) seg.seek(work, a);
+  // rows without work
+  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x)
+    if (s_len[b] == 0)
+      for (int e = tid; e < p.n * p.nq * (HD / 8); e += kThreads) {
+        const int d0 = e % (HD / 8) * 8, h = e / (HD / 8) % p.nq, i = e / (HD / 8) / p.nq;
+        *reinterpret_cast<uint4*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d0) = make_uint4(0, 0, 0, 0);
+      }
+
+  const uint32_t lane_off = tile_off<HD>(lane & 15, lane >> 4);
   for (int at = a; at < z;) {
-    const int b = seg.b, kvh = seg.seg / p.tiles, tile = seg.seg % p.tiles;
-    const int seg0 = at - seg.u, seg1 = seg0 + seg.U, end = min(z, seg1);
-    const int len = s_len[b], last = kv8_last_block(len);
+    const int b = seg.b, row_base = seg_row, segment = seg.b * work.per_seq + seg.seg;
+    const int kvh = p.tiles == 1 ? seg.seg : seg.seg / p.tiles, tile = p.tiles == 1 ? 0 : seg.seg % p.tiles;
+    const int seg0 = at - seg.u, U = seg.U, seg1 = seg0 + U, end = min(z, seg1);
+    const int len = s_len[b], coded = kv8_last_block(len);
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
     const int row0 = tile * NT * 8, rows = min(NT * 8, p.n * group - row0);
 
@@ -424,22 +430,12 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
       dst[0] = make_uint2(x.x, x.y);
       dst[1] = make_uint2(x.z, x.w);
     }
-    if (p.extra && tid < 2 * (HD / 8)) {
-      const int w = tid / (HD / 8), d0 = tid % (HD / 8) * 8;
+    if (p.extra && tid >= kThreads - 2 * (HD / 8)) {
+      const int e = kThreads - 1 - tid, w = e / (HD / 8), d0 = e % (HD / 8) * 8;
       const Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
       *reinterpret_cast<uint4*>(pp_smem + S::kNew + w * HD * 2 + d0 * 2) =
           kv8_load8(p.x[w] + b * p.ldxb[w] + kvh * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
     }
-    __syncthreads();
-    uint32_t qb[NT][HD / 16][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        const uint2 v = lds_u2(base + S::kQ + (nt * 8 + g) * S::kQRow + (16 * k + 4 * t4) * 2);
-        qb[nt][k][0] = v.x;
-        qb[nt][k][1] = v.y;
-      }
     // first position that row (nt, j) does not attend
     int stop[NT][2];
     int min_stop = len;
@@ -451,156 +447,203 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
         stop[nt][j] = r >= rows ? len : i < cnt ? len - cnt + i + 1 : 0;  // padding rows are zero queries
         min_stop = min(min_stop, stop[nt][j]);
       }
+    const float *k_scale = p.c.scale(0, b, kvh, 0), *v_scale = p.c.scale(1, b, kvh, 0);
+    float ks = 0.f, vs = 0.f;  // of the warp's next block
+    if (idx < end && idx - seg0 < coded) {
+      ks = k_scale[idx - seg0];
+      vs = v_scale[idx - seg0];
+    }
+    __syncthreads();
+    uint32_t qb[NT][HD / 16][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const uint2 v = lds_u2(base + S::kQ + (nt * 8 + g) * S::kQRow + (16 * k + 4 * t4) * 2);
+        qb[nt][k][0] = v.x;
+        qb[nt][k][1] = v.y;
+      }
 
     Kv8Acc<NT, HD> acc;
     acc.clear();
     float* score_rows = p.scores ? p.scores + ((int64_t)b * p.nq + kvh * group) * p.c.cap : nullptr;
-    for (; idx < end; idx += kDecWarps) {
-      float gain[NT][2];
-      if (is_coded(cur)) {
-        const int t0 = cur.u * kDecUnit;
-        const float ks = *p.c.scale(0, b, kvh, t0 / kKvBlock) * p.scale2, vs = *p.c.scale(1, b, kvh, t0 / kKvBlock);
-        const int slot = used % kDecSlots;
-        const uint32_t kt = ring + slot * S::kSlot, vt = kt + S::kSide;
-        if (fine) {
-          fine = mbar_wait_bounded(bars + 8 * slot, (used / kDecSlots) & 1, p.status);
-          ++used;
-        }
-        float s[2][NT][4];
+    int u = idx - seg0;
+    const int u_end = end - seg0, coded_end = min(u_end, coded);
+#pragma unroll 1
+    for (; u < coded_end; u += kWarps) {
+      constexpr int MT = kKvBlock / 16;
+      const int t0 = u * kKvBlock;
+      const bool more = u + kWarps < coded_end;
+      const float ks2 = ks * p.scale2, vs1 = vs;
+      if (more) {
+        ks = k_scale[u + kWarps];
+        vs = v_scale[u + kWarps];
+      }
+      if (fine && !mbar_wait_bounded(k_bar, phase, p.status)) {  // status 1; nothing stays in flight
+        fine = false;
+        mbar_wait_bounded(k_bar, phase, p.status);
+        mbar_wait_bounded(v_bar, phase, p.status);
+      }
+      float s[MT][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int k = 0; k < HD / 16; k += 2) {
+          uint32_t r[4];
+          ldsm4(r, (k_slot + mt * 16 * HD) + (lane_off ^ (k << 4)));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
-#pragma unroll
-          for (int k = 0; k < HD / 16; k += 2) {
-            uint32_t r[4];
-            ldsm4(r, kt + tile_off<HD>(16 * mt + (lane & 15), k + (lane >> 4)));
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-              const uint32_t a0 = codes2<0x4140>(r[2 * kk]), a1 = codes2<0x4140>(r[2 * kk + 1]);
-              const uint32_t a2 = codes2<0x4342>(r[2 * kk]), a3 = codes2<0x4342>(r[2 * kk + 1]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_16816(s[mt][nt], a0, a1, a2, a3, qb[nt][k + kk][0], qb[nt][k + kk][1]);
-            }
-          }
-        }
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[mt][nt][e] *= ks;
-              if (t0 + kDecUnit > min_stop && t0 + 16 * mt + g + 8 * (e >> 1) >= stop[nt][e & 1])
-                s[mt][nt][e] = -INFINITY;
-            }
-        if (score_rows) {
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int kk = 0; kk < 2; ++kk) {
+            const uint32_t a0 = codes2<0x4140>(r[2 * kk]), a1 = codes2<0x4140>(r[2 * kk + 1]);
+            const uint32_t a2 = codes2<0x4342>(r[2 * kk]), a3 = codes2<0x4342>(r[2 * kk + 1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int h = nt * 8 + 2 * t4 + (e & 1);
-                if (h < rows) score_rows[(int64_t)h * p.c.cap + t0 + 16 * mt + g + 8 * (e >> 1)] = s[mt][nt][e];
-              }
-        }
-        uint32_t pb[2][NT][2];
-        kv8_softmax<NT, HD, 2>(acc, s, gain, pb);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) gain[nt][j] *= vs;
-#pragma unroll
-        for (int i = 0; i < HD / 16; i += 2) {
-          float u[2][NT][4];
-#pragma unroll
-          for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) u[ii][nt][e] = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            uint32_t r[4];
-            ldsm4_t(r, vt + tile_off<HD>(16 * mt + (lane & 15), i + (lane >> 4)));
-#pragma unroll
-            for (int ii = 0; ii < 2; ++ii) {
-              const uint32_t a0 = codes2<0x4240>(r[2 * ii]), a1 = codes2<0x4341>(r[2 * ii]);
-              const uint32_t a2 = codes2<0x4240>(r[2 * ii + 1]), a3 = codes2<0x4341>(r[2 * ii + 1]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_16816(u[ii][nt], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
-            }
-          }
-#pragma unroll
-          for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                acc.o[i + ii][nt][e] = fmaf(u[ii][nt][e], gain[nt][e & 1], acc.o[i + ii][nt][e]);
-        }
-        __syncwarp();  // the slot's rows are in registers
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        issue_one();
-      } else {
-        // 16 FP16 rows of the tail, straight from memory; rows past the end are zero
-        const int t0 = last * kKvBlock + (cur.u - last * (kKvBlock / kDecUnit)) * kDecTailUnit;
-        auto row = [&](int w, int t) -> const __half* {
-          if (p.extra && t == len - 1) return reinterpret_cast<const __half*>(pp_smem + S::kNew + w * HD * 2);
-          return t < len ? p.c.tail_row(w, b, kvh, t % kKvBlock) : nullptr;
-        };
-        float s[1][NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][nt][e] = 0.f;
-        {
-          const __half *k0 = row(0, t0 + g), *k1 = row(0, t0 + g + 8);
-          uint2 x[HD / 16], y[HD / 16];
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            x[k] = k0 ? *reinterpret_cast<const uint2*>(k0 + 16 * k + 4 * t4) : make_uint2(0, 0);
-            y[k] = k1 ? *reinterpret_cast<const uint2*>(k1 + 16 * k + 4 * t4) : make_uint2(0, 0);
-          }
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_16816(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = t0 + g + 8 * (e >> 1), h = nt * 8 + 2 * t4 + (e & 1);
-            s[0][nt][e] = t < stop[nt][e & 1] ? s[0][nt][e] * p.scale2 : -INFINITY;
-            if (score_rows && h < rows && t < len) score_rows[(int64_t)h * p.c.cap + t] = s[0][nt][e];
-          }
-        uint32_t pb[1][NT][2];
-        kv8_softmax<NT, HD, 1>(acc, s, gain, pb);
-        const __half *v0 = row(1, t0 + 2 * t4), *v1 = row(1, t0 + 2 * t4 + 1);
-        const __half *v2 = row(1, t0 + 2 * t4 + 8), *v3 = row(1, t0 + 2 * t4 + 9);
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const int d = 16 * i + 2 * g;
-          const uint32_t x0 = v0 ? ld_u32(v0 + d) : 0u, x1 = v1 ? ld_u32(v1 + d) : 0u;
-          const uint32_t x2 = v2 ? ld_u32(v2 + d) : 0u, x3 = v3 ? ld_u32(v3 + d) : 0u;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float u[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_16816(u, lo_pair(x0, x1), hi_pair(x0, x1), lo_pair(x2, x3), hi_pair(x2, x3), pb[0][nt][0], pb[0][nt][1]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc.o[i][nt][e] = fmaf(u[e], gain[nt][e & 1], acc.o[i][nt][e]);
+              if (k + kk == 0)
+                mma_16816_0(s[mt][nt], a0, a1, a2, a3, qb[nt][0][0], qb[nt][0][1]);
+              else
+                mma_16816(s[mt][nt], a0, a1, a2, a3, qb[nt][k + kk][0], qb[nt][k + kk][1]);
           }
         }
       }
-      if (idx + kDecWarps < z) cur.advance(work, kDecWarps);
+      __syncwarp();  // the keys are in registers: the next block's may come
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (more) load(&tk, k_slot, k_bar, row_base + (u + kWarps) * kKvBlock);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][nt][e] *= ks2;
+      if (t0 + kKvBlock > min_stop) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t0 + 16 * mt + g + 8 * (e >> 1) >= stop[nt][e & 1]) s[mt][nt][e] = -INFINITY;
+      }
+      if (score_rows) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int h = nt * 8 + 2 * t4 + j;
+            float* row = score_rows + (int64_t)h * p.c.cap + t0 + g;
+            if (h < rows) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                row[16 * mt] = s[mt][nt][j];
+                row[16 * mt + 8] = s[mt][nt][2 + j];
+              }
+            }
+          }
+      }
+      float gain[NT][2];
+      uint32_t pb[MT][NT][2];
+      kv8_softmax<NT, HD, MT>(acc, s, gain, pb);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) gain[nt][j] *= vs1;
+      if (fine && !mbar_wait_bounded(v_bar, phase, p.status)) {
+        if (more) mbar_wait_bounded(k_bar, phase ^ 1, p.status);
+        mbar_wait_bounded(v_bar, phase, p.status);
+        fine = false;
+      }
+      phase ^= 1;
+#pragma unroll
+      for (int i = 0; i < HD / 16; i += 2) {
+        float x[2][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t r[4];
+          ldsm4_t(r, (v_slot + mt * 16 * HD) + (lane_off ^ (i << 4)));
+#pragma unroll
+          for (int ii = 0; ii < 2; ++ii) {
+            const uint32_t a0 = codes2<0x4240>(r[2 * ii]), a1 = codes2<0x4341>(r[2 * ii]);
+            const uint32_t a2 = codes2<0x4240>(r[2 * ii + 1]), a3 = codes2<0x4341>(r[2 * ii + 1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              if (mt == 0)
+                mma_16816_0(x[ii][nt], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+              else
+                mma_16816(x[ii][nt], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+          }
+        }
+#pragma unroll
+        for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc.o[i + ii][nt][e] = fmaf(x[ii][nt][e], gain[nt][e & 1], acc.o[i + ii][nt][e]);
+      }
+      __syncwarp();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (more) load(&tv, v_slot, v_bar, row_base + (u + kWarps) * kKvBlock);
+    }
+#pragma unroll 1
+    for (; u < u_end; u += kWarps) {
+      // 16 FP16 rows of the tail, straight from memory; rows past the end are zero
+      const int t0 = coded * kKvBlock + (u - coded) * kDecTailUnit;
+      auto row = [&](int w, int t) -> const __half* {
+        if (p.extra && t == len - 1) return reinterpret_cast<const __half*>(pp_smem + S::kNew + w * HD * 2);
+        return t < len ? p.c.tail_row(w, b, kvh, t % kKvBlock) : nullptr;
+      };
+      float s[1][NT][4];
+      {
+        const __half *k0 = row(0, t0 + g), *k1 = row(0, t0 + g + 8);
+        uint2 x[HD / 16], y[HD / 16];
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          x[k] = k0 ? *reinterpret_cast<const uint2*>(k0 + 16 * k + 4 * t4) : make_uint2(0, 0);
+          y[k] = k1 ? *reinterpret_cast<const uint2*>(k1 + 16 * k + 4 * t4) : make_uint2(0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (k == 0)
+              mma_16816_0(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
+            else
+              mma_16816(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + g + 8 * (e >> 1), h = nt * 8 + 2 * t4 + (e & 1);
+          s[0][nt][e] = t < stop[nt][e & 1] ? s[0][nt][e] * p.scale2 : -INFINITY;
+          if (score_rows && h < rows && t < len) score_rows[(int64_t)h * p.c.cap + t] = s[0][nt][e];
+        }
+      float gain[NT][2];
+      uint32_t pb[1][NT][2];
+      kv8_softmax<NT, HD, 1>(acc, s, gain, pb);
+      const __half *v0 = row(1, t0 + 2 * t4), *v1 = row(1, t0 + 2 * t4 + 1);
+      const __half *v2 = row(1, t0 + 2 * t4 + 8), *v3 = row(1, t0 + 2 * t4 + 9);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        const int d = 16 * i + 2 * g;
+        const uint32_t x0 = v0 ? ld_u32(v0 + d) : 0u, x1 = v1 ? ld_u32(v1 + d) : 0u;
+        const uint32_t x2 = v2 ? ld_u32(v2 + d) : 0u, x3 = v3 ? ld_u32(v3 + d) : 0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float x[4];
+          mma_16816_0(x, lo_pair(x0, x1), hi_pair(x0, x1), lo_pair(x2, x3), hi_pair(x2, x3), pb[0][nt][0], pb[0][nt][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc.o[i][nt][e] = fmaf(x[e], gain[nt][e & 1], acc.o[i][nt][e]);
+        }
+      }
+    }
+    idx = seg0 + u;
+    if (end < z) {  // the next segment's first blocks travel while this one's results are added up
+      seg.next(work);
+      enter(seg1, seg1 + seg.U);
     }
 
-    // the warps' results, halves pairwise: lanes hold the same rows and dimensions
+    // the warps' results: every warp to the common reference, then added up by
+    // all threads in warp order, two dimensions of a row each
+    float2* ml = reinterpret_cast<float2*>(pp_smem + S::kMl);  // [warp][row]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -609,93 +652,70 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
-        acc.l[nt][j] = l;
+        if (g == 0) ml[warp * NT * 8 + nt * 8 + 2 * t4 + j] = make_float2(acc.m[nt][j], l);
       }
+    __syncthreads();
+    float fa[NT][2];
 #pragma unroll
-    for (int half = kDecWarps / 2; half > 0; half >>= 1) {
-      float* area = reinterpret_cast<float*>(pp_smem + S::kMerge + (warp % half) * S::kMergeWarp) + lane;
-      if (warp >= half && warp < 2 * half) {
-        float* f = area;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
+      for (int j = 0; j < 2; ++j) {
+        float m = -INFINITY;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * NT * 8 + nt * 8 + 2 * t4 + j].x);
+        fa[nt][j] = acc.m[nt][j] == -INFINITY ? 1.f : ex2(acc.m[nt][j] - m);  // such a warp's sums are 0 (or NaN)
+      }
+    const bool whole = at == seg0 && end == seg1;
+    float* rec = p.part + ((int64_t)blockIdx.x * 2 + (a >= seg0 ? 0 : 1)) * kPartFloats;
+    auto out_at = [&](int r, int d) {
+      const int i = p.n == 1 ? 0 : (row0 + r) / group, h = row0 + r - i * group;
+      return reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + (kvh * group + h) * p.ldoh + d);
+    };
+    constexpr int kI = HD / 16 / S::kRounds;  // dimension tiles of a round
 #pragma unroll
-            for (int e = 0; e < 4; ++e, f += 32) *f = acc.o[i][nt][e];
+    for (int round = 0; round < S::kRounds; ++round) {
+      float* area = reinterpret_cast<float*>(pp_smem + S::kMerge);
+      if (round) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j, f += 64) {
-            f[0] = acc.m[nt][j];
-            f[32] = acc.l[nt][j];
-          }
-      }
+          for (int e = 0; e < 4; ++e)
+            area[(warp * S::kPart + (i * NT + nt) * 4 + e) * 32 + lane] = acc.o[round * kI + i][nt][e] * fa[nt][e & 1];
       __syncthreads();
-      if (warp < half) {
-        float fa[NT][2];
-        const float* f = area + HD / 16 * NT * 4 * 32;
+      for (int e = tid; e < kI * NT * 2 * 32; e += kThreads) {
+        const int el = e & 31, j = (e >> 5) & 1, in = e >> 6, nt = in % NT, i = in / NT;
+        const int r = nt * 8 + 2 * (el & 3) + j, d = 16 * (round * kI + i) + 2 * (el >> 2);
+        if (r >= rows) continue;
+        float m = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * NT * 8 + r].x);
 #pragma unroll
-          for (int j = 0; j < 2; ++j, f += 64) {
-            const float m2 = f[0], l2 = f[32];
-            if (m2 > acc.m[nt][j]) acc.rebase(nt, j, m2);
-            fa[nt][j] = m2 == -INFINITY ? 0.f : ex2(m2 - acc.m[nt][j]);
-            acc.l[nt][j] = m2 == -INFINITY ? acc.l[nt][j] + l2 : fmaf(l2, fa[nt][j], acc.l[nt][j]);
-          }
-        f = area;
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e, f += 32) acc.o[i][nt][e] = fmaf(*f, fa[nt][e & 1], acc.o[i][nt][e]);
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 v = ml[w * NT * 8 + r];
+          l = fmaf(v.y, v.x == -INFINITY ? 1.f : ex2(v.x - m), l);
+          const float* f = area + (w * S::kPart + in * 4 + j) * 32 + el;
+          x += f[0];
+          y += f[64];
+        }
+        if (whole) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          *out_at(r, d) = __floats2half2_rn(x * inv, y * inv);
+          if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
+        } else {
+          *reinterpret_cast<float2*>(rec + r * HD + d) = make_float2(x, y);
+          if (d == 0) *reinterpret_cast<float2*>(rec + NT * 8 * HD + 2 * r) = make_float2(m, l);
+        }
       }
-      __syncthreads();
     }
 
-    const int segment = b * work.per_seq + seg.seg;
-    auto store = [&](int r, int d, float x, float y) {  // two dimensions of row r
-      const int i = (row0 + r) / group, h = kvh * group + (row0 + r) % group;
-      *reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d) = __floats2half2_rn(x, y);
-    };
-    if (at == seg0 && end == seg1) {
-      if (warp == 0) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = nt * 8 + 2 * t4 + j;
-            if (r >= rows) continue;
-            const float l = acc.l[nt][j], inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i)
-              store(r, 16 * i + 2 * g, acc.o[i][nt][j] * inv, acc.o[i][nt][2 + j] * inv);
-            if (p.scores && g == 0) p.lse[b * p.nq + kvh * group + r] = acc.m[nt][j] + log2f(l);
-          }
-      }
-    } else {
-      constexpr int kPart = kv8_part_floats(NT, HD);
-      if (warp == 0) {
-        float* rec = p.part + ((int64_t)blockIdx.x * 2 + (a >= seg0 ? 0 : 1)) * kPart;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = nt * 8 + 2 * t4 + j;
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i)
-              *reinterpret_cast<float2*>(rec + r * HD + 16 * i + 2 * g) =
-                  make_float2(acc.o[i][nt][j], acc.o[i][nt][2 + j]);
-            if (g == 0)
-              *reinterpret_cast<float2*>(rec + NT * 8 * HD + 2 * r) = make_float2(acc.m[nt][j], acc.l[nt][j]);
-          }
-        __threadfence();
-        __syncwarp();
-      }
+    if (!whole) {
       // the last CTA of the segment to arrive adds up the partials in order
       const int first = aligned ? segment * each : seg0 / per;
-      const int contrib = aligned ? pieces(seg.U) : (seg1 - 1) / per - first + 1;
+      const int contrib = aligned ? pieces(U) : (seg1 - 1) / per - first + 1;
+      __threadfence();
+      __syncthreads();
       if (tid == 0) {
         const int n = atomicAdd(p.cnt + first, 1);  // at most one segment goes on past a CTA's share
         s_flag = n == contrib - 1;
@@ -706,41 +726,38 @@ __global__ void __launch_bounds__(kDecWarps * 32, 1)
       }
       __syncthreads();
       if (s_flag) {
-        auto rec = [&](int k) {
-          return p.part + ((int64_t)(first + k) * 2 + (aligned || (first + k) * (int64_t)per >= seg0 ? 0 : 1)) * kPart;
+        auto from = [&](int k) {
+          return p.part +
+                 ((int64_t)(first + k) * 2 + (aligned || (first + k) * (int64_t)per >= seg0 ? 0 : 1)) * kPartFloats;
         };
         for (int e = tid; e < rows * (HD / 4); e += kThreads) {
           const int r = e / (HD / 4), d = e % (HD / 4) * 4;
           float m = -INFINITY;
 #pragma unroll 4
-          for (int k = 0; k < contrib; ++k) m = fmaxf(m, __ldcg(rec(k) + NT * 8 * HD + 2 * r));
+          for (int k = 0; k < contrib; ++k) m = fmaxf(m, __ldcg(from(k) + NT * 8 * HD + 2 * r));
           float l = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
           for (int k = 0; k < contrib; ++k) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec(k) + NT * 8 * HD + 2 * r));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec(k) + r * HD + d));
-            const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - m);  // a NaN in an empty row's sums stays one
-            l = fmaf(ml.y, f, l);
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(from(k) + NT * 8 * HD + 2 * r));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(from(k) + r * HD + d));
+            const float f = v.x == -INFINITY ? 1.f : ex2(v.x - m);
+            l = fmaf(v.y, f, l);
             o.x = fmaf(x.x, f, o.x);
             o.y = fmaf(x.y, f, o.y);
             o.z = fmaf(x.z, f, o.z);
             o.w = fmaf(x.w, f, o.w);
           }
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          store(r, d, o.x * inv, o.y * inv);
-          store(r, d + 2, o.z * inv, o.w * inv);
+          *out_at(r, d) = __floats2half2_rn(o.x * inv, o.y * inv);
+          *out_at(r, d + 2) = __floats2half2_rn(o.z * inv, o.w * inv);
           if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
         }
       }
-      __syncthreads();
     }
     at = end;
-    if (at < z) seg.advance(work, seg.U - seg.u);
   }
-  if (!fine)  // a copy did not arrive in time (status 1): leave none in flight
-    for (; used < issued; ++used) mbar_wait_bounded(bars + 8 * (used % kDecSlots), (used / kDecSlots) & 1, p.status);
-  if (p.extra) kv8_store_token<HD>(p, s_len, red);
+  if (p.extra) kv8_store_token<HD, kWarps>(p, s_len, red);
 }
 
 // weights[b][g][t] += sum of the group's exp2(score - lse).

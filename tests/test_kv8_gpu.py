@@ -288,6 +288,39 @@ def test_decode_long_and_many(cuda, batch, lens):
         assert not weights[b, 0, len(p):].any()
 
 
+def test_batches_share_scratch(cuda):
+    """Calls of different sizes in turn on one stream, and a batch that goes in parts."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_decode
+    g = _gen(cuda, 29)
+    B, n = 1100, 70
+    k, v, q = _rand(g, B, n, 1, 64), _rand(g, B, n, 1, 64), _rand(g, B, 3, 64, spread=2.0)
+    cache = _new(B, 1, 128, 64, cuda)
+    pos = torch.arange(B, device=cuda, dtype=torch.int32) % (n - 1)
+    kv8_append(cache, k, v, pos * 0, counts=pos)
+    few = _new(3, 1, 20_032, 64, cuda)
+    kf, vf = _rand(g, 3, 20_000, 1, 64), _rand(g, 3, 20_000, 1, 64)
+    kv8_append(few, kf, vf, _ints([0, 0, 0], cuda))
+    new = k[:, n - 1], v[:, n - 1]
+    a = [kv8_decode(q, *new, cache, pos)]
+    b = [kv8_decode(q[:3], kf[:, 0], vf[:, 0], few, _ints([20_000] * 3, cuda))]
+    a.append(kv8_decode(q, *new, cache, pos))
+    b.append(kv8_decode(q[:3], kf[:, 0], vf[:, 0], few, _ints([20_000] * 3, cuda)))
+    assert torch.equal(*a) and torch.equal(*b) and int(cache.status) == 0
+    ref = kr.RefKV(B, 1, 64)
+    for w, (x, y) in enumerate(((k, new[0]), (v, new[1]))):
+        x, y = x.cpu(), y.cpu()
+        for i in range(B):
+            r, l = ref.s[w][i][0], i % (n - 1)
+            rows = torch.cat([x[i, :l, 0], y[i]])
+            if l + 1 >= 64:
+                c, s = kr.quantise(rows[:64])
+                r.codes.append(c)
+                r.scales.append(s)
+            r.rows, r.len = rows[(l // 64) * 64:], l + 1
+    want, _ = kr.attention(ref, q[:, None], [1] * B)
+    _check_out(a[0], want[:, 0], ref)
+
+
 def test_peaked_scores_and_scale(cuda):
     """A sink that takes nearly all the weight, blocks of very different scale,
     infinite keys in one head only."""
