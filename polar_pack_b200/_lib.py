@@ -206,7 +206,12 @@ def floats4(vals) -> ctypes.Array:
     return _F4(*[float(v) for v in vals])
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)   # the same handle, without a Stream object (2 us less per call)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -250,7 +250,8 @@ int run_decode(const char* who, Kv8DecodeParams& p, float* weights, void* worksp
   }
   if (!weights) return PP_OK;
   const Kv8WeightsParams w{all.scores, all.lse, weights, all.lens, all.rope, all.extra, all.nq, all.c.nkv, all.c.cap};
-  return launch_kernel("kv8_weights_kernel", launch_overlap(), kv8_weights_kernel,
+  // started early whatever the overlap setting: it waits for the decode kernel itself
+  return launch_kernel("kv8_weights_kernel", true, kv8_weights_kernel,
                        dim3((unsigned)cdiv(all.c.cap, 256), (unsigned)all.c.nkv, (unsigned)all.c.batch), dim3(256), 0, s,
                        w);
 }

@@ -403,7 +403,8 @@ int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int*
   if (int rc = pp::launch_kernel("kv8_select_kernel", pp::launch_overlap(), pp::kv8_select_kernel,
                                  dim3((unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kSelThreads), 0, s, p))
     return rc;
-  return pp::launch_kernel("kv8_gather_kernel", pp::launch_overlap(),
+  // started early whatever the overlap setting: it waits for the selection itself
+  return pp::launch_kernel("kv8_gather_kernel", true,
                            p.c.hd == 128 ? pp::kv8_gather_kernel<128> : pp::kv8_gather_kernel<64>,
                            dim3((unsigned)pp::cdiv(keep, pp::kKvBlock), (unsigned)p.c.nkv, (unsigned)p.c.batch * 2),
                            dim3(pp::kThreads), 0, s, p);

@@ -31,6 +31,10 @@ constexpr int kDecTailUnit = 16;  // FP16 rows of a tail unit; a coded unit is a
 // twice the accumulators for 16 rows.
 constexpr int kv8_warps(int nt) { return nt == 1 ? 12 : 8; }
 
+// Units that a CTA takes at least: with fewer than one to a warp, more SMs
+// share a short cache and their warps do not compete for issue slots.
+constexpr int kDecMinUnits = 4;
+
 struct Kv8DecodeParams {
   Kv8Cache c;
   const __half* q;
@@ -316,9 +320,44 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  // lengths and the units before each sequence
-  const int group = p.nq / p.c.nkv;
-  for (int b = tid; b < p.c.batch; b += kThreads) {
+  // Where the segments divide the CTAs, this CTA's segment does not depend on
+  // the lengths: its rows are fetched together with them.
+  const int group = p.nq / p.c.nkv, ctas = gridDim.x;
+  const Kv8Work work{s_len, s_pre, p.c.batch, p.c.nkv * p.tiles};
+  const int each = ctas / (p.c.batch * work.per_seq);  // CTAs per segment, if every one gets as many
+  auto query_row8 = [&](int b, int kvh, int row0, int e) {  // item e of a tile's rows (padding rows are zero)
+    const int r = e / (HD / 8), d0 = e % (HD / 8) * 8;
+    const int i = p.n == 1 ? 0 : (row0 + r) / group, h = row0 + r - i * group;
+    if (r >= NT * 8 || i >= p.n || h >= group) return make_uint4(0, 0, 0, 0);
+    const int t = p.rope.cos ? p.rope.pos[b] + i : 0;
+    if (p.rope.cos && (t < 0 || t >= p.rope.len)) return make_uint4(0, 0, 0, 0);
+    return kv8_load8(p.q + b * p.ldqb + i * p.ldqt + (int64_t)(kvh * group + h) * p.ldqh, d0, HD, p.rope, t);
+  };
+  auto token_row8 = [&](int b, int kvh, int e) {  // the token's key, then its value
+    const int w = e / (HD / 8), d0 = e % (HD / 8) * 8;
+    Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
+    const int t = r.cos ? r.pos[b] : 0;
+    if (r.cos && (t < 0 || t >= r.len)) return make_uint4(0, 0, 0, 0);
+    return kv8_load8(p.x[w] + b * p.ldxb[w] + kvh * p.ldxh[w], d0, HD, r, t);
+  };
+  constexpr int kRowItems = NT * 8 * (HD / 8), kNewItems = 2 * (HD / 8);
+  static_assert(kRowItems <= kThreads && kNewItems <= kThreads, "one item per thread");
+  const bool is_new = p.extra && tid >= kThreads - kNewItems;
+  auto fetch = [&](int b, int kvh, int row0, uint4& row, uint4& token) {
+    if (tid < kRowItems) row = query_row8(b, kvh, row0, tid);
+    if (is_new) token = token_row8(b, kvh, kThreads - 1 - tid);
+  };
+  uint4 row{}, token{};
+  int have = -1;  // the segment whose rows these are
+  if (each > 0 && (int)blockIdx.x / each < p.c.batch * work.per_seq) {
+    have = blockIdx.x / each;
+    const int s = have % work.per_seq;
+    fetch(have / work.per_seq, s / p.tiles, s % p.tiles * NT * 8, row, token);
+  }
+
+  // lengths and the units before each sequence; every warp for itself while a
+  // warp's lanes hold them all (all write the same), else the CTA together
+  auto length = [&](int b) {
     const int len = p.lens[b] + p.extra;
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
     bool ok = len <= p.c.cap;
@@ -327,45 +366,57 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       ok = ok && r >= 0 && r <= p.rope.len - cnt;
     }
     if (!ok && blockIdx.x == 0) atomicExch(p.status, 5);
-    s_len[b] = ok && cnt > 0 ? max(len, 0) : 0;
+    return ok && cnt > 0 ? max(len, 0) : 0;
+  };
+  const bool small = p.c.batch <= 32;
+  if (!small) {
+    for (int b = tid; b < p.c.batch; b += kThreads) s_len[b] = length(b);
+    __syncthreads();
   }
-  __syncthreads();
-  const Kv8Work work{s_len, s_pre, p.c.batch, p.c.nkv * p.tiles};
-  if (warp == 0) {
-    int sum = 0, mx = 0;
+  int max_units = 0;
+  if (small || warp == 0) {
+    int sum = 0;
     for (int b0 = 0; b0 < p.c.batch; b0 += 32) {
-      const int u = b0 + lane < p.c.batch ? Kv8Work::units(s_len[b0 + lane]) : 0;
-      mx = max(mx, u);
+      const int b = b0 + lane;
+      const int len = b >= p.c.batch ? 0 : small ? length(b) : s_len[b];
+      const int u = Kv8Work::units(len);
+      max_units = max(max_units, u);
       int x = u * work.per_seq;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      if (b0 + lane < p.c.batch) s_pre[b0 + lane + 1] = sum + x;
+      if (b < p.c.batch) {
+        if (small) s_len[b] = len;
+        s_pre[b + 1] = sum + x;
+      }
       sum += __shfl_sync(0xffffffffu, x, 31);
     }
-    for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int o = 16; o > 0; o >>= 1) max_units = max(max_units, __shfl_xor_sync(0xffffffffu, max_units, o));
     if (lane == 0) {
       s_pre[0] = 0;
-      s_max = mx;
+      if (!small) s_max = max_units;
     }
+    __syncwarp();
   }
-  __syncthreads();
+  if (!small) {
+    __syncthreads();
+    max_units = s_max;
+  }
 
   // this CTA's share [a, z) of the units
-  const int total = s_pre[p.c.batch], ctas = gridDim.x;
-  const int per = max(kWarps, (total + ctas - 1) / ctas);
-  const int each = ctas / (p.c.batch * work.per_seq);  // CTAs per segment, if every one got as many
-  const bool aligned = each > 0 && (s_max + each - 1) / each <= per + per / 4;
-  auto pieces = [&](int U) { return min(each, (U + kWarps - 1) / kWarps); };
+  const int total = s_pre[p.c.batch];
+  const int per = max(kDecMinUnits, (total + ctas - 1) / ctas);
+  const bool aligned = each > 0 && (max_units + each - 1) / each <= per + per / 4;
+  auto pieces = [&](int U) { return min(each, (U + kDecMinUnits - 1) / kDecMinUnits); };
   int a = 0, z = 0;
   if (aligned) {
-    const int s = blockIdx.x / each, b = s / work.per_seq, j = blockIdx.x % each;
-    if (b < p.c.batch) {
+    if (have >= 0) {
+      const int b = have / work.per_seq, j = blockIdx.x - have * each;
       const int U = Kv8Work::units(s_len[b]), k = pieces(U);
       if (j < k) {
-        const int s0 = s_pre[b] + s % work.per_seq * U;
+        const int s0 = s_pre[b] + (have - b * work.per_seq) * U;
         a = s0 + (int)((int64_t)U * j / k);
         z = s0 + (int)((int64_t)U * (j + 1) / k);
       }
@@ -395,10 +446,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       load(&tv, v_slot, v_bar, seg_row + u * kKvBlock);
     }
   };
-  if (a < z) {
-    seg.seek(work, a);
-    enter(a - seg.u, a - seg.u + seg.U);
-  }
+  if (a < z) seg.seek(work, a);
 
   // rows without work
   for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x)
@@ -410,32 +458,23 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
 
   const uint32_t lane_off = tile_off<HD>(lane & 15, lane >> 4);
   for (int at = a; at < z;) {
-    const int b = seg.b, row_base = seg_row, segment = seg.b * work.per_seq + seg.seg;
+    const int b = seg.b, segment = seg.b * work.per_seq + seg.seg;
     const int kvh = p.tiles == 1 ? seg.seg : seg.seg / p.tiles, tile = p.tiles == 1 ? 0 : seg.seg % p.tiles;
     const int seg0 = at - seg.u, U = seg.U, seg1 = seg0 + U, end = min(z, seg1);
     const int len = s_len[b], coded = kv8_last_block(len);
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
     const int row0 = tile * NT * 8, rows = min(NT * 8, p.n * group - row0);
 
-    // the tile's query rows (padding rows are zero) and the token, as FP16
-    for (int e = tid; e < NT * 8 * (HD / 8); e += kThreads) {
-      const int r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int i = (row0 + r) / group, h = kvh * group + (row0 + r) % group;
-        if (i < cnt)
-          x = kv8_load8(p.q + b * p.ldqb + i * p.ldqt + h * p.ldqh, d0, HD, p.rope, p.rope.cos ? p.rope.pos[b] + i : 0);
-      }
-      uint2* dst = reinterpret_cast<uint2*>(pp_smem + S::kQ + r * S::kQRow + d0 * 2);
-      dst[0] = make_uint2(x.x, x.y);
-      dst[1] = make_uint2(x.z, x.w);
+    // the tile's query rows and the token, fetched ahead of the segment's blocks
+    if (segment != have) fetch(b, kvh, row0, row, token);
+    have = -1;
+    if (at == a) enter(seg0, seg1);
+    if (tid < kRowItems) {
+      uint2* dst = reinterpret_cast<uint2*>(pp_smem + S::kQ + tid / (HD / 8) * S::kQRow + tid % (HD / 8) * 16);
+      dst[0] = make_uint2(row.x, row.y);
+      dst[1] = make_uint2(row.z, row.w);
     }
-    if (p.extra && tid >= kThreads - 2 * (HD / 8)) {
-      const int e = kThreads - 1 - tid, w = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      const Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
-      *reinterpret_cast<uint4*>(pp_smem + S::kNew + w * HD * 2 + d0 * 2) =
-          kv8_load8(p.x[w] + b * p.ldxb[w] + kvh * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
-    }
+    if (is_new) *reinterpret_cast<uint4*>(pp_smem + S::kNew + (kThreads - 1 - tid) * 16) = token;
     // first position that row (nt, j) does not attend
     int stop[NT][2];
     int min_stop = len;
@@ -506,7 +545,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
       __syncwarp();  // the keys are in registers: the next block's may come
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (more) load(&tk, k_slot, k_bar, row_base + (u + kWarps) * kKvBlock);
+      if (more) load(&tk, k_slot, k_bar, seg_row + (u + kWarps) * kKvBlock);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
       __syncwarp();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (more) load(&tv, v_slot, v_bar, row_base + (u + kWarps) * kKvBlock);
+      if (more) load(&tv, v_slot, v_bar, seg_row + (u + kWarps) * kKvBlock);
     }
 #pragma unroll 1
     for (; u < u_end; u += kWarps) {
@@ -732,21 +771,36 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
         };
         for (int e = tid; e < rows * (HD / 4); e += kThreads) {
           const int r = e / (HD / 4), d = e % (HD / 4) * 4;
-          float m = -INFINITY;
-#pragma unroll 4
-          for (int k = 0; k < contrib; ++k) m = fmaxf(m, __ldcg(from(k) + NT * 8 * HD + 2 * r));
-          float l = 0.f;
+          float m = -INFINITY, l = 0.f;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int k = 0; k < contrib; ++k) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(from(k) + NT * 8 * HD + 2 * r));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(from(k) + r * HD + d));
-            const float f = v.x == -INFINITY ? 1.f : ex2(v.x - m);
-            l = fmaf(v.y, f, l);
-            o.x = fmaf(x.x, f, o.x);
-            o.y = fmaf(x.y, f, o.y);
-            o.z = fmaf(x.z, f, o.z);
-            o.w = fmaf(x.w, f, o.w);
+          for (int k0 = 0; k0 < contrib; k0 += 8) {  // eight partials' loads at a time
+            float2 v[8];
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              v[k] = make_float2(-INFINITY, 0.f);
+              x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (k0 + k < contrib) {
+                v[k] = __ldcg(reinterpret_cast<const float2*>(from(k0 + k) + NT * 8 * HD + 2 * r));
+                x[k] = __ldcg(reinterpret_cast<const float4*>(from(k0 + k) + r * HD + d));
+              }
+            }
+            float to = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to = fmaxf(to, v[k].x);
+            const float f0 = m == -INFINITY ? 1.f : ex2(m - to);
+            l *= f0;
+            o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+            m = to;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float f = v[k].x == -INFINITY ? 1.f : ex2(v[k].x - m);
+              l = fmaf(v[k].y, f, l);
+              o.x = fmaf(x[k].x, f, o.x);
+              o.y = fmaf(x[k].y, f, o.y);
+              o.z = fmaf(x[k].z, f, o.z);
+              o.w = fmaf(x[k].w, f, o.w);
+            }
           }
           const float inv = l == 0.f ? 0.f : 1.f / l;
           *out_at(r, d) = __floats2half2_rn(o.x * inv, o.y * inv);

@@ -66,6 +66,8 @@ class KV8Cache:
                                       pair(k_scales.data_ptr(), v_scales.data_ptr()),
                                       pair(k_tail.data_ptr(), v_tail.data_ptr()), b, h, cap, hd)
         self.ref = ctypes.byref(self.desc)
+        self.index = self.device.index
+        self.status_ptr = self.status.data_ptr()
         self._ws: dict = {}
 
     @classmethod
@@ -102,20 +104,20 @@ _scratch: dict = {}
 _scratch_kept: list = []
 
 
-def _workspace(cache: KV8Cache, nbytes: int) -> torch.Tensor:
-    """Zero-filled scratch of the attention calls, one per (device, stream); the
+def _workspace(cache: KV8Cache, nbytes: int) -> tuple:
+    """Zero-filled scratch (address, bytes, tensor) of the attention calls, one per (device, stream); the
     kernels leave its counters at zero.  An outgrown buffer is kept, since a
     captured graph may refer to it.  A capture that needs a new one gets its
     own, whose fill is part of the graph."""
-    key = (cache.device.index, _lib.stream_handle(cache.device))
+    key = (cache.index, _lib.stream_handle(cache.device))
     buf = _scratch.get(key)
-    if buf is None or buf.numel() < nbytes:
+    if buf is None or buf[1] < nbytes:
         new = torch.zeros(max(nbytes, 1 << 20) * 5 // 4, dtype=torch.uint8, device=cache.device)
         if torch.cuda.is_current_stream_capturing():
-            return new
+            return new.data_ptr(), new.numel(), new
         if buf is not None:
             _scratch_kept.append(buf)
-        buf = _scratch[key] = new
+        buf = _scratch[key] = (new.data_ptr(), new.numel(), new)
     return buf
 
 
@@ -130,19 +132,21 @@ def _c_strides(*s: int):
 
 def _rows(t: torch.Tensor, name: str, shape: tuple, cache: KV8Cache) -> torch.Tensor:
     """FP16 rows as the kernels read them: contiguous and 16-byte aligned."""
-    if t.dtype != torch.float16 or t.device != cache.device or tuple(t.shape) != shape:
+    if t.dtype is not torch.float16 or t.shape != shape or t.get_device() != cache.index:
         raise ValueError(f"{name} must be FP16 {list(shape)} on {cache.device}, "
                          f"got {t.dtype} {list(t.shape)} on {t.device}")
-    st = t.stride()
-    if st[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for s in st[:-1]):
-        t = t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() & 15 or not t.is_contiguous():
+        st = t.stride()
+        if st[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for s in st[:-1]):
+            t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _ints(t, name: str, cache: KV8Cache):
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != cache.device or t.shape != (cache.batch,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != cache.index or t.shape != (cache.batch,) or \
+            not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{cache.batch}] on {cache.device}")
     return t.data_ptr()
 
@@ -162,31 +166,34 @@ def _rope(rope, cache: KV8Cache):
 def _weights(w, name: str, cache: KV8Cache):
     if w is None:
         return None
-    if (w.dtype != torch.float32 or w.device != cache.device or not w.is_contiguous()
+    if (w.dtype is not torch.float32 or w.get_device() != cache.index or not w.is_contiguous()
             or w.shape != (cache.batch, cache.kv_heads, cache.capacity)):
         raise ValueError(f"{name} must be contiguous float32 [{cache.batch}, {cache.kv_heads}, {cache.capacity}] "
                          f"on {cache.device}")
     return w.data_ptr()
 
 
-def _output(out, shape, cache: KV8Cache):
+def _output(out, q, cache: KV8Cache):
+    """The output for queries q: given, or new (with q's layout if that is whole)."""
     if out is None:
-        return torch.empty(shape, dtype=torch.float16, device=cache.device)
+        if q.is_contiguous():
+            return torch.empty_like(q)
+        return torch.empty(q.shape, dtype=torch.float16, device=cache.device)
     st = out.stride()
-    if (out.dtype != torch.float16 or out.device != cache.device or tuple(out.shape) != tuple(shape) or st[-1] != 1
+    if (out.dtype is not torch.float16 or out.get_device() != cache.index or out.shape != q.shape or st[-1] != 1
             or out.data_ptr() & 15 or any(s & 7 for s in st[:-1])):
-        raise ValueError(f"out must be FP16 {list(shape)} on {cache.device} with 16-byte aligned contiguous rows")
+        raise ValueError(f"out must be FP16 {list(q.shape)} on {cache.device} with 16-byte aligned contiguous rows")
     return out
 
 
 def _call(cache: KV8Cache, fn: str, *args) -> None:
     """The C call on the current stream of the cache's device."""
-    lib = _lib.load()
-    if torch.cuda.current_device() != cache.device.index:
+    f = getattr(_lib.load(), fn)
+    if torch.cuda.current_device() != cache.index:
         with torch.cuda.device(cache.device):
-            rc = getattr(lib, fn)(cache.ref, *args, cache.status.data_ptr(), _lib.stream_handle(cache.device))
+            rc = f(cache.ref, *args, cache.status_ptr, _lib.stream_handle(cache.device))
     else:
-        rc = getattr(lib, fn)(cache.ref, *args, cache.status.data_ptr(), _lib.stream_handle(cache.device))
+        rc = f(cache.ref, *args, cache.status_ptr, _lib.stream_handle(cache.device))
     if rc:
         _lib.check(rc)
 
@@ -235,11 +242,11 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, counts: 
     n, nq = q.shape[1], q.shape[2]
     shape = (cache.batch, n, nq, cache.head_dim)
     q = _rows(q, "q", shape, cache)
-    out = _output(out, shape, cache)
+    out = _output(out, q, cache)
     ws = _workspace(cache, cache.workspace_bytes(n, nq, False))
     _call(cache, "pp_kv8_attention", q.data_ptr(), _c_strides(*q.stride()[:3]), n, nq, _ints(lens, "lens", cache),
           _ints(counts, "counts", cache), 1 / math.sqrt(cache.head_dim) if scale is None else scale, out.data_ptr(),
-          _c_strides(*out.stride()[:3]), *_rope(rope, cache), ws.data_ptr(), ws.numel())
+          _c_strides(*out.stride()[:3]), *_rope(rope, cache), ws[0], ws[1])
     return out
 
 
@@ -260,12 +267,12 @@ def kv8_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV8Cach
     b, nq, hd = cache.batch, q.shape[1], cache.head_dim
     q = _rows(q, "q", (b, nq, hd), cache)
     k, v = _rows(k, "k", (b, cache.kv_heads, hd), cache), _rows(v, "v", (b, cache.kv_heads, hd), cache)
-    out = _output(out, (b, nq, hd), cache)
+    out = _output(out, q, cache)
     ws = _workspace(cache, cache.workspace_bytes(1, nq, weights is not None))
     _call(cache, "pp_kv8_decode", q.data_ptr(), _c_strides(*q.stride()[:2]), nq, k.data_ptr(),
           _c_strides(*k.stride()[:2]), v.data_ptr(), _c_strides(*v.stride()[:2]), _ints(pos, "pos", cache),
           1 / math.sqrt(hd) if scale is None else scale, _weights(weights, "weights", cache), out.data_ptr(),
-          _c_strides(*out.stride()[:2]), *_rope(rope, cache), ws.data_ptr(), ws.numel())
+          _c_strides(*out.stride()[:2]), *_rope(rope, cache), ws[0], ws[1])
     return out
 
 
