@@ -211,20 +211,26 @@ __device__ __forceinline__ void kv8_softmax(Kv8Acc<NT, HD>& a, float (&s)[MT][NT
 }
 
 // What a CTA knows of the launch's work: effective lengths and unit counts.
+// A segment counts kDecSegmentUnits more units than it has, at its end, for
+// the time between two segments of a CTA (about 3 us, which at the memory's
+// rate is eight blocks): shares with many short segments get fewer blocks.
+constexpr int kDecSegmentUnits = 8;
+
 struct Kv8Work {
   const int* len;   // [batch], 0 for sequences without work
-  const int* pre;   // [batch + 1] units before each sequence, all heads and tiles
+  const int* pre;   // [batch + 1] counted units before each sequence, all heads and tiles
   int batch, per_seq;  // segments per sequence: kv heads x row tiles
   __device__ __forceinline__ static int units(int len) {
     if (len <= 0) return 0;
     const int last = kv8_last_block(len);
     return last + (len - last * kKvBlock + kDecTailUnit - 1) / kDecTailUnit;
   }
+  __device__ __forceinline__ static int counted(int len) { return len > 0 ? units(len) + kDecSegmentUnits : 0; }
 };
 
-// Where a unit index falls: sequence, segment of the sequence, unit.
+// Where a counted unit falls: sequence, segment of the sequence, unit.
 struct Kv8Cursor {
-  int b, seg, u, U;
+  int b, seg, u, U;  // U: counted units of the segment
   __device__ __forceinline__ void seek(const Kv8Work& w, int idx) {
     int lo = 0, hi = w.batch - 1;
     while (lo < hi) {
@@ -233,7 +239,7 @@ struct Kv8Cursor {
       else hi = mid - 1;
     }
     b = lo;
-    U = Kv8Work::units(w.len[b]);
+    U = Kv8Work::counted(w.len[b]);
     seg = (idx - w.pre[b]) / U;
     u = idx - w.pre[b] - seg * U;
   }
@@ -244,7 +250,7 @@ struct Kv8Cursor {
     seg = 0;
     do ++b;
     while (w.pre[b + 1] == w.pre[b]);
-    U = Kv8Work::units(w.len[b]);
+    U = Kv8Work::counted(w.len[b]);
   }
 };
 
@@ -296,6 +302,11 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
   }
 }
 
+// A segment of which a CTA has only a part.
+struct Kv8Part {
+  int b, kvh, row0, rows, seg0, first, contrib, last;
+};
+
 template <int NT, int HD>
 __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p, const __grid_constant__ CUtensorMap tk,
@@ -303,7 +314,8 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
   using S = Kv8DecodeSmem<NT, HD>;
   constexpr int kWarps = S::kWarps, kThreads = kWarps * 32, kPartFloats = kv8_part_floats(NT, HD);
   __shared__ float red[kWarps];
-  __shared__ int s_flag, s_max;
+  __shared__ int s_max;
+  __shared__ Kv8Part s_part[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
   const uint32_t k_slot = base + warp * 2 * S::kSlot, v_slot = k_slot + S::kSlot;
@@ -379,7 +391,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     for (int b0 = 0; b0 < p.c.batch; b0 += 32) {
       const int b = b0 + lane;
       const int len = b >= p.c.batch ? 0 : small ? length(b) : s_len[b];
-      const int u = Kv8Work::units(len);
+      const int u = Kv8Work::counted(len);
       max_units = max(max_units, u);
       int x = u * work.per_seq;
 #pragma unroll
@@ -416,9 +428,9 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       const int b = have / work.per_seq, j = blockIdx.x - have * each;
       const int U = Kv8Work::units(s_len[b]), k = pieces(U);
       if (j < k) {
-        const int s0 = s_pre[b] + (have - b * work.per_seq) * U;
-        a = s0 + (int)((int64_t)U * j / k);
-        z = s0 + (int)((int64_t)U * (j + 1) / k);
+        const int s0 = s_pre[b] + (have - b * work.per_seq) * Kv8Work::counted(s_len[b]);
+        a = s0 + (int)((uint32_t)U * j / k);
+        z = s0 + (int)((uint32_t)U * (j + 1) / k);
       }
     }
   } else {
@@ -426,27 +438,54 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     z = min((int64_t)total, (int64_t)a + per);
   }
 
-  // Warp w takes units a + w, a + w + kWarps, ... of the share.
+  // Warp w takes units a + w, a + w + kWarps, ... of the share.  A block's
+  // keys or values arrive as one tensor box, a tail unit's rows (without the
+  // token, which is not in the tail yet) as one plain copy.
   bool fine = true;
-  auto load = [&](const CUtensorMap* tm, uint32_t dst, uint32_t bar, int row) {
-    if (lane == 0 && fine) {
-      mbar_expect_tx(bar, S::kSlot);
-      tma_load_2d(dst, tm, 0, row, bar);
-    }
-  };
   int idx = a + warp, phase = 0;
   Kv8Cursor seg{};
-  int seg_row = 0;  // the segment's first row of the tensor maps
-  auto enter = [&](int from, int to) {  // starts the warp's first block of the segment of units [from, to)
-    const int tile_head = p.tiles == 1 ? seg.seg : seg.seg / p.tiles;
-    seg_row = (int)(p.c.head(seg.b, tile_head) * p.c.cap);
-    const int u = idx - from;
-    if (idx < min(z, to) && u < kv8_last_block(s_len[seg.b])) {
-      load(&tk, k_slot, k_bar, seg_row + u * kKvBlock);
-      load(&tv, v_slot, v_bar, seg_row + u * kKvBlock);
+  if (a < z) seg.seek(work, a);
+  int seg_head = 0, seg_coded = 0, seg_held = 0;  // sequence and head; blocks and tokens held as codes / in all
+  auto load = [&](int w, int u) {
+    if (lane != 0 || !fine) return;
+    const uint32_t dst = w ? v_slot : k_slot, bar = w ? v_bar : k_bar;
+    if (u < seg_coded) {
+      mbar_expect_tx(bar, S::kSlot);
+      tma_load_2d(dst, w ? &tv : &tk, 0, (seg_head * (p.c.cap / kKvBlock) + u) * kKvBlock, bar);
+    } else {
+      const int r = (u - seg_coded) * kDecTailUnit;
+      const uint32_t bytes = min(kDecTailUnit, max(0, seg_held - seg_coded * kKvBlock - r)) * HD * 2;
+      mbar_expect_tx(bar, bytes);
+      if (bytes) bulk_load(dst, p.c.tail[w] + ((int64_t)seg_head * kKvBlock + r) * HD, bytes, bar);
     }
   };
-  if (a < z) seg.seek(work, a);
+  auto enter = [&](int from) {  // starts the warp's first unit of the segment that begins at unit `from`
+    const int len = s_len[seg.b], u = idx - from;
+    seg_head = (int)p.c.head(seg.b, p.tiles == 1 ? seg.seg : seg.seg / p.tiles);
+    seg_coded = kv8_last_block(len);
+    seg_held = len - p.extra;
+    if (idx < min(z, from + Kv8Work::units(len))) {
+      load(0, u);
+      load(1, u);
+    }
+  };
+
+  // A copy that does not arrive in time sets status 1; nothing stays in flight.
+  auto await_keys = [&]() {
+    if (fine && !mbar_wait_bounded(k_bar, phase, p.status)) {
+      fine = false;
+      mbar_wait_bounded(k_bar, phase, p.status);
+      mbar_wait_bounded(v_bar, phase, p.status);
+    }
+  };
+  auto await_values = [&](bool more) {  // more: the next unit's keys are on their way
+    if (fine && !mbar_wait_bounded(v_bar, phase, p.status)) {
+      fine = false;
+      if (more) mbar_wait_bounded(k_bar, phase ^ 1, p.status);
+      mbar_wait_bounded(v_bar, phase, p.status);
+    }
+    phase ^= 1;
+  };
 
   // rows without work
   for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x)
@@ -456,19 +495,34 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
         *reinterpret_cast<uint4*>(p.out + b * p.ldob + i * p.ldot + h * p.ldoh + d0) = make_uint4(0, 0, 0, 0);
       }
 
+  auto out_at = [&](int b, int kvh, int row0, int r, int d) {
+    const int i = p.n == 1 ? 0 : (row0 + r) / group, h = row0 + r - i * group;
+    return reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh + d);
+  };
   const uint32_t lane_off = tile_off<HD>(lane & 15, lane >> 4);
+  bool entered = false;
+  int turn = 0, pending = 0;
   for (int at = a; at < z;) {
     const int b = seg.b, segment = seg.b * work.per_seq + seg.seg;
     const int kvh = p.tiles == 1 ? seg.seg : seg.seg / p.tiles, tile = p.tiles == 1 ? 0 : seg.seg % p.tiles;
-    const int seg0 = at - seg.u, U = seg.U, seg1 = seg0 + U, end = min(z, seg1);
     const int len = s_len[b], coded = kv8_last_block(len);
+    const int seg0 = at - seg.u, seg1 = seg0 + seg.U, U = Kv8Work::units(len);
+    const int real1 = seg0 + U, end = min(z, seg1), u_end = min(z, real1) - seg0;
+    if (at >= real1) {  // only counted units of this segment fall here
+      at = end;
+      if (end < z) {
+        seg.next(work);
+        idx = at + warp;
+      }
+      continue;
+    }
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
     const int row0 = tile * NT * 8, rows = min(NT * 8, p.n * group - row0);
 
     // the tile's query rows and the token, fetched ahead of the segment's blocks
     if (segment != have) fetch(b, kvh, row0, row, token);
     have = -1;
-    if (at == a) enter(seg0, seg1);
+    if (!entered) enter(seg0);
     if (tid < kRowItems) {
       uint2* dst = reinterpret_cast<uint2*>(pp_smem + S::kQ + tid / (HD / 8) * S::kQRow + tid % (HD / 8) * 16);
       dst[0] = make_uint2(row.x, row.y);
@@ -488,7 +542,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
     const float *k_scale = p.c.scale(0, b, kvh, 0), *v_scale = p.c.scale(1, b, kvh, 0);
     float ks = 0.f, vs = 0.f;  // of the warp's next block
-    if (idx < end && idx - seg0 < coded) {
+    if (idx - seg0 < min(u_end, coded)) {
       ks = k_scale[idx - seg0];
       vs = v_scale[idx - seg0];
     }
@@ -507,22 +561,18 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     acc.clear();
     float* score_rows = p.scores ? p.scores + ((int64_t)b * p.nq + kvh * group) * p.c.cap : nullptr;
     int u = idx - seg0;
-    const int u_end = end - seg0, coded_end = min(u_end, coded);
+    const int coded_end = min(u_end, coded);
 #pragma unroll 1
     for (; u < coded_end; u += kWarps) {
       constexpr int MT = kKvBlock / 16;
       const int t0 = u * kKvBlock;
-      const bool more = u + kWarps < coded_end;
+      const bool more = u + kWarps < u_end;
       const float ks2 = ks * p.scale2, vs1 = vs;
-      if (more) {
+      if (u + kWarps < coded_end) {
         ks = k_scale[u + kWarps];
         vs = v_scale[u + kWarps];
       }
-      if (fine && !mbar_wait_bounded(k_bar, phase, p.status)) {  // status 1; nothing stays in flight
-        fine = false;
-        mbar_wait_bounded(k_bar, phase, p.status);
-        mbar_wait_bounded(v_bar, phase, p.status);
-      }
+      await_keys();
       float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -545,7 +595,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
       __syncwarp();  // the keys are in registers: the next block's may come
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (more) load(&tk, k_slot, k_bar, seg_row + (u + kWarps) * kKvBlock);
+      if (more) load(0, u + kWarps);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -584,12 +634,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) gain[nt][j] *= vs1;
-      if (fine && !mbar_wait_bounded(v_bar, phase, p.status)) {
-        if (more) mbar_wait_bounded(k_bar, phase ^ 1, p.status);
-        mbar_wait_bounded(v_bar, phase, p.status);
-        fine = false;
-      }
-      phase ^= 1;
+      await_values(more);
 #pragma unroll
       for (int i = 0; i < HD / 16; i += 2) {
         float x[2][NT][4];
@@ -619,34 +664,34 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
       __syncwarp();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (more) load(&tv, v_slot, v_bar, seg_row + (u + kWarps) * kKvBlock);
+      if (more) load(1, u + kWarps);
     }
 #pragma unroll 1
     for (; u < u_end; u += kWarps) {
-      // 16 FP16 rows of the tail, straight from memory; rows past the end are zero
+      // 16 FP16 rows of the tail, the token's own from where it was put
       const int t0 = coded * kKvBlock + (u - coded) * kDecTailUnit;
-      auto row = [&](int w, int t) -> const __half* {
-        if (p.extra && t == len - 1) return reinterpret_cast<const __half*>(pp_smem + S::kNew + w * HD * 2);
-        return t < len ? p.c.tail_row(w, b, kvh, t % kKvBlock) : nullptr;
+      const bool more = u + kWarps < u_end;
+      auto row = [&](int w, int r) {
+        return p.extra && t0 + r == len - 1 ? base + S::kNew + w * HD * 2 : (w ? v_slot : k_slot) + r * HD * 2;
       };
+      await_keys();
       float s[1][NT][4];
       {
-        const __half *k0 = row(0, t0 + g), *k1 = row(0, t0 + g + 8);
-        uint2 x[HD / 16], y[HD / 16];
+        const uint32_t k0 = row(0, g) + 8 * t4, k1 = row(0, g + 8) + 8 * t4;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          x[k] = k0 ? *reinterpret_cast<const uint2*>(k0 + 16 * k + 4 * t4) : make_uint2(0, 0);
-          y[k] = k1 ? *reinterpret_cast<const uint2*>(k1 + 16 * k + 4 * t4) : make_uint2(0, 0);
-        }
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
+          const uint2 x = lds_u2(k0 + 32 * k), y = lds_u2(k1 + 32 * k);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             if (k == 0)
-              mma_16816_0(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
+              mma_16816_0(s[0][nt], x.x, y.x, x.y, y.y, qb[nt][k][0], qb[nt][k][1]);
             else
-              mma_16816(s[0][nt], x[k].x, y[k].x, x[k].y, y[k].y, qb[nt][k][0], qb[nt][k][1]);
+              mma_16816(s[0][nt], x.x, y.x, x.y, y.y, qb[nt][k][0], qb[nt][k][1]);
+        }
       }
+      __syncwarp();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (more) load(0, u + kWarps);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -658,13 +703,14 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       float gain[NT][2];
       uint32_t pb[1][NT][2];
       kv8_softmax<NT, HD, 1>(acc, s, gain, pb);
-      const __half *v0 = row(1, t0 + 2 * t4), *v1 = row(1, t0 + 2 * t4 + 1);
-      const __half *v2 = row(1, t0 + 2 * t4 + 8), *v3 = row(1, t0 + 2 * t4 + 9);
+      await_values(more);
+      const uint32_t v0 = row(1, 2 * t4) + 4 * g, v1 = row(1, 2 * t4 + 1) + 4 * g;
+      const uint32_t v2 = row(1, 2 * t4 + 8) + 4 * g, v3 = row(1, 2 * t4 + 9) + 4 * g;
+      const int left = len - t0 - 2 * t4;  // rows past the end count as zero: their contents may be anything
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
-        const int d = 16 * i + 2 * g;
-        const uint32_t x0 = v0 ? ld_u32(v0 + d) : 0u, x1 = v1 ? ld_u32(v1 + d) : 0u;
-        const uint32_t x2 = v2 ? ld_u32(v2 + d) : 0u, x3 = v3 ? ld_u32(v3 + d) : 0u;
+        const uint32_t x0 = left > 0 ? lds_u32(v0 + 32 * i) : 0u, x1 = left > 1 ? lds_u32(v1 + 32 * i) : 0u;
+        const uint32_t x2 = left > 8 ? lds_u32(v2 + 32 * i) : 0u, x3 = left > 9 ? lds_u32(v3 + 32 * i) : 0u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float x[4];
@@ -673,11 +719,20 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
           for (int e = 0; e < 4; ++e) acc.o[i][nt][e] = fmaf(x[e], gain[nt][e & 1], acc.o[i][nt][e]);
         }
       }
+      __syncwarp();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (more) load(1, u + kWarps);
     }
-    idx = seg0 + u;
-    if (end < z) {  // the next segment's first blocks travel while this one's results are added up
+    // the next segment's first units and rows travel while this one's results are added up
+    turn = (turn + u_end - (at - seg0)) % kWarps;  // the warps go on in turn
+    idx = end + (warp >= turn ? warp - turn : warp - turn + kWarps);
+    entered = end < z;
+    if (entered) {
       seg.next(work);
-      enter(seg1, seg1 + seg.U);
+      enter(end);
+      const int s = seg.seg;
+      have = seg.b * work.per_seq + s;
+      fetch(seg.b, p.tiles == 1 ? s : s / p.tiles, p.tiles == 1 ? 0 : s % p.tiles * NT * 8, row, token);
     }
 
     // the warps' results: every warp to the common reference, then added up by
@@ -704,12 +759,8 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * NT * 8 + nt * 8 + 2 * t4 + j].x);
         fa[nt][j] = acc.m[nt][j] == -INFINITY ? 1.f : ex2(acc.m[nt][j] - m);  // such a warp's sums are 0 (or NaN)
       }
-    const bool whole = at == seg0 && end == seg1;
+    const bool whole = at == seg0 && z >= real1;
     float* rec = p.part + ((int64_t)blockIdx.x * 2 + (a >= seg0 ? 0 : 1)) * kPartFloats;
-    auto out_at = [&](int r, int d) {
-      const int i = p.n == 1 ? 0 : (row0 + r) / group, h = row0 + r - i * group;
-      return reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + (kvh * group + h) * p.ldoh + d);
-    };
     constexpr int kI = HD / 16 / S::kRounds;  // dimension tiles of a round
 #pragma unroll
     for (int round = 0; round < S::kRounds; ++round) {
@@ -740,7 +791,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
         }
         if (whole) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          *out_at(r, d) = __floats2half2_rn(x * inv, y * inv);
+          *out_at(b, kvh, row0, r, d) = __floats2half2_rn(x * inv, y * inv);
           if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
         } else {
           *reinterpret_cast<float2*>(rec + r * HD + d) = make_float2(x, y);
@@ -750,66 +801,77 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     }
 
     if (!whole) {
-      // the last CTA of the segment to arrive adds up the partials in order
-      const int first = aligned ? segment * each : seg0 / per;
-      const int contrib = aligned ? pieces(U) : (seg1 - 1) / per - first + 1;
-      __threadfence();
-      __syncthreads();
       if (tid == 0) {
-        const int n = atomicAdd(p.cnt + first, 1);  // at most one segment goes on past a CTA's share
-        s_flag = n == contrib - 1;
-        if (s_flag) {
-          p.cnt[first] = 0;
-          __threadfence();
-        }
+        const int first = aligned ? segment * each : seg0 / per;
+        s_part[pending] = Kv8Part{b, kvh, row0, rows, seg0, first,
+                                  aligned ? pieces(U) : (real1 - 1) / per - first + 1, 0};
       }
-      __syncthreads();
-      if (s_flag) {
-        auto from = [&](int k) {
-          return p.part +
-                 ((int64_t)(first + k) * 2 + (aligned || (first + k) * (int64_t)per >= seg0 ? 0 : 1)) * kPartFloats;
-        };
-        for (int e = tid; e < rows * (HD / 4); e += kThreads) {
-          const int r = e / (HD / 4), d = e % (HD / 4) * 4;
-          float m = -INFINITY, l = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int k0 = 0; k0 < contrib; k0 += 8) {  // eight partials' loads at a time
-            float2 v[8];
-            float4 x[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              v[k] = make_float2(-INFINITY, 0.f);
-              x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (k0 + k < contrib) {
-                v[k] = __ldcg(reinterpret_cast<const float2*>(from(k0 + k) + NT * 8 * HD + 2 * r));
-                x[k] = __ldcg(reinterpret_cast<const float4*>(from(k0 + k) + r * HD + d));
-              }
-            }
-            float to = m;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) to = fmaxf(to, v[k].x);
-            const float f0 = m == -INFINITY ? 1.f : ex2(m - to);
-            l *= f0;
-            o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-            m = to;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float f = v[k].x == -INFINITY ? 1.f : ex2(v[k].x - m);
-              l = fmaf(v[k].y, f, l);
-              o.x = fmaf(x[k].x, f, o.x);
-              o.y = fmaf(x[k].y, f, o.y);
-              o.z = fmaf(x[k].z, f, o.z);
-              o.w = fmaf(x[k].w, f, o.w);
-            }
-          }
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          *out_at(r, d) = __floats2half2_rn(o.x * inv, o.y * inv);
-          *out_at(r, d + 2) = __floats2half2_rn(o.z * inv, o.w * inv);
-          if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
-        }
-      }
+      ++pending;  // at most the share's first and last segment
     }
     at = end;
+  }
+
+  // segments that other CTAs have a part of: the last of them to arrive adds up
+  // the parts in order
+  if (pending) {
+    __threadfence();
+    __syncthreads();
+    if (tid < pending) {
+      Kv8Part& s = s_part[tid];
+      s.last = atomicAdd(p.cnt + s.first, 1) == s.contrib - 1;  // at most one segment goes on past a CTA's share
+      if (s.last) {
+        p.cnt[s.first] = 0;
+        __threadfence();
+      }
+    }
+    __syncthreads();
+    for (int i = 0; i < pending; ++i) {
+      if (!s_part[i].last) continue;
+      const int b = s_part[i].b, kvh = s_part[i].kvh, row0 = s_part[i].row0, rows = s_part[i].rows;
+      const int seg0 = s_part[i].seg0, first = s_part[i].first, contrib = s_part[i].contrib;
+      auto from = [&](int k) {
+        return p.part +
+               ((int64_t)(first + k) * 2 + (aligned || (first + k) * (int64_t)per >= seg0 ? 0 : 1)) * kPartFloats;
+      };
+      for (int e = tid; e < rows * (HD / 4); e += kThreads) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < contrib; k0 += 8) {  // eight partials' loads at a time
+          float2 v[8];
+          float4 x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            v[k] = make_float2(-INFINITY, 0.f);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k0 + k < contrib) {
+              v[k] = __ldcg(reinterpret_cast<const float2*>(from(k0 + k) + NT * 8 * HD + 2 * r));
+              x[k] = __ldcg(reinterpret_cast<const float4*>(from(k0 + k) + r * HD + d));
+            }
+          }
+          float to = m;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) to = fmaxf(to, v[k].x);
+          const float f0 = m == -INFINITY ? 1.f : ex2(m - to);
+          l *= f0;
+          o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+          m = to;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float f = v[k].x == -INFINITY ? 1.f : ex2(v[k].x - m);
+            l = fmaf(v[k].y, f, l);
+            o.x = fmaf(x[k].x, f, o.x);
+            o.y = fmaf(x[k].y, f, o.y);
+            o.z = fmaf(x[k].z, f, o.z);
+            o.w = fmaf(x[k].w, f, o.w);
+          }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *out_at(b, kvh, row0, r, d) = __floats2half2_rn(o.x * inv, o.y * inv);
+        *out_at(b, kvh, row0, r, d + 2) = __floats2half2_rn(o.z * inv, o.w * inv);
+        if (p.scores && d == 0) p.lse[b * p.nq + kvh * group + r] = m + log2f(l);
+      }
+    }
   }
   if (p.extra) kv8_store_token<HD, kWarps>(p, s_len, red);
 }
