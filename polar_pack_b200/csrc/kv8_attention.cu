@@ -1,136 +1,14 @@
-// Attention over the 8-bit KV cache (kv8.cuh): one query row of one kv
-// head's group per CTA.
-//   s_t = scale * q . k_t,  p = softmax(s) over t <= the query's position,
-//   out = sum_t p_t v_t     (FP32 throughout, rounded once)
+// Attention over the 8-bit KV cache (kv8.cuh): the choice between the kernel
+// for few query rows per kv head (kv8_decode.cuh) and the one for many
+// (kv8_prompt.cuh), their plans and the entry points.
 #include "kv8.cuh"
 #include "kv8_decode.cuh"
+#include "kv8_prompt.cuh"
 
 namespace pp {
 namespace {
 
-constexpr int kTile = 128;    // positions per step, one thread each
 constexpr int kMaxGroup = 16;
-
-struct AttnParams {
-  Kv8Cache c;
-  const __half* q;
-  int64_t ldqb, ldqt, ldqh;
-  __half* out;
-  int64_t ldob, ldot, ldoh;
-  const int* lens;
-  const int* counts;
-  int n, nq;
-  float scale;
-  Kv8Rope rope;
-  int* status;
-};
-
-template <int HD>
-__global__ void __launch_bounds__(kTile) kv8_attention_kernel(const AttnParams p) {
-  __shared__ float qs[kMaxGroup][HD];
-  __shared__ float ss[kMaxGroup][kTile];
-  __shared__ float red[kTile / 32];
-  __shared__ __align__(16) __half vrow[HD];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int i = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const int group = p.nq / p.c.nkv;
-  const int len = p.lens[b];
-  const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
-  const int end = len - cnt + i + 1;  // positions attended
-  bool ok = len <= p.c.cap;
-  const int r = p.rope.cos ? p.rope.pos[b] + i : 0;
-  if (p.rope.cos && len > 0 && i < cnt && (r < 0 || r >= p.rope.len)) ok = false;
-  if (!ok && tid == 0 && p.status) atomicExch(p.status, 5);
-  __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)kvh * group * p.ldoh;
-  if (!ok || i >= cnt || end <= 0) {
-    for (int e = tid; e < group * HD; e += kTile) out[e / HD * p.ldoh + e % HD] = __float2half(0.f);
-    return;
-  }
-  const __half* q = p.q + b * p.ldqb + i * p.ldqt + (int64_t)kvh * group * p.ldqh;
-  for (int e = tid; e < group * HD / 8; e += kTile) {
-    const int h = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    const uint4 x = kv8_load8(q + h * p.ldqh, d0, HD, p.rope, r);
-    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(u2h(u[j]));
-      qs[h][d0 + 2 * j] = f.x;
-      qs[h][d0 + 2 * j + 1] = f.y;
-    }
-  }
-  float mx[kMaxGroup], sum[kMaxGroup], acc[kMaxGroup];
-#pragma unroll
-  for (int h = 0; h < kMaxGroup; ++h) {
-    mx[h] = -INFINITY;
-    sum[h] = 0.f;
-    acc[h] = 0.f;
-  }
-  __syncthreads();
-  auto scores = [&](int t, float (&s)[kMaxGroup]) {
-#pragma unroll
-    for (int h = 0; h < kMaxGroup; ++h) s[h] = 0.f;
-    for (int d0 = 0; d0 < HD; d0 += 8) {
-      const bool tail = t / kKvBlock == kv8_last_block(len);
-      float k[8];
-      float mul = 1.f;
-      if (tail) {
-        const uint4 x = *reinterpret_cast<const uint4*>(p.c.tail_row(0, b, kvh, t % kKvBlock) + d0);
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __half22float2(u2h(u[j]));
-          k[2 * j] = f.x;
-          k[2 * j + 1] = f.y;
-        }
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(p.c.code_row(0, b, kvh, t) + d0);
-        for (int j = 0; j < 8; ++j) k[j] = (float)((int)((j < 4 ? x.x : x.y) >> (8 * (j & 3)) & 255u) - 128);
-        mul = *p.c.scale(0, b, kvh, t / kKvBlock);
-      }
-      for (int h = 0; h < group; ++h) {
-        float a = 0.f;
-        for (int j = 0; j < 8; ++j) a = fmaf(qs[h][d0 + j], k[j], a);
-        s[h] = fmaf(a, mul, s[h]);
-      }
-    }
-  };
-  for (int t0 = 0; t0 < end; t0 += kTile) {
-    float s[kMaxGroup];
-    const int t = t0 + tid;
-    if (t < end) scores(t, s);
-    for (int h = 0; h < group; ++h) ss[h][tid] = t < end ? s[h] * p.scale : -INFINITY;
-    __syncthreads();
-    const int rows = min(kTile, end - t0);
-    for (int h = 0; h < group; ++h) {
-      float m = mx[h];
-      for (int j = 0; j < rows; ++j) m = fmaxf(m, ss[h][j]);
-      const float c = mx[h] == -INFINITY ? 0.f : expf(mx[h] - m);
-      sum[h] *= c;
-      acc[h] *= c;
-      mx[h] = m;
-    }
-    if (tid < HD)
-      for (int j = 0; j < rows; ++j) {
-        const int tt = t0 + j;
-        float v;
-        if (tt / kKvBlock == kv8_last_block(len))
-          v = __half2float(p.c.tail_row(1, b, kvh, tt % kKvBlock)[tid]);
-        else
-          v = ((int)p.c.code_row(1, b, kvh, tt)[tid] - 128) * *p.c.scale(1, b, kvh, tt / kKvBlock);
-        for (int h = 0; h < group; ++h) {
-          const float e = expf(ss[h][j] - mx[h]);
-          sum[h] += e;
-          acc[h] = fmaf(e, v, acc[h]);
-        }
-      }
-    else
-      for (int j = 0; j < rows; ++j)
-        for (int h = 0; h < group; ++h) sum[h] += expf(ss[h][j] - mx[h]);
-    __syncthreads();
-  }
-  if (tid < HD)
-    for (int h = 0; h < group; ++h) out[h * p.ldoh + tid] = __float2half_rn(acc[h] / sum[h]);
-}
 
 // How a call with `rows` query rows per kv head runs on kv8_decode_kernel:
 // tiles of 8 rows while one is enough, else of 16.
@@ -155,8 +33,37 @@ DecodePlan plan_decode(const Kv8Cache& c, int64_t n, int64_t nq, bool weights, i
   return d;
 }
 
-bool g_attr[4][64];
-int g_limit[4][64];
+// More rows go to kv8_prompt_kernel.  With few tiles for the SMs, a tile's
+// positions are split into parts of at least eight blocks (by the capacity: the
+// lengths are on the device).
+struct PromptPlan {
+  int tiles, splits;
+  size_t bytes;
+};
+
+PromptPlan plan_prompt(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
+  PromptPlan d{};
+  const int64_t rows = n * (nq / c.nkv);
+  d.tiles = (int)cdiv(rows, kPrRows);
+  const int64_t base = (int64_t)d.tiles * c.nkv * c.batch;
+  int64_t s = ctas / base;
+  if (s > c.cap / kKvBlock / 8) s = c.cap / kKvBlock / 8;
+  d.splits = s > 1 ? (int)s : 1;
+  d.bytes = d.splits > 1 ? (size_t)d.splits * c.batch * c.nkv * rows * (c.hd + 2) * sizeof(float) : 0;
+  return d;
+}
+
+bool g_attr[6][64];
+int g_limit[6][64];
+
+int encode_codes(const Kv8Cache& c, CUtensorMap (&tm)[2]) {
+  const uint64_t rows = (uint64_t)c.batch * c.nkv * c.cap;
+  for (int w = 0; w < 2; ++w)
+    if (int rc = encode_tmap_2d(&tm[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, c.codes[w], c.hd, rows, c.hd, c.hd, kKvBlock,
+                                c.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+      return rc;
+  return PP_OK;
+}
 
 template <int NT, int HD>
 int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
@@ -171,13 +78,33 @@ int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
     return PP_ERR_CUDA;
   }
   CUtensorMap tm[2];
-  const uint64_t rows = (uint64_t)p.c.batch * p.c.nkv * p.c.cap;
-  for (int w = 0; w < 2; ++w)
-    if (int rc = encode_tmap_2d(&tm[w], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.c.codes[w], HD, rows, HD, HD, kKvBlock,
-                                HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
-      return rc;
+  if (int rc = encode_codes(p.c, tm)) return rc;
   return launch_kernel("kv8_decode_kernel", launch_overlap(), kern, dim3((unsigned)ctas), dim3(kv8_warps(NT) * 32),
                        (size_t)smem, s, p, tm[0], tm[1]);
+}
+
+template <int HD>
+int launch_prompt(const Kv8PromptParams& p, cudaStream_t s) {
+  using S = Kv8PromptSmem<HD>;
+  constexpr int kv = 4 + (HD == 128);
+  auto kern = kv8_prompt_kernel<HD>;
+  int lim = 0;
+  if (int rc = ensure_smem_attr(kern, g_attr[kv], g_limit[kv], &lim)) return rc;
+  if (S::kBytes > lim) {
+    set_error("kv8_prompt_kernel: %d bytes of shared memory needed, %d available", S::kBytes, lim);
+    return PP_ERR_CUDA;
+  }
+  CUtensorMap tm[2];
+  if (int rc = encode_codes(p.c, tm)) return rc;
+  const dim3 grid((unsigned)(p.tiles * p.splits), (unsigned)p.c.nkv, (unsigned)p.c.batch);
+  if (int rc = launch_kernel("kv8_prompt_kernel", launch_overlap(), kern, grid, dim3(kPrThreads), (size_t)S::kBytes, s,
+                             p, tm[0], tm[1]))
+    return rc;
+  if (p.splits == 1) return PP_OK;
+  const Kv8JoinParams j{p.part, p.out, p.ldob, p.ldot, p.ldoh, p.c.batch, p.c.nkv, p.n, p.nq, p.splits};
+  const int64_t rows = (int64_t)p.c.batch * p.c.nkv * p.n * (p.nq / p.c.nkv);
+  // started early whatever the overlap setting: it waits for the attention itself
+  return launch_kernel("kv8_join_kernel", true, kv8_join_kernel<HD>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, s, j);
 }
 
 // Query and output rows, heads and sizes, checked.  Sets *empty for a call
@@ -269,14 +196,15 @@ int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64
     return PP_ERR_INVALID;
   }
   *bytes = 0;
-  if (n > 0 && n * (nq / c.nkv) <= pp::kDecodeRows) {
-    const int ctas = pp::device_sm_count(pp::current_device());
-    if (ctas < 1) {
-      pp::set_error("pp_kv8_attention_workspace_bytes: no current CUDA device");
-      return PP_ERR_CUDA;
-    }
-    *bytes = pp::plan_decode(c, n, nq, weights != 0, ctas).bytes;
+  if (n == 0) return PP_OK;
+  const int ctas = pp::device_sm_count(pp::current_device());
+  if (ctas < 1) {
+    pp::set_error("pp_kv8_attention_workspace_bytes: no current CUDA device");
+    return PP_ERR_CUDA;
   }
+  *bytes = n * (nq / c.nkv) <= pp::kDecodeRows ? pp::plan_decode(c, n, nq, weights != 0, ctas).bytes
+                                               : pp::align_up(ctas * sizeof(int), 256) +
+                                                     pp::plan_prompt(c, n, nq, ctas).bytes;
   return PP_OK;
 }
 
@@ -309,12 +237,39 @@ int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_s
     p.status = status;
     return pp::run_decode("pp_kv8_attention", p, nullptr, workspace, workspace_bytes, s);
   }
-  pp::AttnParams a{p.c,     reinterpret_cast<const __half*>(q),
-                   q_strides[0], q_strides[1], q_strides[2], reinterpret_cast<__half*>(out),
-                   out_strides[0], out_strides[1], out_strides[2], lens, counts, (int)n, (int)nq, scale, p.rope, status};
-  return pp::launch_kernel("kv8_attention_kernel", pp::launch_overlap(),
-                           p.c.hd == 128 ? pp::kv8_attention_kernel<128> : pp::kv8_attention_kernel<64>,
-                           dim3((unsigned)n, (unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kTile), 0, s, a);
+  const int ctas = pp::device_sm_count(pp::current_device());
+  if (ctas < 1) {
+    pp::set_error("pp_kv8_attention: no current CUDA device");
+    return PP_ERR_CUDA;
+  }
+  const pp::PromptPlan d = pp::plan_prompt(p.c, n, nq, ctas);
+  const size_t counters = pp::align_up(ctas * sizeof(int), 256);  // of the other kernel's calls on this workspace
+  if (d.bytes && (!workspace || workspace_bytes < counters + d.bytes || !pp::aligned(workspace, 256))) {
+    pp::set_error("pp_kv8_attention: workspace of %zu bytes (256-byte aligned) required", counters + d.bytes);
+    return PP_ERR_WORKSPACE;
+  }
+  pp::Kv8PromptParams a{};
+  a.c = p.c;
+  a.q = reinterpret_cast<const __half*>(q);
+  a.ldqb = q_strides[0];
+  a.ldqt = q_strides[1];
+  a.ldqh = q_strides[2];
+  a.out = reinterpret_cast<__half*>(out);
+  a.ldob = out_strides[0];
+  a.ldot = out_strides[1];
+  a.ldoh = out_strides[2];
+  a.lens = lens;
+  a.counts = counts;
+  a.n = (int)n;
+  a.nq = (int)nq;
+  a.scale2 = fabsf(scale) * 1.44269504088896341f;
+  a.q_sign = scale < 0.f ? 0x80008000u : 0u;
+  a.rope = p.rope;
+  a.tiles = d.tiles;
+  a.splits = d.splits;
+  a.part = d.bytes ? reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + counters) : nullptr;
+  a.status = status;
+  return p.c.hd == 128 ? pp::launch_prompt<128>(a, s) : pp::launch_prompt<64>(a, s);
 }
 
 int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[2], int64_t nq, const void* k,

@@ -1,0 +1,476 @@
+// Prompt attention over the 8-bit KV cache on the tcgen05 tensor cores: many
+// query rows per kv head (kv8_attention.cu launches it).
+//
+// Mathematics as in kv8_decode.cuh, with the running maximum moved only when a
+// row outgrows it by 2^4 and the block scale of the values folded into the
+// weights: with f = s_v / v_ref, v_ref the largest s_v of the range, the tensor
+// core accumulates P' (c_v - 128) for P' = fp16(2^11 f exp(S - m)), and
+// out = v_ref sum P' (c_v - 128) / (2^11 sum exp(S - m)).  2^11 leaves 2^4 for the
+// lagging maximum below FP16's largest number, and keeps weights down to
+// 2^-25 / f of the maximum at full precision.
+//
+// Bound: the matrix products; next to them the 16 exponentials a clock of an
+// SM, which take about as long.  A CTA has 256 rows (query x head of the kv
+// head's group) as two tiles of 128, so that one tile's softmax runs while the
+// other's products do, and each block is unpacked once for both.  Roles:
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row; S from tensor
+//                    memory, P to shared memory, O rescaled in tensor memory
+//                    when its row's maximum moved, the result at the end
+//   warps 8-11       unpack a block's codes (arrived by TMA) to FP16 tiles
+//   warp 12          issues the products: S = Q K^T (M 128, N 64) a block ahead
+//                    of O += P V (M 128, N head_dim)
+//   warp 13          the code boxes' TMA
+// K and V tiles have the same layout, positions x dimensions in 128-byte
+// swizzled rows: K-major for the first product, MN-major for the second.
+// Every wait is bounded; tensor memory is released on every path.
+#pragma once
+
+#include "kv8.cuh"
+#include "kv8_decode.cuh"
+#include "pp_tcgen05.cuh"
+
+namespace pp {
+
+constexpr int kPrRows = 256;                  // query rows of a CTA
+constexpr int kPrTile = 128;                  // rows of one MMA
+constexpr int kPrThreads = 14 * 32;
+constexpr int kPrCodeStages = 3;
+constexpr float kPrLag = 4.f;                 // log2 growth of a maximum that rescales
+constexpr float kPrLift = 11.f;               // log2 factor of the FP16 weights
+
+struct Kv8PromptParams {
+  Kv8Cache c;
+  const __half* q;
+  int64_t ldqb, ldqt, ldqh;
+  __half* out;
+  int64_t ldob, ldot, ldoh;
+  const int* lens;
+  const int* counts;
+  int n, nq;
+  float scale2;       // |scale| * log2(e)
+  uint32_t q_sign;    // 0x80008000 for a negative scale
+  Kv8Rope rope;
+  int tiles, splits;  // row tiles per (sequence, kv head); parts of each tile's positions
+  float* part;        // splits > 1: [splits][batch][kv head][rows][hd + 2]
+  int* status;
+};
+
+template <int HD>
+struct Kv8PromptSmem {
+  static constexpr int kHalves = HD / 64;                        // 64-dimension halves of a tile
+  static constexpr int kQTile = kHalves * kPrTile * 128;
+  static constexpr int kKv = kHalves * kKvBlock * 128;           // an FP16 tile of keys or values
+  static constexpr int kCode = kKvBlock * HD;
+  static constexpr int kQ = 0;
+  static constexpr int kK = 2 * kQTile;                          // two buffers each
+  static constexpr int kV = kK + 2 * kKv;
+  static constexpr int kP = kV + 2 * kKv;                        // one per row tile
+  static constexpr int kCodes = kP + 2 * kPrTile * 128;
+  static constexpr int kBar = kCodes + kPrCodeStages * 2 * kCode;
+  static constexpr int kBytes = kBar + 256;
+};
+
+// Row r of a call's n * group rows: query r / group, head r % group.
+__device__ __forceinline__ int kv8_row_stop(int i, int len, int cnt) { return i < cnt ? len - cnt + i + 1 : 0; }
+
+template <int HD>
+__global__ void __launch_bounds__(kPrThreads, 1)
+    kv8_prompt_kernel(const __grid_constant__ Kv8PromptParams p, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv) {
+  using S = Kv8PromptSmem<HD>;
+  __shared__ float s_red[14];
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
+  // long tiles first: the last rows attend the most positions
+  const int tile = p.tiles - 1 - blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int group = p.nq / p.c.nkv, rows = p.n * group, row0 = tile * kPrRows;
+  // barriers
+  const uint32_t bar = base + S::kBar;
+  const uint32_t code_full = bar, code_empty = bar + 24;           // [3]
+  const uint32_t k_full = bar + 48, k_empty = bar + 64;            // [2]
+  const uint32_t v_full = bar + 80, v_empty = bar + 96;            // [2]
+  const uint32_t s_full = bar + 112, s_empty = bar + 144;          // [tile][2]
+  const uint32_t p_full = bar + 176, p_empty = bar + 192;          // [tile]
+  const uint32_t done = bar + 208;
+  if (tid == 0) {
+    for (int i = 0; i < kPrCodeStages; ++i) {
+      mbar_init(code_full + 8 * i, 1);
+      mbar_init(code_empty + 8 * i, 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + 8 * i, 4);
+      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v_full + 8 * i, 4);
+      mbar_init(v_empty + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4);
+      mbar_init(p_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(s_empty + 8 * i, 4);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  if (warp == 12) {
+    tmem_alloc((uint32_t)__cvta_generic_to_shared(&s_tmem), 512);
+    tmem_relinquish();
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+
+  int len = p.lens[b];
+  const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+  bool ok = len <= p.c.cap;
+  const int rot0 = p.rope.cos ? p.rope.pos[b] : 0;
+  if (p.rope.cos && len > 0 && cnt > 0) ok = ok && rot0 >= 0 && rot0 <= p.rope.len - cnt;
+  if (!ok && tid == 0) atomicExch(p.status, 5);
+  len = ok ? max(len, 0) : 0;
+  // blocks that this CTA's rows attend, and its part of them
+  const int i_first = row0 / group, i_last = min((min(row0 + kPrRows, rows) - 1) / group, cnt - 1);
+  const int max_stop = i_last >= i_first ? max(0, kv8_row_stop(i_last, len, cnt)) : 0;
+  const int blocks = len > 0 ? (max_stop + kKvBlock - 1) / kKvBlock : 0;
+  const int j0 = (int)((int64_t)blocks * split / p.splits), j1 = (int)((int64_t)blocks * (split + 1) / p.splits);
+  const int J = j1 - j0;
+  const int coded = kv8_last_block(len);  // the block after them is the tail
+  const float *k_scale = p.c.scale(0, b, kvh, 0), *v_scale = p.c.scale(1, b, kvh, 0);
+
+  // query rows to the K-major tiles; v_ref
+  if (J > 0) {
+    for (int e = tid; e < kPrRows * (HD / 8); e += kPrThreads) {
+      const int r = e / (HD / 8), d0 = e % (HD / 8) * 8, i = (row0 + r) / group, h = (row0 + r) - i * group;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (i < cnt)
+        x = kv8_load8(p.q + b * p.ldqb + i * p.ldqt + (int64_t)(kvh * group + h) * p.ldqh, d0, HD, p.rope, rot0 + i);
+      x = make_uint4(x.x ^ p.q_sign, x.y ^ p.q_sign, x.z ^ p.q_sign, x.w ^ p.q_sign);
+      const int c = d0 / 8, tr = r & (kPrTile - 1);
+      *reinterpret_cast<uint4*>(pp_smem + S::kQ + r / kPrTile * S::kQTile + c / 8 * (kPrTile * 128) + tr * 128 +
+                                (((c & 7) ^ (tr & 7)) << 4)) = x;
+    }
+    fence_proxy_async();
+  }
+  float vref = j1 > coded ? 1.f : 0.f;  // the tail's rows count as they are
+  for (int j = j0 + tid; j < min(j1, coded); j += kPrThreads) vref = fmaxf(vref, v_scale[j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
+  if (lane == 0) s_red[warp] = vref;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  for (int i = 0; i < kPrThreads / 32; ++i) vref = fmaxf(vref, s_red[i]);
+  if (!(vref > 0.f)) vref = 1.f;  // every value is zero
+  const uint32_t tmem = s_tmem;
+  auto wait = [&](uint32_t b_, int parity) {  // the whole warp's; false: out of time, status 1
+    return __all_sync(0xffffffffu, mbar_wait_bounded(b_, parity, p.status));
+  };
+
+  if (warp < 8) {
+    // -------------------------------------------------------------- softmax
+    const int t = warp >> 2, r = row0 + t * kPrTile + (warp & 3) * 32 + lane;
+    const int i = r / group, h = r - i * group;
+    const int stop = r < rows ? kv8_row_stop(i, len, cnt) : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_cols = tmem + lanes + (uint32_t)(t * HD);
+    const uint32_t p_row = base + S::kP + t * (kPrTile * 128) + ((warp & 3) * 32 + lane) * 128;
+    float m = -INFINITY, l = 0.f;
+    bool fine = true;
+    for (int j = 0; j < J; ++j) {
+      const int blk = j0 + j, buf = j & 1;
+      const bool is_tail = blk >= coded;
+      const float ks = is_tail ? 1.f : k_scale[blk], vs = is_tail ? 1.f : v_scale[blk];
+      const float k = (ks == 0.f ? 1.f : ks) * p.scale2;  // of zero keys the scores are zero whatever the scale
+      const float f = vs == 0.f ? 1.f : vs / vref;
+      const int nv = min(max(stop - blk * kKvBlock, 0), kKvBlock);  // positions of the block that the row attends
+      if (!wait(s_full + 8 * (2 * t + buf), (j >> 1) & 1)) {
+        fine = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s0[32], s1[32];
+      const uint32_t s_cols = tmem + lanes + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
+      tc_ld32(s_cols, s0);
+      tc_ld32(s_cols + 32, s1);
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_empty + 8 * (2 * t + buf));
+      if (__any_sync(0xffffffffu, nv < kKvBlock)) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (c >= nv) s0[c] = 0xff800000u;
+          if (c + 32 >= nv) s1[c] = 0xff800000u;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) mx = fmaxf(mx, fmaxf(__uint_as_float(s0[c]), __uint_as_float(s1[c])));
+      const float top = nv > 0 ? mx * k : -INFINITY;
+      const bool grow = top > m + kPrLag;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float to = grow ? top : m;
+        const float g = m == to || m == -INFINITY ? 1.f : ex2(m - to);  // a row without a maximum has only zeros
+        l *= g;
+        m = to;
+        if (j > 0 && __any_sync(0xffffffffu, g != 1.f)) {
+          // the products up to the last block are in O
+          if (!wait(p_empty + 8 * t, (j - 1) & 1)) {
+            fine = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tc_ld32(o_cols + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * g);
+            tc_st32(o_cols + c, o);
+          }
+          tc_wait_st();
+        }
+      }
+      const float shift = (m == -INFINITY ? 0.f : -m) + kPrLift + __log2f(f);
+      float sum = 0.f;
+      uint32_t w[32];
+      const bool masked = __any_sync(0xffffffffu, nv < kKvBlock);
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        float e0 = ex2(fmaf(__uint_as_float(s0[c]), k, shift)), e1 = ex2(fmaf(__uint_as_float(s0[c + 1]), k, shift));
+        float e2 = ex2(fmaf(__uint_as_float(s1[c]), k, shift)), e3 = ex2(fmaf(__uint_as_float(s1[c + 1]), k, shift));
+        if (masked) {
+          e0 = c < nv ? e0 : 0.f;
+          e1 = c + 1 < nv ? e1 : 0.f;
+          e2 = c + 32 < nv ? e2 : 0.f;
+          e3 = c + 33 < nv ? e3 : 0.f;
+        }
+        sum += (e0 + e1) + (e2 + e3);
+        w[c / 2] = h2u(__floats2half2_rn(e0, e1));
+        w[16 + c / 2] = h2u(__floats2half2_rn(e2, e3));
+      }
+      l = fmaf(sum, 1.f / f, l);
+      if (j > 0 && !wait(p_empty + 8 * t, (j - 1) & 1)) {
+        fine = false;
+        break;
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p_row + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]),
+                     "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3]) : "memory");
+      fence_proxy_async();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * t);
+    }
+    if (J > 0 && fine) fine = wait(p_empty + 8 * t, (J - 1) & 1);
+    tc_fence_after();
+    const bool empty = J == 0 || !fine;
+    const float inv = empty || l == 0.f ? 0.f : vref / l;
+    if (p.splits == 1) {
+      __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh;
+#pragma unroll
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (!empty) {
+          tc_ld32(o_cols + c, o);
+          tc_wait_ld();
+        }
+        if (r < rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              x[u] = empty ? 0u : h2u(__floats2half2_rn(__uint_as_float(o[e + 2 * u]) * inv,
+                                                        __uint_as_float(o[e + 2 * u + 1]) * inv));
+            *reinterpret_cast<uint4*>(out + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+    } else {
+      const int64_t at = (((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r;
+      float* rec = p.part + at * (HD + 2);
+#pragma unroll
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (!empty) {
+          tc_ld32(o_cols + c, o);
+          tc_wait_ld();
+        }
+        if (r < rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            *reinterpret_cast<float2*>(rec + c + e) =
+                empty ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[e]) * vref, __uint_as_float(o[e + 1]) * vref);
+        }
+      }
+      if (r < rows) *reinterpret_cast<float2*>(rec + HD) = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
+    }
+  } else if (warp < 12) {
+    // --------------------------------------------------------------- unpack
+    const int w = warp - 8;  // rows 32 (w & 1) + lane, sides alternately
+    const int r = (w & 1) * 32 + lane;
+    for (int j = 0; j < J; ++j) {
+      const int blk = j0 + j, buf = j & 1, st = j % kPrCodeStages;
+      const bool is_tail = blk >= coded;
+      if (!is_tail && !wait(code_full + 8 * st, (j / kPrCodeStages) & 1)) break;
+      bool fine = true;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const uint32_t empty = side ? v_empty : k_empty, full = side ? v_full : k_full;
+        if (j > 1 && !wait(empty + 8 * buf, ((j >> 1) - 1) & 1)) {
+          fine = false;
+          break;
+        }
+        const uint32_t dst = base + (side ? S::kV : S::kK) + buf * S::kKv + r * 128;
+        const uint32_t src = base + S::kCodes + (2 * st + side) * S::kCode;
+#pragma unroll
+        for (int cc = 0; cc < HD / 32; ++cc) {  // two warps share a row's 16-dimension chunks
+          const int c = 2 * cc + (w >> 1);
+          uint32_t x[8];
+          if (is_tail) {
+            uint4 a = make_uint4(0, 0, 0, 0), d = a;
+            const int t = blk * kKvBlock + r;
+            if (t < len) {
+              const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * c);
+              a = g[0];
+              d = g[1];
+            }
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = d.x, x[5] = d.y, x[6] = d.z, x[7] = d.w;
+          } else {
+            const uint4 v = lds128(src + tile_off<HD>(r, c));
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[2 * e] = codes2<0x4140>(u[e]);
+              x[2 * e + 1] = codes2<0x4342>(u[e]);
+            }
+          }
+          const uint32_t to = dst + c / 4 * (kKvBlock * 128);
+          const int ch = 2 * (c & 3);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(x[0]), "r"(x[1]),
+                       "r"(x[2]), "r"(x[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(x[4]),
+                       "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * buf);
+      }
+      if (!fine) break;
+      if (lane == 0 && !is_tail) mbar_arrive(code_empty + 8 * st);
+    }
+  } else if (warp == 12) {
+    // ----------------------------------------------------------- the products
+    if (lane == 0 && J > 0) {
+      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+      constexpr uint32_t idesc_o =
+          (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+      bool fine = true;
+      auto scores = [&](int t, int j) {
+        const int buf = j & 1;
+        if (t == 0) fine = fine && mbar_wait_bounded(k_full + 8 * buf, (j >> 1) & 1, p.status);
+        if (j > 1) fine = fine && mbar_wait_bounded(s_empty + 8 * (2 * t + buf), ((j >> 1) - 1) & 1, p.status);
+        if (!fine) return;
+        tc_fence_after();
+        const uint32_t qa = base + S::kQ + t * S::kQTile, ka = base + S::kK + buf * S::kKv;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d)
+          tc_mma(tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock),
+                 sw128_desc(qa + d / 4 * (kPrTile * 128) + d % 4 * 32, 16, 1024),
+                 sw128_desc(ka + d / 4 * (kKvBlock * 128) + d % 4 * 32, 16, 1024), idesc_s, d > 0);
+        tc_commit(s_full + 8 * (2 * t + buf));
+        if (t == 1) tc_commit(k_empty + 8 * buf);
+      };
+      scores(0, 0);
+      scores(1, 0);
+      for (int j = 0; j < J && fine; ++j)
+        for (int t = 0; t < 2 && fine; ++t) {
+          if (j + 1 < J) scores(t, j + 1);
+          const int buf = j & 1;
+          if (t == 0) fine = fine && mbar_wait_bounded(v_full + 8 * buf, (j >> 1) & 1, p.status);
+          fine = fine && mbar_wait_bounded(p_full + 8 * t, j & 1, p.status);
+          if (!fine) break;
+          tc_fence_after();
+          const uint32_t pa = base + S::kP + t * (kPrTile * 128), va = base + S::kV + buf * S::kKv;
+#pragma unroll
+          for (int x = 0; x < kKvBlock / 16; ++x)
+            tc_mma(tmem + (uint32_t)(t * HD), sw128_desc(pa + x * 32, 16, 1024),
+                   sw128_desc(va + x * 2048, kKvBlock * 128, 1024), idesc_o, j > 0 || x > 0);
+          tc_commit(p_empty + 8 * t);
+          if (t == 1) tc_commit(v_empty + 8 * buf);
+        }
+      tc_commit(done);  // no product outlives the tensor memory
+      mbar_wait_bounded(done, 0, p.status);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------ code boxes
+    const int n = min(j1, coded) - j0;
+    int issued = 0;
+    for (int j = 0; j < n; ++j, ++issued) {
+      const int st = j % kPrCodeStages;
+      if (j >= kPrCodeStages && !mbar_wait_bounded(code_empty + 8 * st, (j / kPrCodeStages - 1) & 1, p.status)) break;
+      const int y = (int)(p.c.head(b, kvh) * p.c.cap) + (j0 + j) * kKvBlock;
+      mbar_expect_tx(code_full + 8 * st, 2 * S::kCode);
+      tma_load_2d(base + S::kCodes + 2 * st * S::kCode, &tk, 0, y, code_full + 8 * st);
+      tma_load_2d(base + S::kCodes + (2 * st + 1) * S::kCode, &tv, 0, y, code_full + 8 * st);
+    }
+    for (int j = max(0, issued - kPrCodeStages); j < issued; ++j)  // none stays in flight
+      mbar_wait_bounded(code_full + 8 * (j % kPrCodeStages), (j / kPrCodeStages) & 1, p.status);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The parts of a row (splits > 1) added up in order; a warp has one row.
+struct Kv8JoinParams {
+  const float* part;
+  __half* out;
+  int64_t ldob, ldot, ldoh;
+  int batch, nkv, n, nq, splits;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8JoinParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int group = p.nq / p.nkv, rows = p.n * group;
+  const int64_t all = (int64_t)p.batch * p.nkv * rows;
+  const int64_t at = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  if (at >= all) return;
+  const int lane = threadIdx.x & 31, r = (int)(at % rows), kvh = (int)(at / rows % p.nkv), b = (int)(at / rows / p.nkv);
+  constexpr int kPer = HD / 32;
+  float m = -INFINITY, l = 0.f, o[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* rec = p.part + (s * all + at) * (HD + 2);
+    const float2 v = *reinterpret_cast<const float2*>(rec + HD);
+    const float to = fmaxf(m, v.x);
+    const float f0 = m == -INFINITY ? 1.f : ex2(m - to), f1 = v.x == -INFINITY ? 1.f : ex2(v.x - to);
+    m = to;
+    l = fmaf(l, f0, v.y * f1);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(rec + lane * 2 + 32 * e);
+      o[e] = fmaf(o[e], f0, x.x * f1);
+      o[e + 1] = fmaf(o[e + 1], f0, x.y * f1);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int i = r / group, h = r - i * group;
+  __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2)
+    *reinterpret_cast<__half2*>(out + lane * 2 + 32 * e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+}
+
+}  // namespace pp

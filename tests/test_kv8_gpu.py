@@ -217,6 +217,53 @@ def test_prompt(cuda, nq, nkv, hd, n):
     _check_out(out, want, ref)
 
 
+@pytest.mark.parametrize("nq,nkv,hd,scale", [(8, 1, 128, None), (16, 1, 64, -0.3), (10, 2, 128, 0.0)])
+def test_prompt_over_long_cache(cuda, nq, nkv, hd, scale):
+    """Few rows over many positions (split along them), odd scales, rotated queries."""
+    from polar_pack_b200.kv8 import kv8_attention
+    g = _gen(cuda, nq)
+    n, lens, counts = 20, [5000, 20, 1301, 3], [20, 20, 7, 0]
+    cache, ref = _new(4, nkv, 5056, hd, cuda), kr.RefKV(4, nkv, hd)
+    _fill(cache, ref, lens, g)
+    q = _rand(g, 4, n, nq, hd, spread=2.0)
+    cos, sin = (torch.rand(5000, hd, generator=g, device=cuda).half() for _ in "cs")
+    at = [4980, 0, 9, 1]
+    rows = (torch.tensor(at, device=cuda)[:, None] + torch.arange(n, device=cuda)).clamp(max=4999)
+    turned = kr.rope_fp16(q, cos[rows][:, :, None], sin[rows][:, :, None])
+    want, _ = kr.attention(ref, turned, counts, scale=scale)
+    for _ in range(2):
+        out = kv8_attention(q, cache, _ints(lens, cuda), counts=_ints(counts, cuda), scale=scale,
+                            rope=(cos, sin, _ints(at, cuda)))
+        _check_out(out, want, ref)
+    assert int(cache.status) == 0
+
+
+def test_prompt_rows_do_not_mix(cuda):
+    """A query of NaN changes its own row only; value blocks of very different scale."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_attention
+    g = _gen(cuda, 31)
+    n, hd, nq = 200, 128, 2
+    k, v, q = _rand(g, 1, n, 1, hd), _rand(g, 1, n, 1, hd), _rand(g, 1, n, nq, hd)
+    v[0, :64] *= 1e-4
+    v[0, 64:128] = 0
+    cache, ref = _new(1, 1, 256, hd, cuda), kr.RefKV(1, 1, hd)
+    kv8_append(cache, k, v, _ints([0], cuda))
+    ref.append(k, v, [n])
+    out = kv8_attention(q, cache, _ints([n], cuda))
+    want, _ = kr.attention(ref, q, [n])
+    vv = ref.s[1][0][0].values()
+    # a row's weights are FP16 beside the largest scale of the block range: for the first rows, whose values
+    # are 1e-4 of the last ones, their rounding is still relative (2^11 lifts them above FP16's smallest)
+    for i in range(n):
+        bound = OUT_TOL * float(vv[:i + 1].abs().max()) + 2.0 ** -24
+        assert ((out[0, i].cpu().double() - want[0, i]).abs() <= bound).all(), i
+    q[0, 77, 1] = float("nan")
+    bad = kv8_attention(q, cache, _ints([n], cuda))
+    same = torch.ones(n, nq, dtype=torch.bool, device=cuda)
+    same[77, 1] = False
+    assert torch.equal(bad[0][same], out[0][same]) and torch.isnan(bad[0, 77, 1]).all()
+
+
 @pytest.mark.parametrize("nq,nkv,hd", [(16, 2, 128), (7, 1, 64), (16, 1, 128)])
 def test_decode_steps(cuda, nq, nkv, hd):
     """Steps across a block's end: outputs, cache and accumulated weights."""
