@@ -14,11 +14,11 @@
 // head's group) as two tiles of 128, so that one tile's softmax runs while the
 // other's products do, and each block is unpacked once for both.  Roles:
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row; S from tensor
-//                    memory, P to shared memory, O rescaled in tensor memory
-//                    when its row's maximum moved, the result at the end
+//                    memory, P over it, O rescaled in tensor memory when its
+//                    row's maximum moved, the result at the end
 //   warps 8-11       unpack a block's codes (arrived by TMA) to FP16 tiles
-//   warp 12          issues the products: S = Q K^T (M 128, N 64) a block ahead
-//                    of O += P V (M 128, N head_dim)
+//   warp 12          issues the products: S = Q K^T (M 128, N 64) two blocks
+//                    ahead of O += P V (M 128, N head_dim, P from tensor memory)
 //   warp 13          the code boxes' TMA
 // K and V tiles have the same layout, positions x dimensions in 128-byte
 // swizzled rows: K-major for the first product, MN-major for the second.
@@ -33,8 +33,8 @@ namespace pp {
 
 constexpr int kPrRows = 256;                  // query rows of a CTA
 constexpr int kPrTile = 128;                  // rows of one MMA
-constexpr int kPrThreads = 14 * 32;
-constexpr int kPrCodeStages = 3;
+constexpr int kPrThreads = 16 * 32;           // two warps have no role
+constexpr int kPrCodeStages = 4;
 constexpr float kPrLag = 4.f;                 // log2 growth of a maximum that rescales
 constexpr float kPrLift = 11.f;               // log2 factor of the FP16 weights
 
@@ -64,8 +64,7 @@ struct Kv8PromptSmem {
   static constexpr int kQ = 0;
   static constexpr int kK = 2 * kQTile;                          // two buffers each
   static constexpr int kV = kK + 2 * kKv;
-  static constexpr int kP = kV + 2 * kKv;                        // one per row tile
-  static constexpr int kCodes = kP + 2 * kPrTile * 128;
+  static constexpr int kCodes = kV + 2 * kKv;
   static constexpr int kBar = kCodes + kPrCodeStages * 2 * kCode;
   static constexpr int kBytes = kBar + 256;
 };
@@ -78,7 +77,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     kv8_prompt_kernel(const __grid_constant__ Kv8PromptParams p, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
   using S = Kv8PromptSmem<HD>;
-  __shared__ float s_red[14];
+  __shared__ float s_red[kPrThreads / 32];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
@@ -88,11 +87,12 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const int group = p.nq / p.c.nkv, rows = p.n * group, row0 = tile * kPrRows;
   // barriers
   const uint32_t bar = base + S::kBar;
-  const uint32_t code_full = bar, code_empty = bar + 24;           // [3]
-  const uint32_t k_full = bar + 48, k_empty = bar + 64;            // [2]
-  const uint32_t v_full = bar + 80, v_empty = bar + 96;            // [2]
-  const uint32_t s_full = bar + 112, s_empty = bar + 144;          // [tile][2]
-  const uint32_t p_full = bar + 176, p_empty = bar + 192;          // [tile]
+  const uint32_t code_full = bar, code_empty = bar + 32;           // [4]
+  const uint32_t k_full = bar + 64, k_empty = bar + 80;            // [2]
+  const uint32_t v_full = bar + 96, v_empty = bar + 112;           // [2]
+  const uint32_t s_full = bar + 128;                               // [tile][2]
+  const uint32_t p_full = bar + 160;                               // [tile][2]
+  const uint32_t o_full = bar + 192;                               // [tile]
   const uint32_t done = bar + 208;
   if (tid == 0) {
     for (int i = 0; i < kPrCodeStages; ++i) {
@@ -104,12 +104,11 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(k_empty + 8 * i, 1);
       mbar_init(v_full + 8 * i, 4);
       mbar_init(v_empty + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 4);
-      mbar_init(p_empty + 8 * i, 1);
+      mbar_init(o_full + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(s_empty + 8 * i, 4);
+      mbar_init(p_full + 8 * i, 4);
     }
     mbar_init(done, 1);
     fence_mbar_init();
@@ -164,51 +163,54 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   for (int i = 0; i < kPrThreads / 32; ++i) vref = fmaxf(vref, s_red[i]);
   if (!(vref > 0.f)) vref = 1.f;  // every value is zero
   const uint32_t tmem = s_tmem;
-  auto wait = [&](uint32_t b_, int parity) {  // the whole warp's; false: out of time, status 1
-    return __all_sync(0xffffffffu, mbar_wait_bounded(b_, parity, p.status));
-  };
+  auto wait = [&](uint32_t b_, int parity) { return mbar_wait_warp(b_, parity, p.status); };
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");  // 256 x 176 + 256 x 80 = 512 x 128 registers
     // -------------------------------------------------------------- softmax
     const int t = warp >> 2, r = row0 + t * kPrTile + (warp & 3) * 32 + lane;
     const int i = r / group, h = r - i * group;
     const int stop = r < rows ? kv8_row_stop(i, len, cnt) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_cols = tmem + lanes + (uint32_t)(t * HD);
-    const uint32_t p_row = base + S::kP + t * (kPrTile * 128) + ((warp & 3) * 32 + lane) * 128;
     float m = -INFINITY, l = 0.f;
+    const float per_vref = 1.f / vref;
+    float ks = 1.f, vs = 1.f;  // of the next block
+    if (J > 0 && j0 < coded) {
+      ks = k_scale[j0];
+      vs = v_scale[j0];
+    }
     bool fine = true;
+#pragma unroll 1
     for (int j = 0; j < J; ++j) {
       const int blk = j0 + j, buf = j & 1;
-      const bool is_tail = blk >= coded;
-      const float ks = is_tail ? 1.f : k_scale[blk], vs = is_tail ? 1.f : v_scale[blk];
       const float k = (ks == 0.f ? 1.f : ks) * p.scale2;  // of zero keys the scores are zero whatever the scale
-      const float f = vs == 0.f ? 1.f : vs / vref;
+      const float log_f = vs == 0.f ? 0.f : __log2f(vs * per_vref);
+      ks = vs = 1.f;
+      if (blk + 1 < min(j1, coded)) {
+        ks = k_scale[blk + 1];
+        vs = v_scale[blk + 1];
+      }
       const int nv = min(max(stop - blk * kKvBlock, 0), kKvBlock);  // positions of the block that the row attends
-      if (!wait(s_full + 8 * (2 * t + buf), (j >> 1) & 1)) {
-        fine = false;
-        break;
-      }
+      const bool masked = __any_sync(0xffffffffu, nv < kKvBlock);
+      if (!(fine = wait(s_full + 8 * (2 * t + buf), (j >> 1) & 1))) break;
       tc_fence_after();
-      uint32_t s0[32], s1[32];
+      uint32_t s[kKvBlock];
       const uint32_t s_cols = tmem + lanes + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
-      tc_ld32(s_cols, s0);
-      tc_ld32(s_cols + 32, s1);
-      tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty + 8 * (2 * t + buf));
-      if (__any_sync(0xffffffffu, nv < kKvBlock)) {
+      tc_ld64(s_cols, s);
+      if (masked) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (c >= nv) s0[c] = 0xff800000u;
-          if (c + 32 >= nv) s1[c] = 0xff800000u;
-        }
+        for (int c = 0; c < kKvBlock; ++c)
+          if (c >= nv) s[c] = 0xff800000u;
       }
-      float mx = -INFINITY;
+      float mx[4];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) mx = fmaxf(mx, fmaxf(__uint_as_float(s0[c]), __uint_as_float(s1[c])));
-      const float top = nv > 0 ? mx * k : -INFINITY;
+      for (int u = 0; u < 4; ++u) {
+        mx[u] = __uint_as_float(s[16 * u]);
+#pragma unroll
+        for (int c = 1; c < 16; ++c) mx[u] = fmaxf(mx[u], __uint_as_float(s[16 * u + c]));
+      }
+      const float top = nv > 0 ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k : -INFINITY;
       const bool grow = top > m + kPrLag;
       if (__any_sync(0xffffffffu, grow)) {
         const float to = grow ? top : m;
@@ -216,57 +218,41 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         l *= g;
         m = to;
         if (j > 0 && __any_sync(0xffffffffu, g != 1.f)) {
-          // the products up to the last block are in O
-          if (!wait(p_empty + 8 * t, (j - 1) & 1)) {
-            fine = false;
-            break;
-          }
+          if (!(fine = wait(o_full + 8 * t, (j - 1) & 1))) break;  // the products up to the last block are in O
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
             tc_ld32(o_cols + c, o);
-            tc_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * g);
             tc_st32(o_cols + c, o);
           }
-          tc_wait_st();
         }
       }
-      const float shift = (m == -INFINITY ? 0.f : -m) + kPrLift + __log2f(f);
-      float sum = 0.f;
-      uint32_t w[32];
-      const bool masked = __any_sync(0xffffffffu, nv < kKvBlock);
+      const float shift = (m == -INFINITY ? 0.f : -m) + kPrLift + log_f;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t w[32];  // the row's weights, over the scores' first columns
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        float e0 = ex2(fmaf(__uint_as_float(s0[c]), k, shift)), e1 = ex2(fmaf(__uint_as_float(s0[c + 1]), k, shift));
-        float e2 = ex2(fmaf(__uint_as_float(s1[c]), k, shift)), e3 = ex2(fmaf(__uint_as_float(s1[c + 1]), k, shift));
-        if (masked) {
-          e0 = c < nv ? e0 : 0.f;
-          e1 = c + 1 < nv ? e1 : 0.f;
-          e2 = c + 32 < nv ? e2 : 0.f;
-          e3 = c + 33 < nv ? e3 : 0.f;
+      for (int c = 0; c < kKvBlock; c += 4) {
+        float e[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          e[u] = ex2(fmaf(__uint_as_float(s[c + u]), k, shift));
+          if (masked) e[u] = c + u < nv ? e[u] : 0.f;
+          sum[u] += e[u];
         }
-        sum += (e0 + e1) + (e2 + e3);
-        w[c / 2] = h2u(__floats2half2_rn(e0, e1));
-        w[16 + c / 2] = h2u(__floats2half2_rn(e2, e3));
+        w[c / 2] = h2u(__floats2half2_rn(e[0], e[1]));
+        w[c / 2 + 1] = h2u(__floats2half2_rn(e[2], e[3]));
       }
-      l = fmaf(sum, 1.f / f, l);
-      if (j > 0 && !wait(p_empty + 8 * t, (j - 1) & 1)) {
-        fine = false;
-        break;
-      }
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(p_row + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]),
-                     "r"(w[4 * c + 1]), "r"(w[4 * c + 2]), "r"(w[4 * c + 3]) : "memory");
-      fence_proxy_async();
+      tc_st32(s_cols, w);
+      l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ex2(-log_f), l);
+      tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * t);
+      if (lane == 0) mbar_arrive(p_full + 8 * (2 * t + buf));
     }
-    if (J > 0 && fine) fine = wait(p_empty + 8 * t, (J - 1) & 1);
+    if (J > 0 && fine) fine = wait(done, 0);  // o_full may be one or two phases on: its parity does not tell
     tc_fence_after();
     const bool empty = J == 0 || !fine;
     const float inv = empty || l == 0.f ? 0.f : vref / l;
@@ -277,7 +263,6 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         uint32_t o[32];
         if (!empty) {
           tc_ld32(o_cols + c, o);
-          tc_wait_ld();
         }
         if (r < rows) {
 #pragma unroll
@@ -299,7 +284,6 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         uint32_t o[32];
         if (!empty) {
           tc_ld32(o_cols + c, o);
-          tc_wait_ld();
         }
         if (r < rows) {
 #pragma unroll
@@ -310,104 +294,135 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       }
       if (r < rows) *reinterpret_cast<float2*>(rec + HD) = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
     }
-  } else if (warp < 12) {
+  } else {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+   if (warp < 12) {
     // --------------------------------------------------------------- unpack
-    const int w = warp - 8;  // rows 32 (w & 1) + lane, sides alternately
+    const int w = warp - 8;  // rows 32 (w & 1) + lane, sixteen-dimension chunks of parity w >> 1
     const int r = (w & 1) * 32 + lane;
-    for (int j = 0; j < J; ++j) {
-      const int blk = j0 + j, buf = j & 1, st = j % kPrCodeStages;
-      const bool is_tail = blk >= coded;
-      if (!is_tail && !wait(code_full + 8 * st, (j / kPrCodeStages) & 1)) break;
-      bool fine = true;
+    constexpr int kChunks = HD / 32;
+    // a tile's rows into registers, then as FP16 into its buffer
+    auto read = [&](int side, int j, uint4 (&x)[kChunks]) {
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const uint32_t empty = side ? v_empty : k_empty, full = side ? v_full : k_full;
-        if (j > 1 && !wait(empty + 8 * buf, ((j >> 1) - 1) & 1)) {
-          fine = false;
-          break;
+      for (int cc = 0; cc < kChunks; ++cc)
+        x[cc] = lds128(base + S::kCodes + (2 * (j % kPrCodeStages) + side) * S::kCode + tile_off<HD>(r, 2 * cc + (w >> 1)));
+    };
+    auto put = [&](int side, int j, int c, uint4 lo, uint4 hi) {
+      const uint32_t to = base + (side ? S::kV : S::kK) + (j & 1) * S::kKv + c / 4 * (kKvBlock * 128) + r * 128;
+      const int ch = 2 * (c & 3);
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(lo.x), "r"(lo.y),
+                   "r"(lo.z), "r"(lo.w) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(hi.x), "r"(hi.y),
+                   "r"(hi.z), "r"(hi.w) : "memory");
+    };
+    auto write = [&](int side, int j, const uint4 (&x)[kChunks]) {
+#pragma unroll
+      for (int cc = 0; cc < kChunks; ++cc)
+        put(side, j, 2 * cc + (w >> 1),
+            make_uint4(codes2<0x4140>(x[cc].x), codes2<0x4342>(x[cc].x), codes2<0x4140>(x[cc].y), codes2<0x4342>(x[cc].y)),
+            make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w), codes2<0x4342>(x[cc].w)));
+    };
+    auto write_tail = [&](int side, int j) {  // FP16 rows from memory, zero past the end
+#pragma unroll
+      for (int cc = 0; cc < kChunks; ++cc) {
+        const int c = 2 * cc + (w >> 1);
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if ((j0 + j) * kKvBlock + r < len) {
+          const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * c);
+          lo = g[0];
+          hi = g[1];
         }
-        const uint32_t dst = base + (side ? S::kV : S::kK) + buf * S::kKv + r * 128;
-        const uint32_t src = base + S::kCodes + (2 * st + side) * S::kCode;
-#pragma unroll
-        for (int cc = 0; cc < HD / 32; ++cc) {  // two warps share a row's 16-dimension chunks
-          const int c = 2 * cc + (w >> 1);
-          uint32_t x[8];
-          if (is_tail) {
-            uint4 a = make_uint4(0, 0, 0, 0), d = a;
-            const int t = blk * kKvBlock + r;
-            if (t < len) {
-              const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * c);
-              a = g[0];
-              d = g[1];
-            }
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = d.x, x[5] = d.y, x[6] = d.z, x[7] = d.w;
-          } else {
-            const uint4 v = lds128(src + tile_off<HD>(r, c));
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[2 * e] = codes2<0x4140>(u[e]);
-              x[2 * e + 1] = codes2<0x4342>(u[e]);
-            }
-          }
-          const uint32_t to = dst + c / 4 * (kKvBlock * 128);
-          const int ch = 2 * (c & 3);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(x[0]), "r"(x[1]),
-                       "r"(x[2]), "r"(x[3]) : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(x[4]),
-                       "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + 8 * buf);
+        put(side, j, c, lo, hi);
       }
-      if (!fine) break;
-      if (lane == 0 && !is_tail) mbar_arrive(code_empty + 8 * st);
+    };
+    // keys run two blocks ahead of values
+#pragma unroll 1
+    for (int j = -2; j < J; ++j) {
+      const int jv = j, jk = j + 2;
+      const bool do_v = jv >= 0, do_k = jk < J, tail_v = j0 + jv >= coded, tail_k = j0 + jk >= coded;
+      bool fine = true;
+      uint4 xv[kChunks], xk[kChunks];
+      if (do_v && !tail_v) read(1, jv, xv);  // arrived: its keys were read two blocks ago
+      if (do_k && !tail_k) {
+        fine = wait(code_full + 8 * (jk % kPrCodeStages), (jk / kPrCodeStages) & 1);
+        read(0, jk, xk);
+      }
+      if (do_v) {
+        if (jv > 1) fine = fine && wait(v_empty + 8 * (jv & 1), ((jv >> 1) - 1) & 1);
+        if (!fine) break;
+        if (tail_v) write_tail(1, jv);
+        else write(1, jv, xv);
+      }
+      if (do_k) {
+        if (jk > 1) fine = fine && wait(k_empty + 8 * (jk & 1), ((jk >> 1) - 1) & 1);
+        if (!fine) break;
+        if (tail_k) write_tail(0, jk);
+        else write(0, jk, xk);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (do_v) mbar_arrive(v_full + 8 * (jv & 1));
+        if (do_k) mbar_arrive(k_full + 8 * (jk & 1));
+        if (do_v && !tail_v) mbar_arrive(code_empty + 8 * (jv % kPrCodeStages));
+      }
     }
   } else if (warp == 12) {
     // ----------------------------------------------------------- the products
-    if (lane == 0 && J > 0) {
+    if (J > 0) {
       constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
       constexpr uint32_t idesc_o =
           (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+      // descriptors of the tiles; offsets within them add to the address field
+      const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
+      const uint64_t v_desc = sw128_desc(base + S::kV, kKvBlock * 128, 1024);
       bool fine = true;
       auto scores = [&](int t, int j) {
         const int buf = j & 1;
-        if (t == 0) fine = fine && mbar_wait_bounded(k_full + 8 * buf, (j >> 1) & 1, p.status);
-        if (j > 1) fine = fine && mbar_wait_bounded(s_empty + 8 * (2 * t + buf), ((j >> 1) - 1) & 1, p.status);
+        if (t == 0) fine = fine && wait(k_full + 8 * buf, (j >> 1) & 1);
         if (!fine) return;
         tc_fence_after();
-        const uint32_t qa = base + S::kQ + t * S::kQTile, ka = base + S::kK + buf * S::kKv;
+        if (elect_one()) {
+          const uint64_t qd = q_desc + (uint32_t)(t * (S::kQTile >> 4)), kd = k_desc + (uint32_t)(buf * (S::kKv >> 4));
+          const uint32_t dst = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d)
-          tc_mma(tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock),
-                 sw128_desc(qa + d / 4 * (kPrTile * 128) + d % 4 * 32, 16, 1024),
-                 sw128_desc(ka + d / 4 * (kKvBlock * 128) + d % 4 * 32, 16, 1024), idesc_s, d > 0);
-        tc_commit(s_full + 8 * (2 * t + buf));
-        if (t == 1) tc_commit(k_empty + 8 * buf);
-      };
-      scores(0, 0);
-      scores(1, 0);
-      for (int j = 0; j < J && fine; ++j)
-        for (int t = 0; t < 2 && fine; ++t) {
-          if (j + 1 < J) scores(t, j + 1);
-          const int buf = j & 1;
-          if (t == 0) fine = fine && mbar_wait_bounded(v_full + 8 * buf, (j >> 1) & 1, p.status);
-          fine = fine && mbar_wait_bounded(p_full + 8 * t, j & 1, p.status);
-          if (!fine) break;
-          tc_fence_after();
-          const uint32_t pa = base + S::kP + t * (kPrTile * 128), va = base + S::kV + buf * S::kKv;
-#pragma unroll
-          for (int x = 0; x < kKvBlock / 16; ++x)
-            tc_mma(tmem + (uint32_t)(t * HD), sw128_desc(pa + x * 32, 16, 1024),
-                   sw128_desc(va + x * 2048, kKvBlock * 128, 1024), idesc_o, j > 0 || x > 0);
-          tc_commit(p_empty + 8 * t);
-          if (t == 1) tc_commit(v_empty + 8 * buf);
+          for (int d = 0; d < HD / 16; ++d)
+            tc_mma(dst, qd + (d / 4 * (kPrTile * 128) + d % 4 * 32 >> 4), kd + (d / 4 * (kKvBlock * 128) + d % 4 * 32 >> 4),
+                   idesc_s, d > 0);
+          tc_commit(s_full + 8 * (2 * t + buf));
+          if (t == 1) tc_commit(k_empty + 8 * buf);
         }
-      tc_commit(done);  // no product outlives the tensor memory
-      mbar_wait_bounded(done, 0, p.status);
+        __syncwarp();
+      };
+      // Scores run two blocks ahead, into the buffer whose weights the product
+      // issued just before reads: products execute in the order of issue.
+#pragma unroll 1
+      for (int j = -2; j < J && fine; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j >= 0) {
+            const int buf = j & 1;
+            if (t == 0) fine = fine && wait(v_full + 8 * buf, (j >> 1) & 1);
+            fine = fine && wait(p_full + 8 * (2 * t + buf), (j >> 1) & 1);
+            if (!fine) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vd = v_desc + (uint32_t)(buf * (S::kKv >> 4));
+              const uint32_t pa = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
+#pragma unroll
+              for (int x = 0; x < kKvBlock / 16; ++x)
+                tc_mma_ta(tmem + (uint32_t)(t * HD), pa + 8 * x, vd + (x * 2048 >> 4), idesc_o, j > 0 || x > 0);
+              tc_commit(o_full + 8 * t);
+              if (t == 1) tc_commit(v_empty + 8 * buf);
+            }
+            __syncwarp();
+          }
+          if (j + 2 < J) scores(t, j + 2);
+        }
+      if (elect_one()) tc_commit(done);
+      wait(done, 0);  // no product outlives the tensor memory
     }
-  } else if (lane == 0) {
+  } else if (warp == 13 && lane == 0) {
     // ------------------------------------------------------------ code boxes
     const int n = min(j1, coded) - j0;
     int issued = 0;
@@ -421,6 +436,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     }
     for (int j = max(0, issued - kPrCodeStages); j < issued; ++j)  // none stays in flight
       mbar_wait_bounded(code_full + 8 * (j % kPrCodeStages), (j / kPrCodeStages) & 1, p.status);
+   }
   }
   tc_fence_before();
   __syncthreads();
