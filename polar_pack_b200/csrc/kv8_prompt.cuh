@@ -16,10 +16,11 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row; S from tensor
 //                    memory, P over it, O rescaled in tensor memory when its
 //                    row's maximum moved, the result at the end
-//   warps 8-11       unpack a block's codes (arrived by TMA) to FP16 tiles
-//   warp 12          issues the products: S = Q K^T (M 128, N 64) two blocks
-//                    ahead of O += P V (M 128, N head_dim, P from tensor memory)
-//   warp 13          the code boxes' TMA
+//   warps 8-11       unpack a block's value codes (arrived by TMA) to FP16 tiles,
+//   warps 12-15      its key codes
+//   warp 16          issues S = Q K^T (M 128, N 64), two blocks ahead of
+//   warp 18          which issues O += P V (M 128, N head_dim, P from tensor memory)
+//   warp 17          the code boxes' TMA
 // K and V tiles have the same layout, positions x dimensions in 128-byte
 // swizzled rows: K-major for the first product, MN-major for the second.
 // Every wait is bounded; tensor memory is released on every path.
@@ -33,7 +34,7 @@ namespace pp {
 
 constexpr int kPrRows = 256;                  // query rows of a CTA
 constexpr int kPrTile = 128;                  // rows of one MMA
-constexpr int kPrThreads = 16 * 32;           // two warps have no role
+constexpr int kPrThreads = 20 * 32;           // the last warp has no role
 constexpr int kPrCodeStages = 4;
 constexpr float kPrLag = 4.f;                 // log2 growth of a maximum that rescales
 constexpr float kPrLift = 11.f;               // log2 factor of the FP16 weights
@@ -69,6 +70,26 @@ struct Kv8PromptSmem {
   static constexpr int kBytes = kBar + 256;
 };
 
+// Pairs of FP32 values, two operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Row r of a call's n * group rows: query r / group, head r % group.
 __device__ __forceinline__ int kv8_row_stop(int i, int len, int cnt) { return i < cnt ? len - cnt + i + 1 : 0; }
 
@@ -92,21 +113,21 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const uint32_t v_full = bar + 96, v_empty = bar + 112;           // [2]
   const uint32_t s_full = bar + 128;                               // [tile][2]
   const uint32_t p_full = bar + 160;                               // [tile][2]
-  const uint32_t o_full = bar + 192;                               // [tile]
-  const uint32_t done = bar + 208;
+  const uint32_t o_full = bar + 192;                               // [tile][2]
+  const uint32_t done = bar + 224;
   if (tid == 0) {
     for (int i = 0; i < kPrCodeStages; ++i) {
       mbar_init(code_full + 8 * i, 1);
-      mbar_init(code_empty + 8 * i, 4);
+      mbar_init(code_empty + 8 * i, 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + 8 * i, 4);
       mbar_init(k_empty + 8 * i, 1);
       mbar_init(v_full + 8 * i, 4);
       mbar_init(v_empty + 8 * i, 1);
-      mbar_init(o_full + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) {
+      mbar_init(o_full + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 4);
     }
@@ -115,7 +136,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc((uint32_t)__cvta_generic_to_shared(&s_tmem), 512);
     tmem_relinquish();
   }
@@ -166,7 +187,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   auto wait = [&](uint32_t b_, int parity) { return mbar_wait_warp(b_, parity, p.status); };
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");  // 256 x 176 + 256 x 80 = 512 x 128 registers
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");  // 256 x 144 + 384 x 64 = 640 x 96 registers
     // -------------------------------------------------------------- softmax
     const int t = warp >> 2, r = row0 + t * kPrTile + (warp & 3) * 32 + lane;
     const int i = r / group, h = r - i * group;
@@ -184,7 +205,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 #pragma unroll 1
     for (int j = 0; j < J; ++j) {
       const int blk = j0 + j, buf = j & 1;
-      const float k = (ks == 0.f ? 1.f : ks) * p.scale2;  // of zero keys the scores are zero whatever the scale
+      const float k = fmaxf(ks * p.scale2, 1e-30f);  // positive: a masked score stays -inf
       const float log_f = vs == 0.f ? 0.f : __log2f(vs * per_vref);
       ks = vs = 1.f;
       if (blk + 1 < min(j1, coded)) {
@@ -195,22 +216,28 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       const bool masked = __any_sync(0xffffffffu, nv < kKvBlock);
       if (!(fine = wait(s_full + 8 * (2 * t + buf), (j >> 1) & 1))) break;
       tc_fence_after();
-      uint32_t s[kKvBlock];
       const uint32_t s_cols = tmem + lanes + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
-      tc_ld64(s_cols, s);
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kKvBlock; ++c)
-          if (c >= nv) s[c] = 0xff800000u;
-      }
+      // the maximum first; the scores are read again for the weights, half a row
+      // at a time (64 registers fewer)
       float mx[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        mx[u] = __uint_as_float(s[16 * u]);
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32];
+        tc_ld32(s_cols + 32 * c, s);
+        if (masked) {
 #pragma unroll
-        for (int c = 1; c < 16; ++c) mx[u] = fmaxf(mx[u], __uint_as_float(s[16 * u + c]));
+          for (int u = 0; u < 32; ++u)
+            if (32 * c + u >= nv) s[u] = 0xff800000u;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float x = __uint_as_float(s[16 * u]);
+#pragma unroll
+          for (int e = 1; e < 16; ++e) x = fmaxf(x, __uint_as_float(s[16 * u + e]));
+          mx[2 * c + u] = x;
+        }
       }
-      const float top = nv > 0 ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k : -INFINITY;
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * k;
       const bool grow = top > m + kPrLag;
       if (__any_sync(0xffffffffu, grow)) {
         const float to = grow ? top : m;
@@ -218,7 +245,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         l *= g;
         m = to;
         if (j > 0 && __any_sync(0xffffffffu, g != 1.f)) {
-          if (!(fine = wait(o_full + 8 * t, (j - 1) & 1))) break;  // the products up to the last block are in O
+          // the products up to the last block are in O
+          if (!(fine = wait(o_full + 8 * (2 * t + (buf ^ 1)), ((j - 1) >> 1) & 1))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
@@ -231,28 +259,37 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         }
       }
       const float shift = (m == -INFINITY ? 0.f : -m) + kPrLift + log_f;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t w[32];  // the row's weights, over the scores' first columns
+      const uint64_t k2 = pack2(k, k), shift2 = pack2(shift, shift);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < kKvBlock; c += 4) {
-        float e[4];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], w[16];  // half a row's weights, over scores that have been read
+        tc_ld32(s_cols + 32 * c, s);
+        if (masked) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          e[u] = ex2(fmaf(__uint_as_float(s[c + u]), k, shift));
-          if (masked) e[u] = c + u < nv ? e[u] : 0.f;
-          sum[u] += e[u];
+          for (int u = 0; u < 32; ++u)
+            if (32 * c + u >= nv) s[u] = 0xff800000u;
         }
-        w[c / 2] = h2u(__floats2half2_rn(e[0], e[1]));
-        w[c / 2 + 1] = h2u(__floats2half2_rn(e[2], e[3]));
+#pragma unroll
+        for (int u = 0; u < 32; u += 2) {
+          float x, y;
+          unpack2(fma2(pack2(__uint_as_float(s[u]), __uint_as_float(s[u + 1])), k2, shift2), x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[u / 2 & 1] = add2(sum[u / 2 & 1], pack2(x, y));
+          w[u / 2] = h2u(__floats2half2_rn(x, y));
+        }
+        tc_st16(s_cols + 16 * c, w);
       }
-      tc_st32(s_cols, w);
-      l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ex2(-log_f), l);
+      float sx, sy;
+      unpack2(add2(sum[0], sum[1]), sx, sy);
+      l = fmaf(sx + sy, ex2(-log_f), l);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + 8 * (2 * t + buf));
     }
-    if (J > 0 && fine) fine = wait(done, 0);  // o_full may be one or two phases on: its parity does not tell
+    if (J > 0 && fine) fine = wait(done, 0);
     tc_fence_after();
     const bool empty = J == 0 || !fine;
     const float inv = empty || l == 0.f ? 0.f : vref / l;
@@ -295,134 +332,126 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       if (r < rows) *reinterpret_cast<float2*>(rec + HD) = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
     }
   } else {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-   if (warp < 12) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+   if (warp < 16) {
     // --------------------------------------------------------------- unpack
-    const int w = warp - 8;  // rows 32 (w & 1) + lane, sixteen-dimension chunks of parity w >> 1
+    // warps 8-11 values, 12-15 keys; rows 32 (w & 1) + lane, sixteen-dimension
+    // chunks of parity w >> 1
+    const int w = warp & 3, side = warp < 12 ? 1 : 0;
     const int r = (w & 1) * 32 + lane;
     constexpr int kChunks = HD / 32;
-    // a tile's rows into registers, then as FP16 into its buffer
-    auto read = [&](int side, int j, uint4 (&x)[kChunks]) {
+    const uint32_t full = side ? v_full : k_full, empty = side ? v_empty : k_empty;
+    const uint32_t src = base + S::kCodes + side * S::kCode, dst = base + (side ? S::kV : S::kK) + r * 128;
+#pragma unroll 1
+    for (int j = 0; j < J; ++j) {
+      const int st = j % kPrCodeStages, buf = j & 1;
+      const bool is_tail = j0 + j >= coded;
+      uint4 lo[kChunks], hi[kChunks];
+      bool fine = true;
+      if (!is_tail) {
+        fine = wait(code_full + 8 * st, (j / kPrCodeStages) & 1);
+        uint4 x[kChunks];
 #pragma unroll
-      for (int cc = 0; cc < kChunks; ++cc)
-        x[cc] = lds128(base + S::kCodes + (2 * (j % kPrCodeStages) + side) * S::kCode + tile_off<HD>(r, 2 * cc + (w >> 1)));
-    };
-    auto put = [&](int side, int j, int c, uint4 lo, uint4 hi) {
-      const uint32_t to = base + (side ? S::kV : S::kK) + (j & 1) * S::kKv + c / 4 * (kKvBlock * 128) + r * 128;
-      const int ch = 2 * (c & 3);
-      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(lo.x), "r"(lo.y),
-                   "r"(lo.z), "r"(lo.w) : "memory");
-      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(hi.x), "r"(hi.y),
-                   "r"(hi.z), "r"(hi.w) : "memory");
-    };
-    auto write = [&](int side, int j, const uint4 (&x)[kChunks]) {
+        for (int cc = 0; cc < kChunks; ++cc)
+          x[cc] = lds128(src + 2 * st * S::kCode + tile_off<HD>(r, 2 * cc + (w >> 1)));
 #pragma unroll
-      for (int cc = 0; cc < kChunks; ++cc)
-        put(side, j, 2 * cc + (w >> 1),
-            make_uint4(codes2<0x4140>(x[cc].x), codes2<0x4342>(x[cc].x), codes2<0x4140>(x[cc].y), codes2<0x4342>(x[cc].y)),
-            make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w), codes2<0x4342>(x[cc].w)));
-    };
-    auto write_tail = [&](int side, int j) {  // FP16 rows from memory, zero past the end
+        for (int cc = 0; cc < kChunks; ++cc) {
+          lo[cc] = make_uint4(codes2<0x4140>(x[cc].x), codes2<0x4342>(x[cc].x), codes2<0x4140>(x[cc].y),
+                              codes2<0x4342>(x[cc].y));
+          hi[cc] = make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w),
+                              codes2<0x4342>(x[cc].w));
+        }
+      } else {  // FP16 rows from memory, zero past the end
+#pragma unroll
+        for (int cc = 0; cc < kChunks; ++cc) {
+          lo[cc] = hi[cc] = make_uint4(0, 0, 0, 0);
+          if ((j0 + j) * kKvBlock + r < len) {
+            const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * (2 * cc + (w >> 1)));
+            lo[cc] = g[0];
+            hi[cc] = g[1];
+          }
+        }
+      }
+      if (j > 1) fine = fine && wait(empty + 8 * buf, ((j >> 1) - 1) & 1);
+      if (!fine) break;
 #pragma unroll
       for (int cc = 0; cc < kChunks; ++cc) {
-        const int c = 2 * cc + (w >> 1);
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if ((j0 + j) * kKvBlock + r < len) {
-          const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * c);
-          lo = g[0];
-          hi = g[1];
-        }
-        put(side, j, c, lo, hi);
-      }
-    };
-    // keys run two blocks ahead of values
-#pragma unroll 1
-    for (int j = -2; j < J; ++j) {
-      const int jv = j, jk = j + 2;
-      const bool do_v = jv >= 0, do_k = jk < J, tail_v = j0 + jv >= coded, tail_k = j0 + jk >= coded;
-      bool fine = true;
-      uint4 xv[kChunks], xk[kChunks];
-      if (do_v && !tail_v) read(1, jv, xv);  // arrived: its keys were read two blocks ago
-      if (do_k && !tail_k) {
-        fine = wait(code_full + 8 * (jk % kPrCodeStages), (jk / kPrCodeStages) & 1);
-        read(0, jk, xk);
-      }
-      if (do_v) {
-        if (jv > 1) fine = fine && wait(v_empty + 8 * (jv & 1), ((jv >> 1) - 1) & 1);
-        if (!fine) break;
-        if (tail_v) write_tail(1, jv);
-        else write(1, jv, xv);
-      }
-      if (do_k) {
-        if (jk > 1) fine = fine && wait(k_empty + 8 * (jk & 1), ((jk >> 1) - 1) & 1);
-        if (!fine) break;
-        if (tail_k) write_tail(0, jk);
-        else write(0, jk, xk);
+        const int c = 2 * cc + (w >> 1), ch = 2 * (c & 3);
+        const uint32_t to = dst + buf * S::kKv + c / 4 * (kKvBlock * 128);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(lo[cc].x),
+                     "r"(lo[cc].y), "r"(lo[cc].z), "r"(lo[cc].w) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(hi[cc].x),
+                     "r"(hi[cc].y), "r"(hi[cc].z), "r"(hi[cc].w) : "memory");
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        if (do_v) mbar_arrive(v_full + 8 * (jv & 1));
-        if (do_k) mbar_arrive(k_full + 8 * (jk & 1));
-        if (do_v && !tail_v) mbar_arrive(code_empty + 8 * (jv % kPrCodeStages));
+        mbar_arrive(full + 8 * buf);
+        if (!is_tail) mbar_arrive(code_empty + 8 * st);
       }
     }
-  } else if (warp == 12) {
-    // ----------------------------------------------------------- the products
-    if (J > 0) {
-      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
-      constexpr uint32_t idesc_o =
-          (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
-      // descriptors of the tiles; offsets within them add to the address field
-      const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
-      const uint64_t v_desc = sw128_desc(base + S::kV, kKvBlock * 128, 1024);
-      bool fine = true;
-      auto scores = [&](int t, int j) {
-        const int buf = j & 1;
-        if (t == 0) fine = fine && wait(k_full + 8 * buf, (j >> 1) & 1);
-        if (!fine) return;
+  } else if (warp == 16) {
+    // ------------------------------------------------------------- S = Q K^T
+    // Two blocks ahead of the second product, into the buffer whose weights it
+    // has read.  Descriptors' offsets within a tile add to their address field.
+    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+    const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
+    bool fine = true;
+#pragma unroll 1
+    for (int j = 0; j < J && fine; ++j) {
+      const int buf = j & 1;
+      const uint64_t kd = k_desc + (uint32_t)(buf * (S::kKv >> 4));
+      fine = wait(k_full + 8 * buf, (j >> 1) & 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (j > 1) fine = fine && wait(o_full + 8 * (2 * t + buf), ((j >> 1) - 1) & 1);
+        if (!fine) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t qd = q_desc + (uint32_t)(t * (S::kQTile >> 4)), kd = k_desc + (uint32_t)(buf * (S::kKv >> 4));
+          const uint64_t qd = q_desc + (uint32_t)(t * (S::kQTile >> 4));
           const uint32_t dst = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
 #pragma unroll
           for (int d = 0; d < HD / 16; ++d)
             tc_mma(dst, qd + (d / 4 * (kPrTile * 128) + d % 4 * 32 >> 4), kd + (d / 4 * (kKvBlock * 128) + d % 4 * 32 >> 4),
-                   idesc_s, d > 0);
+                   idesc, d > 0);
           tc_commit(s_full + 8 * (2 * t + buf));
           if (t == 1) tc_commit(k_empty + 8 * buf);
         }
         __syncwarp();
-      };
-      // Scores run two blocks ahead, into the buffer whose weights the product
-      // issued just before reads: products execute in the order of issue.
-#pragma unroll 1
-      for (int j = -2; j < J && fine; ++j)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= 0) {
-            const int buf = j & 1;
-            if (t == 0) fine = fine && wait(v_full + 8 * buf, (j >> 1) & 1);
-            fine = fine && wait(p_full + 8 * (2 * t + buf), (j >> 1) & 1);
-            if (!fine) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vd = v_desc + (uint32_t)(buf * (S::kKv >> 4));
-              const uint32_t pa = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
-#pragma unroll
-              for (int x = 0; x < kKvBlock / 16; ++x)
-                tc_mma_ta(tmem + (uint32_t)(t * HD), pa + 8 * x, vd + (x * 2048 >> 4), idesc_o, j > 0 || x > 0);
-              tc_commit(o_full + 8 * t);
-              if (t == 1) tc_commit(v_empty + 8 * buf);
-            }
-            __syncwarp();
-          }
-          if (j + 2 < J) scores(t, j + 2);
-        }
-      if (elect_one()) tc_commit(done);
-      wait(done, 0);  // no product outlives the tensor memory
+      }
     }
-  } else if (warp == 13 && lane == 0) {
+    if (J > 0) wait(done, 0);  // no product outlives the tensor memory
+  } else if (warp == 18) {
+    // --------------------------------------------------------------- O += P V
+    constexpr uint32_t idesc =
+        (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+    const uint64_t v_desc = sw128_desc(base + S::kV, kKvBlock * 128, 1024);
+    bool fine = true;
+#pragma unroll 1
+    for (int j = 0; j < J && fine; ++j) {
+      const int buf = j & 1;
+      const uint64_t vd = v_desc + (uint32_t)(buf * (S::kKv >> 4));
+      fine = wait(v_full + 8 * buf, (j >> 1) & 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        fine = fine && wait(p_full + 8 * (2 * t + buf), (j >> 1) & 1);
+        if (!fine) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t pa = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
+#pragma unroll
+          for (int x = 0; x < kKvBlock / 16; ++x)
+            tc_mma_ta(tmem + (uint32_t)(t * HD), pa + 8 * x, vd + (x * 2048 >> 4), idesc, j > 0 || x > 0);
+          tc_commit(o_full + 8 * (2 * t + buf));
+          if (t == 1) tc_commit(v_empty + 8 * buf);
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) tc_commit(done);
+    __syncwarp();
+    wait(done, 0);
+  } else if (warp == 17 && lane == 0) {
     // ------------------------------------------------------------ code boxes
     const int n = min(j1, coded) - j0;
     int issued = 0;
@@ -440,7 +469,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
