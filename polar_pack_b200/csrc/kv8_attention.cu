@@ -96,7 +96,7 @@ int launch_prompt(const Kv8PromptParams& p, cudaStream_t s) {
   }
   CUtensorMap tm[2];
   if (int rc = encode_codes(p.c, tm)) return rc;
-  const dim3 grid((unsigned)(p.tiles * p.splits), (unsigned)p.c.nkv, (unsigned)p.c.batch);
+  const dim3 grid((unsigned)(p.c.nkv * p.c.batch), (unsigned)(p.tiles * p.splits));
   if (int rc = launch_kernel("kv8_prompt_kernel", launch_overlap(), kern, grid, dim3(kPrThreads), (size_t)S::kBytes, s,
                              p, tm[0], tm[1]))
     return rc;

@@ -52,7 +52,7 @@ struct Kv8PromptParams {
   uint32_t q_sign;    // 0x80008000 for a negative scale
   Kv8Rope rope;
   int tiles, splits;  // row tiles per (sequence, kv head); parts of each tile's positions
-  float* part;        // splits > 1: [splits][batch][kv head][rows][hd + 2]
+  float* part;        // splits > 1: [splits][batch][kv head][rows][hd] sums, then the same rows' (maximum, sum)
   int* status;
 };
 
@@ -98,13 +98,13 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     kv8_prompt_kernel(const __grid_constant__ Kv8PromptParams p, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
   using S = Kv8PromptSmem<HD>;
-  __shared__ float s_red[kPrThreads / 32];
+  __shared__ float s_red[8];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
-  // long tiles first: the last rows attend the most positions
-  const int tile = p.tiles - 1 - blockIdx.x / p.splits, split = blockIdx.x % p.splits;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  // long tiles first, of all heads: the last rows attend the most positions
+  const int tile = p.tiles - 1 - blockIdx.y / p.splits, split = blockIdx.y % p.splits;
+  const int kvh = blockIdx.x % p.c.nkv, b = blockIdx.x / p.c.nkv;
   const int group = p.nq / p.c.nkv, rows = p.n * group, row0 = tile * kPrRows;
   // barriers
   const uint32_t bar = base + S::kBar;
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const uint32_t s_full = bar + 128;                               // [tile][2]
   const uint32_t p_full = bar + 160;                               // [tile][2]
   const uint32_t o_full = bar + 192;                               // [tile][2]
-  const uint32_t done = bar + 224;
+  const uint32_t done = bar + 224, q_full = bar + 232;
   if (tid == 0) {
     for (int i = 0; i < kPrCodeStages; ++i) {
       mbar_init(code_full + 8 * i, 1);
@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       mbar_init(p_full + 8 * i, 4);
     }
     mbar_init(done, 1);
+    mbar_init(q_full, 8);
     fence_mbar_init();
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
@@ -159,36 +160,51 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const int coded = kv8_last_block(len);  // the block after them is the tail
   const float *k_scale = p.c.scale(0, b, kvh, 0), *v_scale = p.c.scale(1, b, kvh, 0);
 
-  // query rows to the K-major tiles; v_ref
-  if (J > 0) {
-    for (int e = tid; e < kPrRows * (HD / 8); e += kPrThreads) {
-      const int r = e / (HD / 8), d0 = e % (HD / 8) * 8, i = (row0 + r) / group, h = (row0 + r) - i * group;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (i < cnt)
-        x = kv8_load8(p.q + b * p.ldqb + i * p.ldqt + (int64_t)(kvh * group + h) * p.ldqh, d0, HD, p.rope, rot0 + i);
-      x = make_uint4(x.x ^ p.q_sign, x.y ^ p.q_sign, x.z ^ p.q_sign, x.w ^ p.q_sign);
-      const int c = d0 / 8, tr = r & (kPrTile - 1);
-      *reinterpret_cast<uint4*>(pp_smem + S::kQ + r / kPrTile * S::kQTile + c / 8 * (kPrTile * 128) + tr * 128 +
-                                (((c & 7) ^ (tr & 7)) << 4)) = x;
-    }
-    fence_proxy_async();
-  }
-  float vref = j1 > coded ? 1.f : 0.f;  // the tail's rows count as they are
-  for (int j = j0 + tid; j < min(j1, coded); j += kPrThreads) vref = fmaxf(vref, v_scale[j]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
-  if (lane == 0) s_red[warp] = vref;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  for (int i = 0; i < kPrThreads / 32; ++i) vref = fmaxf(vref, s_red[i]);
-  if (!(vref > 0.f)) vref = 1.f;  // every value is zero
   const uint32_t tmem = s_tmem;
   auto wait = [&](uint32_t b_, int parity) { return mbar_wait_warp(b_, parity, p.status); };
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");  // 256 x 144 + 384 x 64 = 640 x 96 registers
     // -------------------------------------------------------------- softmax
+    // the query rows to their tiles, K-major, while the first blocks are on their
+    // way: sixteen loads at a time; and the largest value scale of the blocks
+    float vref = j1 > coded ? 1.f : 0.f;  // the tail's rows count as they are
+    if (J > 0) {
+      constexpr int kItems = kPrRows * (HD / 8) / 256, kBatch = 16 < kItems ? 16 : kItems;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kItems; k0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int e = (k0 + k) * 256 + tid, rr = e / (HD / 8), d0 = e % (HD / 8) * 8;
+          const int qi = (row0 + rr) / group, qh = (row0 + rr) - qi * group;
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (qi < cnt)
+            x[k] = kv8_load8(p.q + b * p.ldqb + qi * p.ldqt + (int64_t)(kvh * group + qh) * p.ldqh, d0, HD, p.rope,
+                             rot0 + qi);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int e = (k0 + k) * 256 + tid, rr = e / (HD / 8), c = e % (HD / 8), tr = rr & (kPrTile - 1);
+          *reinterpret_cast<uint4*>(pp_smem + S::kQ + rr / kPrTile * S::kQTile + c / 8 * (kPrTile * 128) + tr * 128 +
+                                    (((c & 7) ^ (tr & 7)) << 4)) =
+              make_uint4(x[k].x ^ p.q_sign, x[k].y ^ p.q_sign, x[k].z ^ p.q_sign, x[k].w ^ p.q_sign);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      for (int j = j0 + tid; j < min(j1, coded); j += 256) vref = fmaxf(vref, v_scale[j]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
+    if (lane == 0) s_red[warp] = vref;
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps, all of which come here
+    for (int k = 0; k < 8; ++k) vref = fmaxf(vref, s_red[k]);
+    if (!(vref > 0.f)) vref = 1.f;  // every value is zero
     const int t = warp >> 2, r = row0 + t * kPrTile + (warp & 3) * 32 + lane;
     const int i = r / group, h = r - i * group;
     const int stop = r < rows ? kv8_row_stop(i, len, cnt) : 0;
@@ -293,44 +309,52 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     tc_fence_after();
     const bool empty = J == 0 || !fine;
     const float inv = empty || l == 0.f ? 0.f : vref / l;
-    if (p.splits == 1) {
-      __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh;
+    // The results leave by way of shared memory, which nothing else uses any
+    // more, so that a row's bytes go out side by side (a thread has a whole row).
+    const bool parts = p.splits > 1;
+    char* mine = reinterpret_cast<char*>(pp_smem) + warp * (32 * HD * 4);  // this warp's 32 rows
+    char* to = nullptr;  // where row `lane` goes
+    if (r < rows)
+      to = parts ? reinterpret_cast<char*>(p.part + ((((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r) * HD)
+                 : reinterpret_cast<char*>(p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh);
+    const int row_bytes = parts ? HD * 4 : HD * 2;
 #pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        if (!empty) {
-          tc_ld32(o_cols + c, o);
-        }
-        if (r < rows) {
+    for (int c = 0; c < HD; c += 32) {
+      uint32_t o[32];
+      if (!empty) tc_ld32(o_cols + c, o);
+      else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t x[4];
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+      }
+      if (parts) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              x[u] = empty ? 0u : h2u(__floats2half2_rn(__uint_as_float(o[e + 2 * u]) * inv,
-                                                        __uint_as_float(o[e + 2 * u + 1]) * inv));
-            *reinterpret_cast<uint4*>(out + c + e) = make_uint4(x[0], x[1], x[2], x[3]);
-          }
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4*>(mine + lane * row_bytes + (((c + e) / 4 ^ (lane & 7)) << 4)) =
+              make_float4(__uint_as_float(o[e]) * vref, __uint_as_float(o[e + 1]) * vref,
+                          __uint_as_float(o[e + 2]) * vref, __uint_as_float(o[e + 3]) * vref);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t x[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            x[u] = h2u(__floats2half2_rn(__uint_as_float(o[e + 2 * u]) * inv, __uint_as_float(o[e + 2 * u + 1]) * inv));
+          *reinterpret_cast<uint4*>(mine + lane * row_bytes + (((c + e) / 8 ^ (lane & 7)) << 4)) =
+              make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
-    } else {
-      const int64_t at = (((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r;
-      float* rec = p.part + at * (HD + 2);
-#pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        if (!empty) {
-          tc_ld32(o_cols + c, o);
-        }
-        if (r < rows) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            *reinterpret_cast<float2*>(rec + c + e) =
-                empty ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[e]) * vref, __uint_as_float(o[e + 1]) * vref);
-        }
-      }
-      if (r < rows) *reinterpret_cast<float2*>(rec + HD) = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
     }
+    __syncwarp();
+    const int chunks = row_bytes / 16;  // 8, 16 or 32: a power of two
+#pragma unroll 4
+    for (int k = lane; k < 32 * chunks; k += 32) {
+      const int rr = k / chunks, c = k % chunks;
+      char* dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), rr));
+      if (dst) *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(mine + rr * row_bytes + ((c ^ (rr & 7)) << 4));
+    }
+    if (parts && r < rows)
+      reinterpret_cast<float2*>(p.part + (int64_t)p.splits * p.c.batch * p.c.nkv * rows * HD)
+          [(((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r] = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
   } else {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
    if (warp < 16) {
@@ -396,7 +420,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     // has read.  Descriptors' offsets within a tile add to their address field.
     constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
     const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
-    bool fine = true;
+    bool fine = J == 0 || wait(q_full, 0);
 #pragma unroll 1
     for (int j = 0; j < J && fine; ++j) {
       const int buf = j & 1;
@@ -493,21 +517,41 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8JoinParams p) {
   if (at >= all) return;
   const int lane = threadIdx.x & 31, r = (int)(at % rows), kvh = (int)(at / rows % p.nkv), b = (int)(at / rows / p.nkv);
   constexpr int kPer = HD / 32;
+  const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.splits * all * HD);
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float* rec = p.part + (s * all + at) * (HD + 2);
-    const float2 v = *reinterpret_cast<const float2*>(rec + HD);
-    const float to = fmaxf(m, v.x);
-    const float f0 = m == -INFINITY ? 1.f : ex2(m - to), f1 = v.x == -INFINITY ? 1.f : ex2(v.x - to);
-    m = to;
-    l = fmaf(l, f0, v.y * f1);
+  for (int s0 = 0; s0 < p.splits; s0 += 4) {  // four parts' loads at a time
+    float2 v[4], x[4][kPer / 2];
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(rec + lane * 2 + 32 * e);
-      o[e] = fmaf(o[e], f0, x.x * f1);
-      o[e + 1] = fmaf(o[e + 1], f0, x.y * f1);
+    for (int s = 0; s < 4; ++s) {
+      v[s] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e) x[s][e] = make_float2(0.f, 0.f);
+      if (s0 + s < p.splits) {
+        v[s] = ml[(s0 + s) * all + at];
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e)
+          x[s][e] = *reinterpret_cast<const float2*>(p.part + ((s0 + s) * all + at) * HD + lane * 2 + 64 * e);
+      }
+    }
+    float to = m;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) to = fmaxf(to, v[s].x);
+    const float f0 = m == -INFINITY ? 1.f : ex2(m - to);
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] *= f0;
+    m = to;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const float f = v[s].x == -INFINITY ? 1.f : ex2(v[s].x - m);
+      l = fmaf(v[s].y, f, l);
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e) {
+        o[2 * e] = fmaf(x[s][e].x, f, o[2 * e]);
+        o[2 * e + 1] = fmaf(x[s][e].y, f, o[2 * e + 1]);
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -515,7 +559,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8JoinParams p) {
   __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2)
-    *reinterpret_cast<__half2*>(out + lane * 2 + 32 * e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+    *reinterpret_cast<__half2*>(out + lane * 2 + 32 * e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);  // e even: 64 halves apart
 }
 
 }  // namespace pp
