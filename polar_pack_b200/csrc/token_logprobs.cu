@@ -2,9 +2,26 @@
 // of rows of logits.
 //   m = max x,  Z = sum e^(x - m)
 //   logprob = x_token - m - ln Z,  entropy = ln Z - sum e^(x - m) (x - m) / Z
+// (both terms of the entropy are positive: no cancellation).
+//
+// Bound: the logits' bytes for many rows; next to them one exponential per
+// logit, 16 a clock and SM, which at the measured memory rate are three
+// quarters of the time for 2-byte logits.  One pass: a thread keeps its own
+// (maximum, Z, W = sum e^(x - m) (x - m)), moved to a new maximum when a vector
+// of logits exceeds it.  The alternatives come from the same pass: logits are
+// whole numbers (value, then lower index), all different, and those at or
+// above the row's bound go to a list in shared memory.  At least `top` logits
+// are always at or above the bound: at first it is the top-th largest of the
+// best of 64 groups of threads, later the top-th of the list, so that after
+// the first batch hardly any logit is listed.  Few rows are spread over
+// clusters of up to eight CTAs, whose results meet in the first one's shared
+// memory.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "pp_common.cuh"
 #include "pp_host.h"
@@ -12,7 +29,16 @@
 namespace pp {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBatch = 4;        // vectors of a thread in flight
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 64;      // of threads, whose best logits give the first bound
+constexpr int kList = 2048;      // keys that the list holds
+constexpr int kPrune = 128;      // a longer list is cut to the `top` largest
+constexpr float kLog2e = 1.44269504088896341f;
 
 struct ScoreParams {
   const void* x;
@@ -32,11 +58,22 @@ __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Larger values first, NaN before all, equal values by the lower index.
-__device__ __forceinline__ uint64_t rank_key(float x, int i) {
-  uint32_t u = __float_as_uint(x + 0.f);
-  u = x != x ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
-  return (uint64_t)u << 32 | (uint32_t)(0x7fffffff - i);
+using Key = unsigned long long;
+
+// Larger values first, NaN before all (-0 counts as 0).
+__device__ __forceinline__ uint32_t order(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+// Equal values by the lower index: one whole number each.
+__device__ __forceinline__ Key rank_key(float x, int i) {
+  return (Key)order(x) << 32 | (uint32_t)(0x7fffffff - i);
+}
+
+__device__ __forceinline__ float ex2a(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Sums over e^(x - m), kept beside the maximum they refer to.
@@ -44,8 +81,8 @@ struct Stat {
   float m, z, w;  // maximum, sum e^(x-m), sum e^(x-m) (x-m)
   __device__ __forceinline__ void rescale(float to) {
     if (to == m) return;
-    const float d = m - to, f = m == -INFINITY ? 0.f : expf(d);
-    w = f == 0.f ? 0.f : f * (w + d * z);
+    const float d = m - to, f = m == -INFINITY ? 0.f : ex2a(d * kLog2e);
+    w = f == 0.f ? 0.f : f * fmaf(d, z, w);
     z = f == 0.f ? 0.f : f * z;
     m = to;
   }
@@ -58,74 +95,330 @@ struct Stat {
   }
 };
 
+struct Shared {
+  Key list[kList];
+  Key kept[32];
+  Key best[kGroups];
+  Stat stat[kWarps];
+  Key bound;  // keys below it are not among the row's top
+  int count;       // listed keys
+  int held;        // of them from earlier batches
+};
+
+// A CTA's part of a row, read by the first CTA of the cluster.
+struct Result {
+  Stat stat;
+  int nan, kept;
+  Key keys[32];
+};
+
+// The `top` largest of the first n listed keys, in order, to s.kept.  Every
+// thread of the CTA comes here.
+__device__ void rank_list(Shared& s, int n, int top) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const Key k = s.list[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += s.list[j] > k;
+    if (rank < top) s.kept[rank] = k;
+  }
+  __syncthreads();
+}
+
+// The list becomes its `top` largest, in order.
+__device__ void prune(Shared& s, int top) {
+  const int n = s.count;
+  rank_list(s, n, top);
+  const int left = min(n, top);
+  if ((int)threadIdx.x < left) s.list[threadIdx.x] = s.kept[threadIdx.x];
+  if (threadIdx.x == 0) {
+    s.count = s.held = left;
+    if (left == top) s.bound = s.kept[top - 1];
+  }
+  __syncthreads();
+}
+
+// 16 bytes of logits.
 template <typename T>
+struct Vec {
+  static constexpr int kN = 16 / sizeof(T);
+  uint4 v;
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(word(i));
+    else if constexpr (std::is_same<T, __half>::value)
+      return __half2float(__ushort_as_half((unsigned short)(word(i >> 1) >> (16 * (i & 1)))));
+    else return __uint_as_float(i & 1 ? word(i >> 1) & 0xffff0000u : word(i >> 1) << 16);
+  }
+  // The largest; NaN if there is one.
+  __device__ __forceinline__ float top() const {
+    if constexpr (sizeof(T) == 4) {
+      float m = get(0);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(get(i)));
+      return m;
+    } else {
+      uint32_t m = v.x;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+        else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+      }
+      const Vec<T> r{make_uint4(m, 0, 0, 0)};
+      float a = r.get(0);
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(r.get(1)));
+      return a;
+    }
+  }
+};
+
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const ScoreParams p) {
-  __shared__ Stat st[kThreads / 32];
-  __shared__ uint64_t best[kThreads / 32];
+  __shared__ Shared s;
+  __shared__ Result mine;
+  constexpr int N = Vec<T>::kN;
   pdl_launch_dependents();
   pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  for (int64_t r = blockIdx.x / parts; r < p.rows; r += gridDim.x / parts) {
     const T* x = reinterpret_cast<const T*>(p.x) + r * p.ldx;
-    Stat s{-INFINITY, 0.f, 0.f};
-    bool nan = false;
-    for (int i = tid; i < p.vocab; i += kThreads) {
-      const float v = to_f(x[i]);
-      nan |= v != v;
-      if (v > s.m) s.rescale(v);
-      const float d = v - s.m, e = v == -INFINITY ? 0.f : expf(d);
-      s.z += e;
-      if (e > 0.f) s.w = fmaf(e, d, s.w);
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      Stat t{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.z, o),
-             __shfl_xor_sync(0xffffffffu, s.w, o)};
-      s.merge(t);
-    }
-    if (lane == 0) st[warp] = s;
-    nan = __syncthreads_or(nan);
-    s = st[0];
-    for (int i = 1; i < kThreads / 32; ++i) s.merge(st[i]);
-    float lse = s.m + logf(s.z), ent = logf(s.z) - s.w / s.z;
-    if (s.m == -INFINITY) {
-      lse = 0.f;
-      ent = 0.f;
-    }
-    if (nan || s.m == INFINITY) {
-      lse = nan ? NAN : INFINITY;
-      ent = NAN;
-    }
-    if (tid == 0) {
-      const int t = p.tokens[r];
-      p.logprob[r] = t < 0 ? 0.f : t < p.vocab ? to_f(x[t]) - lse : NAN;
-      p.entropy[r] = ent;
-      if (t >= p.vocab && p.status) atomicExch(p.status, 4);
-    }
-    uint64_t prev = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-      uint64_t b = 0;
-      for (int i = tid; i < p.vocab; i += kThreads) {
-        const uint64_t key = rank_key(to_f(x[i]), i);
-        if ((k == 0 || key < prev) && key > b) b = key;
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t c = __shfl_xor_sync(0xffffffffu, b, o);
-        b = c > b ? c : b;
-      }
-      if (lane == 0) best[warp] = b;
-      __syncthreads();
-      b = best[0];
-      for (int i = 1; i < kThreads / 32; ++i) b = best[i] > b ? best[i] : b;
-      __syncthreads();
-      prev = b;
+    // 16-byte vectors between the ends of the row that are not aligned
+    const int head = min(p.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+    const int vecs = (p.vocab - head) / N;
+    const int v0 = (int)((int64_t)vecs * part / parts), v1 = (int)((int64_t)vecs * (part + 1) / parts);
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    if (TOP) {
       if (tid == 0) {
-        const int i = 0x7fffffff - (int)(uint32_t)b;
-        p.top_ids[r * p.top + k] = i;
-        p.top_logprobs[r * p.top + k] = to_f(x[i]) - lse;
+        s.bound = 0;
+        s.count = s.held = 0;
+      }
+      __syncthreads();
+    }
+    Stat st{-INFINITY, 0.f, 0.f};
+    bool nan = false;
+    auto raise = [&](float top) {  // top: a largest logit
+      nan |= top != top;
+      if (top > st.m) st.rescale(top);
+    };
+    auto add = [&](float v) {  // a logit, after raise; -inf counts nothing
+      const float d = fmaxf(v - st.m, -200.f), e = ex2a(d * kLog2e);
+      st.z += e;
+      st.w = fmaf(e, d, st.w);
+    };
+    auto enlist = [&](float v, int i) {
+      const Key k = rank_key(v, i);
+      if (k >= s.bound) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kList) s.list[at] = k;
+      }
+    };
+    for (int b0 = v0; b0 < v1; b0 += kThreads * kBatch) {
+      Vec<T> q[kBatch];
+      float top[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = b0 + k * kThreads + tid;
+        if (i < v1) q[k].v = ldg_stream(xv + i);
+      }
+      uint32_t best = 0;  // order of this thread's best logit of the batch
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = b0 + k * kThreads + tid;
+        if (i < v1) {
+          top[k] = q[k].top();
+          raise(top[k]);
+          if (st.m > -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) add(q[k].get(e));
+          }
+          if (TOP) best = max(best, order(top[k]));
+        }
+      }
+      if constexpr (TOP) {
+        // equal logits of later batches have higher indices: only larger ones count
+        const bool has = best > (uint32_t)(s.bound >> 32);
+        const int with = __syncthreads_count(has);
+        if (with == 0) continue;
+        if (with > kGroups) {
+          // the bound, at least the top-th largest of the groups' best keys
+          Key k64 = 0;
+          if (has) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+              const int i = b0 + k * kThreads + tid;
+              if (i < v1 && order(top[k]) == best) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) k64 = max(k64, (Key)rank_key(q[k].get(e), head + i * N + e));
+              }
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < kThreads / kGroups; o <<= 1)
+            k64 = max(k64, (Key)__shfl_xor_sync(0xffffffffu, k64, o));
+          if (tid % (kThreads / kGroups) == 0) s.best[tid / (kThreads / kGroups)] = k64;
+          __syncthreads();
+          if (tid < kGroups) {
+            const Key me = s.best[tid];
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < kGroups; ++j) rank += s.best[j] > me;
+            if (rank == p.top - 1 && me > s.bound) s.bound = me;  // keys differ (empty groups: 0, never above)
+          }
+          __syncthreads();
+        }
+        for (;;) {
+          if (has) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+              const int i = b0 + k * kThreads + tid;
+              if (i < v1 && order(top[k]) >= (uint32_t)(s.bound >> 32)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) enlist(q[k].get(e), head + i * N + e);
+              }
+            }
+          }
+          __syncthreads();
+          if (s.count <= kList) break;
+          // too many: the top-th of those listed is a higher bound; list again
+          rank_list(s, kList, p.top);
+          if (tid == 0) {
+            s.bound = max(s.bound, (Key)s.kept[p.top - 1]);
+            s.count = s.held;
+          }
+          __syncthreads();
+        }
+        if (s.count > kPrune) prune(s, p.top);
+        else {
+          if (tid == 0) s.held = s.count;
+          __syncthreads();
+        }
       }
     }
-    __syncthreads();
+    // the logits at the row's ends, by the last CTA's first threads: fewer than two vectors
+    if (part == parts - 1) {
+      const int tail = p.vocab - head - vecs * N;
+      if (tid < head + tail) {
+        const int i = tid < head ? tid : head + vecs * N + (tid - head);
+        const float v = to_f(x[i]);
+        raise(v);
+        if (st.m > -INFINITY) add(v);
+        if (TOP) enlist(v, i);
+      }
+    }
+    // the CTA's sums
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Stat t{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.z, o),
+                   __shfl_xor_sync(0xffffffffu, st.w, o)};
+      st.merge(t);
+    }
+    if (lane == 0) s.stat[warp] = st;
+    nan = __syncthreads_or(nan);
+    if (TOP) prune(s, p.top);
+    if (warp == 0) {
+      st = lane < kWarps ? s.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) {
+        const Stat t{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.z, o),
+                     __shfl_xor_sync(0xffffffffu, st.w, o)};
+        st.merge(t);
+      }
+      st = Stat{__shfl_sync(0xffffffffu, st.m, 0), __shfl_sync(0xffffffffu, st.z, 0),
+                __shfl_sync(0xffffffffu, st.w, 0)};
+    }
+    if (parts > 1) {
+      if (tid == 0) {
+        mine.stat = st;
+        mine.nan = nan;
+        mine.kept = TOP ? s.count : 0;
+      }
+      if (TOP && tid < s.count) mine.keys[tid] = s.list[tid];
+      cluster.sync();
+      if (part == 0) {
+        if (warp == 0) {
+          Stat all = st;
+          for (int k = 1; k < parts; ++k) {  // in order
+            const Result* o = cluster.map_shared_rank(&mine, k);
+            all.merge(o->stat);
+            nan |= o->nan != 0;
+          }
+          st = all;
+        }
+        if (TOP) {
+          int at = s.count;
+          for (int k = 1; k < parts; ++k) {
+            const Result* o = cluster.map_shared_rank(&mine, k);
+            const int n = o->kept;
+            if (tid < n) s.list[at + tid] = o->keys[tid];
+            at += n;
+          }
+          __syncthreads();
+          if (tid == 0) s.count = at;
+          __syncthreads();
+          prune(s, p.top);
+        }
+      }
+      cluster.sync();  // the others' results have been read
+    }
+    if (part == 0 && warp == 0) {
+      const float log_z = logf(st.z);
+      float lse = st.m + log_z, ent = log_z - st.w / st.z;
+      if (st.m == -INFINITY) lse = ent = 0.f;  // nothing but -inf
+      if (nan || st.m == INFINITY) {
+        lse = nan ? NAN : INFINITY;
+        ent = NAN;
+      }
+      if (lane == 0) {
+        const int t = p.tokens[r];
+        p.logprob[r] = t < 0 ? 0.f : t < p.vocab ? to_f(x[t]) - lse : NAN;
+        p.entropy[r] = ent;
+        if (t >= p.vocab && p.status) atomicExch(p.status, 4);
+      }
+      if (TOP && lane < p.top) {
+        const int i = 0x7fffffff - (int)(uint32_t)s.list[lane];
+        p.top_ids[r * p.top + lane] = i;
+        p.top_logprobs[r * p.top + lane] = to_f(x[i]) - lse;
+      }
+    }
+    if (TOP) __syncthreads();  // the list has been read
   }
+}
+
+template <typename T>
+int launch(const ScoreParams& p, cudaStream_t stream) {
+  const int sms = device_sm_count(current_device());
+  if (sms < 1) {
+    set_error("pp_token_logprobs: no current CUDA device");
+    return PP_ERR_CUDA;
+  }
+  // few rows: as many CTAs to each (a power of two) as keep them all on SMs of
+  // their own, and a batch of vectors to every CTA at least
+  int parts = 1;
+  while (parts < kMaxCluster && p.rows * parts * 2 <= sms &&
+         (int64_t)p.vocab * (int)sizeof(T) >= (int64_t)parts * 2 * kThreads * 16)
+    parts *= 2;
+  cudaLaunchConfig_t cfg{};
+  const int64_t rows = p.rows < (1 << 24) ? p.rows : (1 << 24);
+  cfg.gridDim = dim3((unsigned)(rows * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = launch_overlap() ? 2 : 1;
+  const cudaError_t e = p.top ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, p)
+                              : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("token_logprobs_kernel: %s", cudaGetErrorString(e));
+    return PP_ERR_CUDA;
+  }
+  return check_launch("token_logprobs_kernel");
 }
 
 }  // namespace
@@ -144,10 +437,8 @@ extern "C" int pp_token_logprobs(const void* logits, int dtype, int64_t ldx, int
                   PP_LOGPROBS_MAX_TOP);
     return PP_ERR_INVALID;
   }
-  pp::ScoreParams p{logits, ldx, rows, (int)vocab, tokens, (int)top, logprob, entropy, top_ids, top_logprobs, status};
-  const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : (1 << 20));
-  auto kern = dtype == PP_F16 ? pp::token_logprobs_kernel<__half>
-              : dtype == PP_BF16 ? pp::token_logprobs_kernel<__nv_bfloat16> : pp::token_logprobs_kernel<float>;
-  return pp::launch_kernel("token_logprobs_kernel", pp::launch_overlap(), kern, dim3(grid), dim3(pp::kThreads), 0,
-                           reinterpret_cast<cudaStream_t>(stream), p);
+  const pp::ScoreParams p{logits, ldx, rows, (int)vocab, tokens, (int)top, logprob, entropy, top_ids, top_logprobs, status};
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == PP_F16 ? pp::launch<__half>(p, s) : dtype == PP_BF16 ? pp::launch<__nv_bfloat16>(p, s)
+                                                                       : pp::launch<float>(p, s);
 }
