@@ -8,14 +8,15 @@
 // logit, 16 a clock and SM, which at the measured memory rate are three
 // quarters of the time for 2-byte logits.  One pass: a thread keeps its own
 // (maximum, Z, W = sum e^(x - m) (x - m)), moved to a new maximum when a vector
-// of logits exceeds it.  The alternatives come from the same pass: logits are
-// whole numbers (value, then lower index), all different, and those at or
-// above the row's bound go to a list in shared memory.  At least `top` logits
-// are always at or above the bound: at first it is the top-th largest of the
-// best of 64 groups of threads, later the top-th of the list, so that after
-// the first batch hardly any logit is listed.  Few rows are spread over
-// clusters of up to eight CTAs, whose results meet in the first one's shared
-// memory.
+// of logits exceeds it, and the place of its largest logit.  For the
+// alternatives logits are whole numbers (value, then lower index), all
+// different; the top-th largest of the best of 64 groups of threads is a bound
+// that at least `top` logits reach, and only the logits of threads whose best
+// reaches it, a few of the 512, are gone through again (by all threads) for a
+// list in shared memory, of which the `top` largest are ranked.  A row that lists
+// more than there is room for goes through its logits batch by batch, with a
+// bound that follows the list.  Few rows are spread over clusters of up to
+// eight CTAs, whose results meet in the first one's shared memory.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -37,7 +38,6 @@ constexpr int kBatch = 4;        // vectors of a thread in flight
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;      // of threads, whose best logits give the first bound
 constexpr int kList = 2048;      // keys that the list holds
-constexpr int kPrune = 128;      // a longer list is cut to the `top` largest
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct ScoreParams {
@@ -95,14 +95,43 @@ struct Stat {
   }
 };
 
+// Pairs of FP32 values, two operations an instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+
+// A thread's sums over pairs of logits, beside the maximum m.
+struct PairSums {
+  uint64_t z = 0, w = 0;
+  __device__ __forceinline__ void add(float a, float b, uint64_t minus_m, uint64_t log2e) {
+    uint64_t d, y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair(a, b)), "l"(minus_m));
+    float d0, d1, e0, e1;
+    split(d, d0, d1);
+    d = pair(fmaxf(d0, -200.f), fmaxf(d1, -200.f));  // -inf counts nothing
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(d), "l"(log2e));
+    split(y, e0, e1);
+    const uint64_t e = pair(ex2a(e0), ex2a(e1));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(z) : "l"(e));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(w) : "l"(e), "l"(d));
+  }
+};
+
 struct Shared {
   Key list[kList];
   Key kept[32];
   Key best[kGroups];
+  uint16_t who[kThreads];  // threads whose best logit reaches the bound
+  int interested;
   Stat stat[kWarps];
   Key bound;  // keys below it are not among the row's top
   int count;       // listed keys
-  int held;        // of them from earlier batches
+  int held;        // of them from earlier batches of a second passage
 };
 
 // A CTA's part of a row, read by the first CTA of the cluster.
@@ -127,7 +156,7 @@ __device__ void rank_list(Shared& s, int n, int top) {
 
 // The list becomes its `top` largest, in order.
 __device__ void prune(Shared& s, int top) {
-  const int n = s.count;
+  const int n = min(s.count, kList);
   rank_list(s, n, top);
   const int left = min(n, top);
   if ((int)threadIdx.x < left) s.list[threadIdx.x] = s.kept[threadIdx.x];
@@ -173,7 +202,7 @@ struct Vec {
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const ScoreParams p) {
+__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const ScoreParams p) {
   __shared__ Shared s;
   __shared__ Result mine;
   constexpr int N = Vec<T>::kN;
@@ -192,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const ScorePar
     if (TOP) {
       if (tid == 0) {
         s.bound = 0;
-        s.count = s.held = 0;
+        s.count = s.held = s.interested = 0;
       }
       __syncthreads();
     }
@@ -214,85 +243,122 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const ScorePar
         if (at < kList) s.list[at] = k;
       }
     };
+    const uint64_t log2e = pair(kLog2e, kLog2e);
+    // this thread's logits of a batch whose vectors may hold listed ones
+    auto scan = [&](int b0, auto&& use) {
+#pragma unroll 1
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = b0 + k * kThreads + tid;
+        if (i >= v1) break;
+        const Vec<T> v{xv[i]};
+        if (order(v.top()) < (uint32_t)(s.bound >> 32)) continue;
+#pragma unroll 1
+        for (int e = 0; e < N; ++e) use(v.get(e), head + i * N + e);
+      }
+    };
+    // the bound to the top-th largest of the groups' best keys, if that is higher
+    auto bound_from = [&](Key best) {
+#pragma unroll
+      for (int o = 1; o < kThreads / kGroups; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (tid % (kThreads / kGroups) == 0) s.best[tid / (kThreads / kGroups)] = best;
+      __syncthreads();
+      if (tid < kGroups) {
+        const Key me = s.best[tid];
+        int above = 0, equal = 0;
+#pragma unroll 8
+        for (int j = 0; j < kGroups; ++j) {
+          above += s.best[j] > me;
+          equal += s.best[j] == me;
+        }
+        if (above < p.top && above + equal >= p.top && me > s.bound) s.bound = me;  // all who write write the same
+      }
+      __syncthreads();
+    };
+    float best = -INFINITY;  // this thread's largest logit (a NaN counts as that), and its vector
+    int best_at = -1;
+#pragma unroll 1
     for (int b0 = v0; b0 < v1; b0 += kThreads * kBatch) {
       Vec<T> q[kBatch];
-      float top[kBatch];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int i = b0 + k * kThreads + tid;
         if (i < v1) q[k].v = ldg_stream(xv + i);
       }
-      uint32_t best = 0;  // order of this thread's best logit of the batch
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int i = b0 + k * kThreads + tid;
         if (i < v1) {
-          top[k] = q[k].top();
-          raise(top[k]);
+          const float top = q[k].top();
+          raise(top);
           if (st.m > -INFINITY) {
+            PairSums sums;
+            const uint64_t minus_m = pair(-st.m, -st.m);
 #pragma unroll
-            for (int e = 0; e < N; ++e) add(q[k].get(e));
+            for (int e = 0; e < N; e += 2) sums.add(q[k].get(e), q[k].get(e + 1), minus_m, log2e);
+            float a, c;
+            split(sums.z, a, c);
+            st.z += a + c;
+            split(sums.w, a, c);
+            st.w += a + c;
           }
-          if (TOP) best = max(best, order(top[k]));
+          if (TOP && (best_at < 0 || !(top <= best)) && best == best) {
+            best = top;
+            best_at = i;
+          }
         }
       }
-      if constexpr (TOP) {
-        // equal logits of later batches have higher indices: only larger ones count
-        const bool has = best > (uint32_t)(s.bound >> 32);
-        const int with = __syncthreads_count(has);
-        if (with == 0) continue;
-        if (with > kGroups) {
-          // the bound, at least the top-th largest of the groups' best keys
-          Key k64 = 0;
-          if (has) {
+    }
+    if constexpr (TOP) {
+      // the bound from the last logits of the best vectors: none is above its vector's best
+      bound_from(best_at < 0 ? 0 : rank_key(best, head + best_at * N + N - 1));
+      if (best_at >= 0 && rank_key(best, head + best_at * N) >= s.bound) s.who[atomicAdd(&s.interested, 1)] = tid;
+      __syncthreads();
+      const int per = (v1 - v0 + kThreads - 1) / kThreads, items = s.interested * per;
+#pragma unroll 1
+      for (int it0 = tid; it0 < items; it0 += kThreads * kBatch) {
+        Vec<T> q[kBatch];
+        int at[kBatch];
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int i = b0 + k * kThreads + tid;
-              if (i < v1 && order(top[k]) == best) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) k64 = max(k64, (Key)rank_key(q[k].get(e), head + i * N + e));
-              }
-            }
-          }
-#pragma unroll
-          for (int o = 1; o < kThreads / kGroups; o <<= 1)
-            k64 = max(k64, (Key)__shfl_xor_sync(0xffffffffu, k64, o));
-          if (tid % (kThreads / kGroups) == 0) s.best[tid / (kThreads / kGroups)] = k64;
-          __syncthreads();
-          if (tid < kGroups) {
-            const Key me = s.best[tid];
-            int rank = 0;
-#pragma unroll 8
-            for (int j = 0; j < kGroups; ++j) rank += s.best[j] > me;
-            if (rank == p.top - 1 && me > s.bound) s.bound = me;  // keys differ (empty groups: 0, never above)
-          }
-          __syncthreads();
+        for (int k = 0; k < kBatch; ++k) {
+          const int it = it0 + k * kThreads;
+          at[k] = it < items ? v0 + it % per * kThreads + s.who[it / per] : v1;
+          if (at[k] < v1) q[k].v = xv[at[k]];
         }
-        for (;;) {
-          if (has) {
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-              const int i = b0 + k * kThreads + tid;
-              if (i < v1 && order(top[k]) >= (uint32_t)(s.bound >> 32)) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) enlist(q[k].get(e), head + i * N + e);
-              }
+        for (int k = 0; k < kBatch; ++k)
+          if (at[k] < v1 && order(q[k].top()) >= (uint32_t)(s.bound >> 32)) {
+#pragma unroll 1
+            for (int e = 0; e < N; ++e) enlist(q[k].get(e), head + at[k] * N + e);
+          }
+      }
+    }
+    if constexpr (TOP) {
+      __syncthreads();
+      const bool over = s.count > kList - 2 * N;  // the row's ends, not listed yet, need room too
+      __syncthreads();  // everyone has read the count before it changes
+      if (over) {
+        // A second passage, batch by batch: the list holds the best so far, its
+        // last the bound.  Equal logits of later batches rank below it.
+        if (tid == 0) s.count = s.held = 0;
+        __syncthreads();
+        for (int b0 = v0; b0 < v1; b0 += kThreads * kBatch) {
+          Key best = 0;
+          scan(b0, [&](float v, int i) { best = max(best, rank_key(v, i)); });
+          if (__syncthreads_count(best >= s.bound) == 0) continue;
+          bound_from(best);
+          for (;;) {
+            if (best >= s.bound) scan(b0, enlist);
+            __syncthreads();
+            if (s.count <= kList) break;
+            // too many: the top-th of those listed is a higher bound; list again
+            rank_list(s, kList, p.top);
+            if (tid == 0) {
+              s.bound = max(s.bound, s.kept[p.top - 1]);
+              s.count = s.held;
             }
+            __syncthreads();
           }
-          __syncthreads();
-          if (s.count <= kList) break;
-          // too many: the top-th of those listed is a higher bound; list again
-          rank_list(s, kList, p.top);
-          if (tid == 0) {
-            s.bound = max(s.bound, (Key)s.kept[p.top - 1]);
-            s.count = s.held;
-          }
-          __syncthreads();
-        }
-        if (s.count > kPrune) prune(s, p.top);
-        else {
-          if (tid == 0) s.held = s.count;
-          __syncthreads();
+          prune(s, p.top);
         }
       }
     }
@@ -376,7 +442,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const ScorePar
         p.entropy[r] = ent;
         if (t >= p.vocab && p.status) atomicExch(p.status, 4);
       }
-      if (TOP && lane < p.top) {
+      if (TOP && lane < min(p.top, s.count)) {  // as many as `top` are always listed, unless the logits change meanwhile
         const int i = 0x7fffffff - (int)(uint32_t)s.list[lane];
         p.top_ids[r * p.top + lane] = i;
         p.top_logprobs[r * p.top + lane] = to_f(x[i]) - lse;

@@ -34,19 +34,31 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     past the vocabulary gets NaN and sets ``status`` (device int32) to 4.
     Equal logits are ranked by the lower index, NaN before every number.
     """
-    dev = _lib.require_cuda(logits, tokens, status)
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    index = logits.get_device()
+    if index < 0 or tokens.get_device() != index or (status is not None and status.get_device() != index):
+        _lib.require_cuda(logits, tokens, status)
+    dtype = _DTYPES.get(logits.dtype)
+    if logits.dim() != 2 or dtype is None or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be FP16, BF16 or float32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
-    if tokens.dtype != torch.int32 or tokens.shape != (rows,) or not tokens.is_contiguous():
+    if tokens.dtype is not torch.int32 or tokens.shape != (rows,) or not tokens.is_contiguous():
         raise ValueError(f"tokens must be contiguous int32 [{rows}]")
+    if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0..{MAX_TOP} and at most the vocabulary")
-    score = torch.empty(2, rows, dtype=torch.float32, device=dev)
-    ids = torch.empty(rows, top, dtype=torch.int32, device=dev)
-    lps = torch.empty(rows, top, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("pp_token_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), rows, vocab,
-                  tokens.data_ptr(), top, score[0].data_ptr(), score[1].data_ptr(), ids.data_ptr(), lps.data_ptr(),
-                  _lib.ptr(status), _lib.stream_handle(dev))
-    return TokenLogprobs(score[0], score[1], ids, lps)
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    ids = tokens.new_empty((rows, top))
+    lps = torch.empty_like(ids, dtype=torch.float32)
+    fn = _lib.load().pp_token_logprobs
+    args = (logits.data_ptr(), dtype, logits.stride(0), rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(),
+            entropy.data_ptr(), ids.data_ptr(), lps.data_ptr(), _lib.ptr(status), _lib.stream_handle(logits.device))
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    else:
+        rc = fn(*args)
+    if rc:
+        _lib.check(rc)
+    return TokenLogprobs(logprob, entropy, ids, lps)

@@ -71,6 +71,15 @@ def test_orders(cuda, shape):
         _check(rows, torch.tensor([30_000, 0, V - 1], dtype=torch.int32, device=cuda), 32)
 
 
+@pytest.mark.parametrize("top", [1, 20])
+def test_many_rows_of_ties(cuda, top):
+    """Rows that list more logits than there is room for, on every SM at once."""
+    V = 20_003
+    i = torch.arange(V, device=cuda, dtype=torch.float32)
+    x = torch.stack([i * 0 - 1.5, (i / V * 8), i % 3, (i > 2500).float() * 4]).repeat(250, 1).half()
+    _check(x, torch.full((1000,), 5, dtype=torch.int32, device=cuda), top)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_masked_rows(cuda, dtype):
     """-inf entries and rows of nothing else, the type's lowest value, NaN, +inf, -0."""
