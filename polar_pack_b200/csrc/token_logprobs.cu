@@ -202,7 +202,7 @@ struct Vec {
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const ScoreParams p) {
+__global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(const ScoreParams p) {
   __shared__ Shared s;
   __shared__ Result mine;
   constexpr int N = Vec<T>::kN;
@@ -403,25 +403,23 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Score
       if (TOP && tid < s.count) mine.keys[tid] = s.list[tid];
       cluster.sync();
       if (part == 0) {
-        if (warp == 0) {
-          Stat all = st;
-          for (int k = 1; k < parts; ++k) {  // in order
-            const Result* o = cluster.map_shared_rank(&mine, k);
-            all.merge(o->stat);
-            nan |= o->nan != 0;
-          }
-          st = all;
+        if (warp == 0) {  // a lane reads one part's sums; merged in order
+          const Result* o = cluster.map_shared_rank(&mine, lane < parts ? lane : 0);
+          const Stat part_st = o->stat;
+          nan = __any_sync(0xffffffffu, o->nan != 0);
+          st = Stat{-INFINITY, 0.f, 0.f};
+          for (int k = 0; k < parts; ++k)
+            st.merge(Stat{__shfl_sync(0xffffffffu, part_st.m, k), __shfl_sync(0xffffffffu, part_st.z, k),
+                          __shfl_sync(0xffffffffu, part_st.w, k)});
         }
         if (TOP) {
-          int at = s.count;
-          for (int k = 1; k < parts; ++k) {
-            const Result* o = cluster.map_shared_rank(&mine, k);
-            const int n = o->kept;
-            if (tid < n) s.list[at + tid] = o->keys[tid];
-            at += n;
+          // 32 places for each part's keys; empty ones rank last
+          if (tid < parts * 32) {
+            const Result* o = cluster.map_shared_rank(&mine, tid / 32);
+            s.list[tid] = tid % 32 < o->kept ? o->keys[tid % 32] : 0;
           }
           __syncthreads();
-          if (tid == 0) s.count = at;
+          if (tid == 0) s.count = parts * 32;
           __syncthreads();
           prune(s, p.top);
         }
