@@ -21,6 +21,12 @@ namespace pp {
 
 constexpr int kKvBlock = 64;
 
+// a[w] of a kernel parameter, without a copy of the array in local memory.
+template <typename T>
+__device__ __forceinline__ T pick(const T (&a)[2], int w) {
+  return w ? a[1] : a[0];
+}
+
 struct Kv8Cache {
   uint8_t* codes[2];  // keys, values
   float* scales[2];
@@ -29,13 +35,13 @@ struct Kv8Cache {
 
   __device__ __forceinline__ int64_t head(int b, int h) const { return (int64_t)b * nkv + h; }
   __device__ __forceinline__ uint8_t* code_row(int w, int b, int h, int t) const {
-    return codes[w] + (head(b, h) * cap + t) * hd;
+    return pick(codes, w) + (head(b, h) * cap + t) * hd;
   }
   __device__ __forceinline__ float* scale(int w, int b, int h, int block) const {
-    return scales[w] + head(b, h) * (cap / kKvBlock) + block;
+    return pick(scales, w) + head(b, h) * (cap / kKvBlock) + block;
   }
   __device__ __forceinline__ __half* tail_row(int w, int b, int h, int slot) const {
-    return tail[w] + (head(b, h) * kKvBlock + slot) * hd;
+    return pick(tail, w) + (head(b, h) * kKvBlock + slot) * hd;
   }
 };
 
@@ -72,12 +78,22 @@ __device__ __forceinline__ uint4 kv8_load8(const __half* row, int d0, int hd, co
 // largest finite FP16 number.
 __device__ __forceinline__ float kv8_finite(float x) { return x != x ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f); }
 
+__device__ __forceinline__ uint32_t kv8_word(uint4 x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+// Largest magnitude of eight values; not finite if one is not.
 __device__ __forceinline__ float kv8_amax8(uint4 x) {
+  __half2 m = __hmax2_nan(__hmax2_nan(__habs2(u2h(x.x)), __habs2(u2h(x.y))),
+                          __hmax2_nan(__habs2(u2h(x.z)), __habs2(u2h(x.w))));
+  const float2 f = __half22float2(m);
+  return f.x <= 65504.f && f.y <= 65504.f ? fmaxf(f.x, f.y) : INFINITY;
+}
+
+// The same of the values that quantisation sees.
+__device__ __forceinline__ float kv8_amax8_finite(uint4 x) {
   float m = 0.f;
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(u2h(w[i]));
+    const float2 f = __half22float2(u2h(kv8_word(x, i)));
     m = fmaxf(m, fmaxf(fabsf(kv8_finite(f.x)), fabsf(kv8_finite(f.y))));
   }
   return m;
@@ -86,30 +102,91 @@ __device__ __forceinline__ float kv8_amax8(uint4 x) {
 // Correctly rounded divisions, so that the codes follow from the definition.
 __device__ __forceinline__ float kv8_scale(float amax) { return __fdiv_rn(amax, 127.f); }
 
-__device__ __forceinline__ uint32_t kv8_code(float x, float scale) {
-  return scale > 0.f ? (uint32_t)(128 + (int)rintf(__fdiv_rn(kv8_finite(x), scale))) : 128u;
+// round(x / scale) + 128 in the low byte of the result: adding 1.5 * 2^23 + 128
+// rounds to a whole number, ties to even.  x * (1 / scale) is within 2^-22 of
+// the quotient (both below 128), so only within 1e-4 of a tie can it round
+// otherwise: those few are divided.
+__device__ __forceinline__ uint32_t kv8_code(float x, float scale, float per_scale) {
+  constexpr float kWhole = 12583040.f;
+  float q = x * per_scale;
+  const float y = q + kWhole, off = q - (y - kWhole);
+  if (fabsf(off) > 0.4999f) return __float_as_uint(__fdiv_rn(x, scale) + kWhole);
+  return __float_as_uint(y);
 }
 
-__device__ __forceinline__ uint2 kv8_codes8(uint4 x, float scale) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t o[2] = {0, 0};
+// Codes of eight values.  finite: all of the block's values are.
+__device__ __forceinline__ uint2 kv8_codes8(uint4 x, float scale, float per_scale, bool finite) {
+  uint32_t o[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(u2h(w[i]));
-    o[i >> 1] |= (kv8_code(f.x, scale) | kv8_code(f.y, scale) << 8) << (16 * (i & 1));
+  for (int h = 0; h < 2; ++h) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 f = __half22float2(u2h(kv8_word(x, 2 * h + i)));
+      if (!finite) f = make_float2(kv8_finite(f.x), kv8_finite(f.y));
+      c[2 * i] = kv8_code(f.x, scale, per_scale);
+      c[2 * i + 1] = kv8_code(f.y, scale, per_scale);
+    }
+    o[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
   }
   return make_uint2(o[0], o[1]);
 }
 
-// fp16((code - 128) * scale) of eight codes.
+// fp16((code - 128) * scale) of eight codes: a byte in the low end of 2^23 is
+// 2^23 + code, exactly.
 __device__ __forceinline__ uint4 kv8_values8(uint2 c, float scale) {
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t w = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
-    r[i] = h2u(__floats2half2_rn(((int)(w & 255u) - 128) * scale, ((int)((w >> 8) & 255u) - 128) * scale));
+    const uint32_t w = i < 2 ? c.x : c.y;
+    const float a = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7442 : 0x7440)) - 8388736.f;
+    const float b = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7443 : 0x7441)) - 8388736.f;
+    r[i] = h2u(__floats2half2_rn(a * scale, b * scale));
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// A block's scale (0 where all values are: their quotient is then 0 too).  The
+// smallest FP16 number / 127 still has a finite reciprocal.
+struct Kv8Scale {
+  float scale, per_scale;
+  bool finite;  // all of the block's values are
+};
+
+__device__ __forceinline__ Kv8Scale kv8_make_scale(float amax, bool finite) {
+  const float s = kv8_scale(amax);
+  return Kv8Scale{s, s > 0.f ? __fdiv_rn(1.f, s) : 0.f, finite};
+}
+
+__device__ __forceinline__ uint2 kv8_codes8(uint4 x, const Kv8Scale& q) {
+  return kv8_codes8(x, q.scale, q.per_scale, q.finite);
+}
+
+// Largest magnitudes over the CTA's threads and values v; where one is not
+// finite they are counted again as quantisation sees them.  Every thread gets
+// the result; red has a place for each warp.
+template <int N, int THREADS>
+__device__ __forceinline__ Kv8Scale kv8_block_scale(const uint4 (&v)[N], float* red) {
+  auto all = [&](float m) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, red[i]);
+    return m;
+  };
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, kv8_amax8(v[i]));
+  m = all(m);
+  if (m <= 65504.f) return kv8_make_scale(m, true);
+  m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, kv8_amax8_finite(v[i]));
+  return kv8_make_scale(all(m), false);
 }
 
 // Eight stored values of position t of a sequence of `len` tokens, FP16.

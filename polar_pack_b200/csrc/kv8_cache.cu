@@ -49,18 +49,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Maximum over the CTA; every thread gets it.
-__device__ __forceinline__ float cta_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) v = fmaxf(v, red[i]);
-  return v;
-}
-
 struct AppendParams {
   Kv8Cache c;
   const __half* x[2];  // keys, values: row (b, i, head) at b * ldb + i * ldt + head * ldh
@@ -98,10 +86,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
   const int len = pos + cnt, last = kv8_last_block(len);
   const int block = pos / kKvBlock + blockIdx.x;
   if (block > last) return;
-  const __half* x = p.x[w] + b * p.ldb[w] + h * p.ldh[w];
-  auto row8 = [&](int t, int d0) { return kv8_load8(x + (int64_t)(t - pos) * p.ldt[w], d0, HD, rope, r0 + t - pos); };
+  const __half* x = pick(p.x, w) + b * pick(p.ldb, w) + h * pick(p.ldh, w);
+  const int64_t ldt = pick(p.ldt, w);
+  auto row8 = [&](int t, int d0) { return kv8_load8(x + (int64_t)(t - pos) * ldt, d0, HD, rope, r0 + t - pos); };
   uint4 v[kVecs];
-  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
@@ -111,18 +99,18 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
       v[i] = *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
     else if (t < len)
       v[i] = row8(t, d0);
-    m = fmaxf(m, kv8_amax8(v[i]));
   }
-  const float scale = kv8_scale(cta_max(m, red));  // the barrier also orders the tail's reads before its writes
   if ((block + 1) * kKvBlock <= len) {
+    const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[i], scale);
+      *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[i], q);
     }
-    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = scale;
+    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = q.scale;
   }
   if (blockIdx.x != 0) return;
+  __syncthreads();  // the tail's old rows have been read
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
@@ -141,23 +129,31 @@ struct RestoreParams {
   int* status;
 };
 
-// One thread restores eight dimensions of one position and head.
+// CTA (64 positions, head, sequence and side): a thread restores kVecs vectors
+// of eight dimensions, all read before the first is written.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) kv8_restore_kernel(const RestoreParams p) {
+  constexpr int kVecs = kKvBlock * HD / 8 / kThreads;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t per = (int64_t)p.count * p.c.nkv * (HD / 8);
-  const int64_t e = blockIdx.x * (int64_t)kThreads + threadIdx.x;
-  const int b = blockIdx.z >> 1, w = blockIdx.z & 1;
-  const int len = p.lens[b];
+  const int h = blockIdx.y, b = blockIdx.z >> 1, w = blockIdx.z & 1;
+  const int len = p.lens[b], first = p.start ? p.start[b] : 0;
   const bool ok = len <= p.c.cap;
-  if (!ok && e == 0 && p.status) atomicExch(p.status, 5);
-  if (e >= per) return;
-  const int d0 = (int)(e % (HD / 8)) * 8, h = (int)(e / (HD / 8) % p.c.nkv);
-  const int64_t t = e / (HD / 8) / p.c.nkv + (p.start ? p.start[b] : 0);
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (ok && t >= 0 && t < len) v = kv8_read8(p.c, w, b, h, (int)t, len, d0);
-  *reinterpret_cast<uint4*>(p.out[w] + b * per * 8 + e * 8) = v;
+  if (!ok && blockIdx.x == 0 && h == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, 5);
+  uint4 v[kVecs];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int e = k * kThreads + threadIdx.x, i = blockIdx.x * kKvBlock + e / (HD / 8);
+    const int64_t t = (int64_t)first + i;
+    v[k] = make_uint4(0, 0, 0, 0);
+    if (ok && i < p.count && t >= 0 && t < len) v[k] = kv8_read8(p.c, w, b, h, (int)t, len, e % (HD / 8) * 8);
+  }
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int e = k * kThreads + threadIdx.x, i = blockIdx.x * kKvBlock + e / (HD / 8);
+    if (i < p.count)
+      *reinterpret_cast<uint4*>(pick(p.out, w) + (((int64_t)b * p.count + i) * p.c.nkv + h) * HD + e % (HD / 8) * 8) = v[k];
+  }
 }
 
 // ------------------------------------------------------------- eviction --
@@ -180,16 +176,21 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelThreads = 1024;
+constexpr int kSelRounds = 32;            // of kSelThreads keys, whose kept ones are counted together
+constexpr int kSelCached = 48 * 1024;     // keys that fit shared memory
 
 // CTA (head, sequence) finds the keep-th largest key by four passes over the
-// keys' bytes (a histogram each), then writes the kept positions in order:
-// those above it, and as many equal to it, lowest first, as there is room.
-__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictParams p) {
+// keys' bytes (a histogram each, equal bytes of a warp counted at once), then
+// writes the kept positions in order: those above it, and as many equal to it,
+// lowest first, as there is room.  The keys stay in shared memory where they
+// fit (`cached` keys).
+__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictParams p, int cached) {
   __shared__ int hist[256];
-  __shared__ int warp_gt[32], warp_eq[32];
+  __shared__ int above_of[kSelRounds * 32 + 1], equal_of[kSelRounds * 32 + 1];  // kept before a round's warp
   __shared__ int s_digit, s_left;
   pdl_launch_dependents();
   pdl_wait();
+  uint32_t* keys = reinterpret_cast<uint32_t*>(pp_smem);
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int len = p.lens[b];
   const bool ok = len <= p.c.cap;
@@ -200,62 +201,104 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictPara
   const float* wt = p.weights + p.c.head(b, h) * p.c.cap;
   float* to_wt = p.to_weights + p.to.head(b, h) * p.to.cap;
   int* kept = p.kept + p.c.head(b, h) * p.keep;
-  auto key = [&](int t) { return t < p.sinks || t >= len - p.recent ? 0xffffffffu : weight_key(wt[t]); };
+  auto make_key = [&](int t) { return t < p.sinks || t >= len - p.recent ? 0xffffffffu : weight_key(wt[t]); };
   for (int t = m + tid; t < p.keep; t += kSelThreads) kept[t] = -1;
   for (int t = m + tid; t < p.to.cap; t += kSelThreads) to_wt[t] = 0.f;
+  if (m == len) {
+    for (int t = tid; t < len; t += kSelThreads) {
+      kept[t] = t;
+      to_wt[t] = wt[t];
+    }
+    return;
+  }
+#pragma unroll 4
+  for (int t = tid; t < min(len, cached); t += kSelThreads) keys[t] = make_key(t);
+  auto key = [&](int t) { return t < cached ? keys[t] : make_key(t); };  // a thread reads its own
   uint32_t cut = 0;
   int left = m;  // kept positions among the keys that agree with `cut` so far
-  if (m < len) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int t = tid; t < len; t += kSelThreads) {
-        const uint32_t k = key(t);
-        if (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+#pragma unroll 2
+    for (int t0 = 0; t0 < len; t0 += kSelThreads) {
+      const int t = t0 + tid;
+      const uint32_t k = t < len ? key(t) : 0;
+      const bool in = t < len && (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8)));
+      const uint32_t d = in ? (k >> shift) & 255 : 256;
+      if (__any_sync(0xffffffffu, in)) {
+        const uint32_t same = __match_any_sync(0xffffffffu, d);
+        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
       }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255, above = 0;
-        while (d > 0 && above + hist[d] < left) above += hist[d--];
-        s_digit = d;
-        s_left = left - above;
-      }
-      __syncthreads();
-      cut |= (uint32_t)s_digit << shift;
-      left = s_left;
-    }
-  }
-  int base_gt = 0, base_eq = 0;  // kept above / equal before this round
-  for (int t0 = 0; t0 < len; t0 += kSelThreads) {
-    const int t = t0 + tid;
-    const uint32_t k = t < len ? key(t) : 0;
-    const bool gt = t < len && (m == len || k > cut), eq = t < len && m < len && k == cut;
-    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      warp_gt[warp] = __popc(bg);
-      warp_eq[warp] = __popc(be);
     }
     __syncthreads();
-    int g = base_gt, q = base_eq;
-    int tg = 0, te = 0;
-    for (int i = 0; i < 32; ++i) {
-      if (i == warp) {
-        g += tg;
-        q += te;
+    if (warp == 0) {
+      // the digit at which the count from the top reaches `left`: lane l has digits 255 - 8 l and down
+      int n[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += n[i] = hist[255 - 8 * lane - i];
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
       }
-      tg += warp_gt[i];
-      te += warp_eq[i];
+      int above = upto - sum;
+      if (above < left && upto >= left) {
+        int i = 0;
+        while (above + n[i] < left) above += n[i++];
+        s_digit = 255 - 8 * lane - i;
+        s_left = left - above;
+      }
     }
-    const uint32_t below = (1u << lane) - 1;
-    g += __popc(bg & below);
-    q += __popc(be & below);
-    if (gt || (eq && q < left)) {
-      const int at = g + min(q, left);
-      kept[at] = t;
-      to_wt[at] = wt[t];
+    __syncthreads();
+    cut |= (uint32_t)s_digit << shift;
+    left = s_left;
+  }
+  int base_gt = 0, base_eq = 0;  // kept above / equal before these rounds
+  for (int r0 = 0; r0 < len; r0 += kSelRounds * kSelThreads) {
+    const int rounds = min(kSelRounds, (len - r0 + kSelThreads - 1) / kSelThreads);
+    for (int i = 0; i < rounds; ++i) {
+      const int t = r0 + i * kSelThreads + tid;
+      const uint32_t k = t < len ? key(t) : 0;
+      const uint32_t bg = __ballot_sync(0xffffffffu, t < len && k > cut), be = __ballot_sync(0xffffffffu, t < len && k == cut);
+      if (lane == 0) {
+        above_of[i * 32 + warp] = __popc(bg);
+        equal_of[i * 32 + warp] = __popc(be);
+      }
     }
-    base_gt += tg;
-    base_eq += te;
+    __syncthreads();
+    if (warp < 2) {  // exclusive sums over the rounds' warps
+      int* a = warp == 0 ? above_of : equal_of;
+      int sum = 0;
+      for (int i = 0; i < rounds; ++i) {
+        const int n = a[i * 32 + lane];
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        a[i * 32 + lane] = sum + x - n;
+        sum += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) a[kSelRounds * 32] = sum;
+    }
+    __syncthreads();
+    for (int i = 0; i < rounds; ++i) {
+      const int t = r0 + i * kSelThreads + tid;
+      const uint32_t k = t < len ? key(t) : 0;
+      const bool gt = t < len && k > cut, eq = t < len && k == cut;
+      const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1;
+      const int g = base_gt + above_of[i * 32 + warp] + __popc(bg & below);
+      const int q = base_eq + equal_of[i * 32 + warp] + __popc(be & below);
+      if (gt || (eq && q < left)) {
+        const int at = g + min(q, left);
+        kept[at] = t;
+        to_wt[at] = wt[t];
+      }
+    }
+    base_gt += above_of[kSelRounds * 32];
+    base_eq += equal_of[kSelRounds * 32];
     __syncthreads();
   }
 }
@@ -282,26 +325,31 @@ __global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const EvictParams 
   const bool whole = full && f % kKvBlock == 0 && src[kKvBlock - 1] - f == kKvBlock - 1 &&
                      f / kKvBlock != kv8_last_block(len);
   uint4 v[kVecs];
-  float mx = 0.f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
     v[i] = src[r] >= 0 ? kv8_read8(p.c, w, b, h, src[r], len, d0) : make_uint4(0, 0, 0, 0);
-    mx = fmaxf(mx, kv8_amax8(v[i]));
   }
-  const float scale = kv8_scale(cta_max(mx, red));
+  if (last) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
+      if (src[r] >= 0) *reinterpret_cast<uint4*>(p.to.tail_row(w, b, h, r) + d0) = v[i];
+    }
+  }
+  if (!full) return;
+  const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    if (full) {
-      const uint2 c = whole ? *reinterpret_cast<const uint2*>(p.c.code_row(w, b, h, f + r) + d0)
-                            : kv8_codes8(v[i], scale);
-      *reinterpret_cast<uint2*>(p.to.code_row(w, b, h, block * kKvBlock + r) + d0) = c;
-    }
-    if (last && src[r] >= 0) *reinterpret_cast<uint4*>(p.to.tail_row(w, b, h, r) + d0) = v[i];
+    const uint2 c = whole ? *reinterpret_cast<const uint2*>(p.c.code_row(w, b, h, f + r) + d0) : kv8_codes8(v[i], q);
+    *reinterpret_cast<uint2*>(p.to.code_row(w, b, h, block * kKvBlock + r) + d0) = c;
   }
-  if (full && threadIdx.x == 0) *p.to.scale(w, b, h, block) = whole ? *p.c.scale(w, b, h, f / kKvBlock) : scale;
+  if (threadIdx.x == 0) *p.to.scale(w, b, h, block) = whole ? *p.c.scale(w, b, h, f / kKvBlock) : q.scale;
 }
+
+bool g_select_attr[64];
+int g_select_limit[64];
 
 }  // namespace
 }  // namespace pp
@@ -356,14 +404,10 @@ int pp_kv8_restore(const pp_kv8_cache* cache, const int* lens, const int* start,
   p.out[0] = reinterpret_cast<__half*>(k);
   p.out[1] = reinterpret_cast<__half*>(v);
   p.status = status;
-  const int64_t blocks = pp::cdiv(count * p.c.nkv * (p.c.hd / 8), pp::kThreads);
-  if (blocks > INT32_MAX) {
-    pp::set_error("pp_kv8_restore: too many positions in one call");
-    return PP_ERR_INVALID;
-  }
   return pp::launch_kernel("kv8_restore_kernel", pp::launch_overlap(),
                            p.c.hd == 128 ? pp::kv8_restore_kernel<128> : pp::kv8_restore_kernel<64>,
-                           dim3((unsigned)blocks, 1, (unsigned)p.c.batch * 2), dim3(pp::kThreads), 0,
+                           dim3((unsigned)pp::cdiv(count, pp::kKvBlock), (unsigned)p.c.nkv, (unsigned)p.c.batch * 2),
+                           dim3(pp::kThreads), 0,
                            reinterpret_cast<cudaStream_t>(stream), p);
 }
 
@@ -400,8 +444,13 @@ int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int*
   p.recent = (int)recent;
   p.status = status;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int lim = 0;
+  if (int rc = pp::ensure_smem_attr(pp::kv8_select_kernel, pp::g_select_attr, pp::g_select_limit, &lim)) return rc;
+  int cached = p.c.cap < pp::kSelCached ? p.c.cap : pp::kSelCached;
+  if (cached * 4 > lim) cached = lim / 4;
   if (int rc = pp::launch_kernel("kv8_select_kernel", pp::launch_overlap(), pp::kv8_select_kernel,
-                                 dim3((unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kSelThreads), 0, s, p))
+                                 dim3((unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kSelThreads), (size_t)cached * 4,
+                                 s, p, cached))
     return rc;
   // started early whatever the overlap setting: it waits for the selection itself
   return pp::launch_kernel("kv8_gather_kernel", true,

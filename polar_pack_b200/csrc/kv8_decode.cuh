@@ -263,7 +263,7 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
   const int cta = gridDim.x - 1 - blockIdx.x;  // idle CTAs of short launches come first
   auto row8 = [&](int w, int b, int h, int d0) {
     Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
-    return kv8_load8(p.x[w] + b * p.ldxb[w] + h * p.ldxh[w], d0, HD, r, r.cos ? r.pos[b] : 0);
+    return kv8_load8(pick(p.x, w) + b * pick(p.ldxb, w) + h * pick(p.ldxh, w), d0, HD, r, r.cos ? r.pos[b] : 0);
   };
   for (int i = cta * WARPS + warp; i < items; i += gridDim.x * WARPS) {
     const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
@@ -275,30 +275,21 @@ __device__ __forceinline__ void kv8_store_token(const Kv8DecodeParams& p, const 
     const int w = i & 1, h = (i >> 1) % p.c.nkv, b = (i >> 1) / p.c.nkv, len = s_len[b];
     if (len <= 0 || len % kKvBlock) continue;  // the same for the whole CTA
     uint4 v[kVecs];
-    float m = 0.f;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
       v[k] = e >= kItems ? make_uint4(0, 0, 0, 0)
              : r == kKvBlock - 1 ? row8(w, b, h, d0)
                                  : *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
-      m = fmaxf(m, kv8_amax8(v[k]));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __syncthreads();
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    for (int k = 0; k < WARPS; ++k) m = fmaxf(m, red[k]);
-    const float scale = kv8_scale(m);
+    const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
     const int block = len / kKvBlock - 1;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int e = k * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      if (e < kItems)
-        *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[k], scale);
+      if (e < kItems) *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[k], q);
     }
-    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = scale;
+    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = q.scale;
   }
 }
 
@@ -350,7 +341,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     Kv8Rope r = w == 0 ? p.rope : Kv8Rope{};
     const int t = r.cos ? r.pos[b] : 0;
     if (r.cos && (t < 0 || t >= r.len)) return make_uint4(0, 0, 0, 0);
-    return kv8_load8(p.x[w] + b * p.ldxb[w] + kvh * p.ldxh[w], d0, HD, r, t);
+    return kv8_load8(pick(p.x, w) + b * pick(p.ldxb, w) + kvh * pick(p.ldxh, w), d0, HD, r, t);
   };
   constexpr int kRowItems = NT * 8 * (HD / 8), kNewItems = 2 * (HD / 8);
   static_assert(kRowItems <= kThreads && kNewItems <= kThreads, "one item per thread");
@@ -456,7 +447,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       const int r = (u - seg_coded) * kDecTailUnit;
       const uint32_t bytes = min(kDecTailUnit, max(0, seg_held - seg_coded * kKvBlock - r)) * HD * 2;
       mbar_expect_tx(bar, bytes);
-      if (bytes) bulk_load(dst, p.c.tail[w] + ((int64_t)seg_head * kKvBlock + r) * HD, bytes, bar);
+      if (bytes) bulk_load(dst, pick(p.c.tail, w) + ((int64_t)seg_head * kKvBlock + r) * HD, bytes, bar);
     }
   };
   auto enter = [&](int from) {  // starts the warp's first unit of the segment that begins at unit `from`
