@@ -19,7 +19,9 @@ Two ways to serve the Linears of a ``.quadpack`` from HBM without unpacking:
   KV-cache append fused in) and SwiGLU are this library's kernels
   (``decode_ops.cu``).  The step has fixed
   buffers and a device-side position, so it can be captured once as a CUDA
-  graph and replayed for every token.
+  graph and replayed for every token.  Its keys and values are FP16, or 8-bit
+  caches with an optional token budget (``kv8.py``); ``score`` and
+  ``logprobs`` read its logits (``scoring.py``).
 """
 from __future__ import annotations
 
@@ -31,7 +33,9 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .kv8 import BLOCK, KV8Cache, kv8_decode, kv8_evict
 from .quadpack import QuadLinearGroup, QuadTailedLinear, layer_offsets, quad_linear
+from .scoring import TokenLogprobs, token_logprobs
 
 
 # --------------------------------------------------------------- loader ----
@@ -255,10 +259,24 @@ class QuadDecoder:
     (:class:`GatheredLinear`); norms, attention and SwiGLU run on every rank
     over the gathered activations, so every rank holds the whole step's
     state and the logits.
+
+    ``kv_bits=8`` keeps keys and values in 8 bits (:class:`~.kv8.KV8Cache`, one
+    per layer) instead of FP16.  With ``kv_budget`` the caches hold at most
+    ``kv_budget + kv_slack`` tokens: a step that finds them full first evicts
+    down to ``kv_budget`` in every layer and kv head, keeping the first
+    ``kv_sinks`` tokens, the last ``kv_recent`` and those with the largest
+    accumulated attention weight (:func:`~.kv8.kv8_evict`).  Rotation
+    positions go on counting, up to ``cfg.max_pos``.
     """
 
     def __init__(self, pack, cfg: DecoderConfig, extras: DecoderExtras, attn_splits: int | None = None, world: int = 1,
-                 rank: int = 0):
+                 rank: int = 0, kv_bits: int = 16, kv_budget: int | None = None, kv_slack: int = 256,
+                 kv_recent: int = 64, kv_sinks: int = 4):
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 8 or 16")
+        if kv_budget is not None and (kv_bits != 8 or kv_budget < 1 or kv_slack < 1 or kv_recent < 0 or kv_sinks < 0
+                                      or kv_recent + kv_sinks > kv_budget):
+            raise ValueError("a kv_budget needs kv_bits=8, a positive slack and room for kv_sinks + kv_recent tokens")
         self.pack, self.cfg, self.ex = pack, cfg, extras
         dev = self.device = pack.device
         self.lib = _lib.load()
@@ -291,8 +309,24 @@ class QuadDecoder:
         # o Linears gain less than the extra stores cost
         self.xn_il = torch.zeros(4 * H, **f16)
         self.act_il = torch.zeros(4 * I, **f16)
-        self.kc = [torch.zeros(4, cfg.max_pos, cfg.kv_heads, cfg.head_dim, **f16) for _ in range(cfg.layers)]
-        self.vc = [torch.zeros(4, cfg.max_pos, cfg.kv_heads, cfg.head_dim, **f16) for _ in range(cfg.layers)]
+        self.kv_budget, self.kv_recent, self.kv_sinks = kv_budget, kv_recent, kv_sinks
+        self.kv8 = None
+        if kv_bits == 8:
+            room = cfg.max_pos if kv_budget is None else min(cfg.max_pos, kv_budget + kv_slack)
+            self.kv_room = room
+            new = lambda: KV8Cache.empty(4, cfg.kv_heads, room, cfg.head_dim, dev, status=self.status)
+            self.kv8 = [new() for _ in range(cfg.layers)]
+            # a spare layer that evictions gather into, and the attention weights they go by
+            self.kv8_spare = new() if kv_budget is not None else None
+            self.kv8_weights = [c.new_weights() if kv_budget is not None else None for c in self.kv8]
+            self.kv8_ws = self.kv8[0].new_workspace(1, cfg.q_heads, kv_budget is not None)
+            self.held = torch.zeros(4, dtype=torch.int32, device=dev)      # tokens in the caches
+            self.rot = torch.zeros(4, dtype=torch.int32, device=dev)       # rotation position (= pos)
+            self.n_held = 0
+            self.kc = self.vc = []
+        else:
+            self.kc = [torch.zeros(4, cfg.max_pos, cfg.kv_heads, cfg.head_dim, **f16) for _ in range(cfg.layers)]
+            self.vc = [torch.zeros(4, cfg.max_pos, cfg.kv_heads, cfg.head_dim, **f16) for _ in range(cfg.layers)]
         self.cos, self.sin = rope_tables(cfg, dev)
         # attention: position ranges per (model, kv head); by default one per
         # 256 positions of the cache (a CTA's eight 32-position warp tiles at
@@ -346,7 +380,8 @@ class QuadDecoder:
 
     def launches_per_step(self) -> int:
         n = lambda g: len(g.calls) if isinstance(g, GatheredLinear) else 1
-        return 2 + self.cfg.layers * 4 + sum(n(g) for grp in self.groups for c in grp for g in c) + \
+        attn = 0 if self.kv8 is None else (self.kv_budget is not None) + (self.peers is not None)
+        return 2 + self.cfg.layers * (4 + attn) + sum(n(g) for grp in self.groups for c in grp for g in c) + \
             sum(n(g) for g in self.head) + (1 if self.peers is not None else 0)   # + the logits wait
 
     def close(self) -> None:
@@ -377,12 +412,15 @@ class QuadDecoder:
             c(L.pp_rmsnorm_rows(self.h.data_ptr(), H, self._in_norm[l], H, cfg.rms_eps, self.xn.data_ptr(), H,
                                 None, *(self._wait(1) if l > 0 else none), s))
             run(g_qkv)
-            c(L.pp_decode_attention(self.qkv.data_ptr(), self.qkv.stride(0), cfg.q_heads, cfg.kv_heads,
-                                    cfg.head_dim, self.cos.data_ptr(), self.sin.data_ptr(), self._kc[l],
-                                    self._vc[l], cfg.max_pos, self.pos.data_ptr(), self.scale, self.attn.data_ptr(),
-                                    self.attn.stride(0), None, self.splits,
-                                    self.attn_ws.data_ptr(),
-                                    self.attn_ws.numel(), self.status.data_ptr(), *self._wait(0), s))
+            if self.kv8 is not None:
+                self._attend8(l, s)
+            else:
+                c(L.pp_decode_attention(self.qkv.data_ptr(), self.qkv.stride(0), cfg.q_heads, cfg.kv_heads,
+                                        cfg.head_dim, self.cos.data_ptr(), self.sin.data_ptr(), self._kc[l],
+                                        self._vc[l], cfg.max_pos, self.pos.data_ptr(), self.scale, self.attn.data_ptr(),
+                                        self.attn.stride(0), None, self.splits,
+                                        self.attn_ws.data_ptr(),
+                                        self.attn_ws.numel(), self.status.data_ptr(), *self._wait(0), s))
             run(g_o)
             c(L.pp_rmsnorm_rows(self.h.data_ptr(), H, self._post_norm[l], H, cfg.rms_eps, self.xn.data_ptr(), H,
                                 self.xn_il.data_ptr(), *self._wait(1), s))
@@ -396,13 +434,53 @@ class QuadDecoder:
         if self.peers is not None:
             self.peers.wait(3, s)
 
+    def _attend8(self, l: int, s) -> None:
+        """Attention of layer l over its 8-bit cache, on the current stream (handle s)."""
+        cfg = self.cfg
+        if self.peers is not None:
+            self.peers.wait(0, s)
+        rows = self.qkv.view(4, cfg.q_heads + 2 * cfg.kv_heads, cfg.head_dim)
+        q, k, v = rows.split((cfg.q_heads, cfg.kv_heads, cfg.kv_heads), dim=1)
+        kv8_decode(q, k, v, self.kv8[l], self.held, weights=self.kv8_weights[l], scale=self.scale,
+                   rope=(self.cos, self.sin, self.rot), out=self.attn.view(4, cfg.q_heads, cfg.head_dim),
+                   workspace=self.kv8_ws)
+
+    def evict(self) -> None:
+        """Evict every layer's cache down to ``kv_budget`` tokens now (``step``
+        does it when the caches are full)."""
+        if self.kv_budget is None:
+            raise ValueError("the decoder has no kv_budget")
+        if self.n_held <= self.kv_budget:
+            return
+        n = -(-self.kv_budget // BLOCK)     # blocks that hold kept tokens
+        spare, spare_w = self.kv8_spare, self.kv8_spare.new_weights()
+        for cache, w in zip(self.kv8, self.kv8_weights):
+            kv8_evict(cache, spare, self.held, w, self.kv_budget, sinks=self.kv_sinks, recent=self.kv_recent,
+                      into_weights=spare_w)
+            for name in ("k_codes", "v_codes"):
+                getattr(cache, name)[:, :, :n * BLOCK].copy_(getattr(spare, name)[:, :, :n * BLOCK])
+            for name in ("k_scales", "v_scales"):
+                getattr(cache, name)[:, :, :n].copy_(getattr(spare, name)[:, :, :n])
+            for name in ("k_tail", "v_tail"):
+                getattr(cache, name).copy_(getattr(spare, name))
+            w.copy_(spare_w)
+        self.held.fill_(self.kv_budget)
+        self.n_held = self.kv_budget
+
     def _advance(self) -> None:
         self.pos.add_(1)
+        if self.kv8 is not None:
+            self.held.add_(1)
+            self.rot.add_(1)
 
     def step(self, tokens=None) -> torch.Tensor:
         """One token per model; returns the logits buffer ``[4][vocab]``."""
         if tokens is not None:
             self.tokens.copy_(torch.as_tensor(tokens, dtype=torch.int32), non_blocking=True)
+        if self.kv8 is not None:
+            if self.kv_budget is not None and self.n_held == self.kv_room:
+                self.evict()
+            self.n_held += 1
         if self.graph is not None:
             self.graph.replay()
         else:
@@ -410,10 +488,36 @@ class QuadDecoder:
             self._advance()
         return self.logits
 
+    def logprobs(self, tokens, top: int = 0) -> TokenLogprobs:
+        """Log probability of one token per model under the last step's logits,
+        with entropy and the ``top`` likeliest tokens (:func:`~.scoring.token_logprobs`)."""
+        t = torch.as_tensor(tokens, dtype=torch.int32).to(self.device)
+        return token_logprobs(self.logits, t, top=top)
+
+    def score(self, tokens) -> torch.Tensor:
+        """Teacher-forced scores of ``tokens`` ``[4][n]`` from the decoder's
+        current state: the log probabilities ``[4][n - 1]`` of tokens 1.. after
+        those before them.  ``(-score.mean(1)).exp()`` are the four models'
+        perplexities, as the reference's perplexity tools measure them."""
+        t = torch.as_tensor(tokens, dtype=torch.int32).to(self.device)
+        if t.dim() != 2 or t.shape[0] != 4 or t.shape[1] < 1:
+            raise ValueError("tokens must be [4][n], n at least 1")
+        t = t.t().contiguous()
+        out = torch.empty(t.shape[0] - 1, 4, dtype=torch.float32, device=self.device)
+        for i in range(t.shape[0] - 1):
+            self.tokens.copy_(t[i])
+            self.step()
+            out[i].copy_(token_logprobs(self.logits, t[i + 1]).logprob)
+        return out.t()
+
     def capture(self, stream: torch.cuda.Stream) -> None:
         """Capture one step (kernels + position advance) as a CUDA graph; the
         decoder state (position, caches) is unchanged by the capture."""
+        if self.kv8 is not None and self.n_held == self.kv_room:
+            raise ValueError("the caches are full: take a step or evict before a capture")
         pos0 = self.pos.clone()
+        kept = [] if self.kv8 is None else [(x, x.clone()) for x in (self.held, self.rot, *self.kv8_weights)
+                                            if x is not None]
         with torch.cuda.stream(stream):
             self._run(stream.cuda_stream)       # warm-up outside the graph (argument caches)
             self._advance()
@@ -423,9 +527,18 @@ class QuadDecoder:
             self._run(stream.cuda_stream)
             self._advance()
         self.pos.copy_(pos0)
+        for x, x0 in kept:
+            x.copy_(x0)
         torch.cuda.synchronize(self.device)
         self.graph = g
 
     def reset(self) -> None:
         self.pos.zero_()
         self.status.zero_()
+        if self.kv8 is not None:
+            self.held.zero_()
+            self.rot.zero_()
+            self.n_held = 0
+            for w in self.kv8_weights:
+                if w is not None:
+                    w.zero_()

@@ -71,18 +71,23 @@ class KV8Cache:
         self._ws: dict = {}
 
     @classmethod
-    def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, device) -> "KV8Cache":
+    def empty(cls, batch: int, kv_heads: int, capacity: int, head_dim: int, device,
+              status: torch.Tensor | None = None) -> "KV8Cache":
         """A cache for ``capacity`` positions (rounded up to whole blocks)."""
         cap = -(-max(capacity, 1) // BLOCK) * BLOCK
         new = lambda *s, t: torch.zeros(*s, dtype=t, device=device)
         codes = [new(batch, kv_heads, cap, head_dim, t=torch.uint8) for _ in "kv"]
         scales = [new(batch, kv_heads, cap // BLOCK, t=torch.float32) for _ in "kv"]
         tails = [new(batch, kv_heads, BLOCK, head_dim, t=torch.float16) for _ in "kv"]
-        return cls(*codes, *scales, *tails)
+        return cls(*codes, *scales, *tails, status=status)
 
     def new_weights(self) -> torch.Tensor:
         """Zeroed attention weights for :func:`kv8_decode` to accumulate."""
         return torch.zeros(self.batch, self.kv_heads, self.capacity, dtype=torch.float32, device=self.device)
+
+    def new_workspace(self, n: int, q_heads: int, weights: bool = False) -> torch.Tensor:
+        """Scratch for attention calls of at most these sizes on this cache's shape."""
+        return torch.zeros(self.workspace_bytes(n, q_heads, weights), dtype=torch.uint8, device=self.device)
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales,
@@ -104,17 +109,26 @@ _scratch: dict = {}
 _scratch_kept: list = []
 
 
-def _workspace(cache: KV8Cache, nbytes: int) -> tuple:
-    """Zero-filled scratch (address, bytes, tensor) of the attention calls, one per (device, stream); the
-    kernels leave its counters at zero.  An outgrown buffer is kept, since a
-    captured graph may refer to it.  A capture that needs a new one gets its
-    own, whose fill is part of the graph."""
+def _workspace(cache: KV8Cache, n: int, q_heads: int, weights: bool, given) -> tuple:
+    """Zero-filled scratch (address, bytes, tensor) of the attention calls; the
+    kernels leave its counters at zero.  Without a given one there is one per
+    (device, stream), and an outgrown buffer is kept, since launched work may
+    still use it.  A call in a capture gets its own, whose fill is part of the
+    graph: the graph may be replayed on any stream."""
+    nbytes = cache.workspace_bytes(n, q_heads, weights)
+    if given is not None:
+        if (given.dtype is not torch.uint8 or given.get_device() != cache.index or not given.is_contiguous()
+                or given.data_ptr() & 255 or given.numel() < nbytes):
+            raise ValueError(f"workspace must be a contiguous 256-byte aligned uint8 tensor of at least {nbytes} "
+                             f"bytes on {cache.device}")
+        return given.data_ptr(), given.numel(), given
+    if torch.cuda.is_current_stream_capturing():
+        new = torch.zeros(nbytes, dtype=torch.uint8, device=cache.device)
+        return new.data_ptr(), nbytes, new
     key = (cache.index, _lib.stream_handle(cache.device))
     buf = _scratch.get(key)
     if buf is None or buf[1] < nbytes:
         new = torch.zeros(max(nbytes, 1 << 20) * 5 // 4, dtype=torch.uint8, device=cache.device)
-        if torch.cuda.is_current_stream_capturing():
-            return new.data_ptr(), new.numel(), new
         if buf is not None:
             _scratch_kept.append(buf)
         buf = _scratch[key] = (new.data_ptr(), new.numel(), new)
@@ -228,14 +242,16 @@ def kv8_restore(cache: KV8Cache, lens: torch.Tensor, start: torch.Tensor | None 
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, counts: torch.Tensor | None = None,
-                  scale: float | None = None, rope=None, out: torch.Tensor | None = None) -> torch.Tensor:
+                  scale: float | None = None, rope=None, out: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the last ``counts[b]`` (default: n) of each sequence's
     ``lens[b]`` tokens: ``q`` ``[batch, n, q_heads, head_dim]`` -> the same shape.
 
     Rows ``i >= counts[b]`` and rows that attend nothing are zero.  ``scale``
     defaults to ``1 / sqrt(head_dim)``; ``rope = (cos, sin, positions)``
     rotates the queries.  ``q_heads`` is a multiple of ``kv_heads``, at most 16
-    to each.
+    to each.  ``workspace`` (:meth:`KV8Cache.new_workspace`) may be given for
+    calls that run in order; otherwise one is kept per stream.
     """
     if q.dim() != 4:
         raise ValueError("q must be [batch, tokens, q_heads, head_dim]")
@@ -243,7 +259,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, counts: 
     shape = (cache.batch, n, nq, cache.head_dim)
     q = _rows(q, "q", shape, cache)
     out = _output(out, q, cache)
-    ws = _workspace(cache, cache.workspace_bytes(n, nq, False))
+    ws = _workspace(cache, n, nq, False, workspace)
     _call(cache, "pp_kv8_attention", q.data_ptr(), _c_strides(*q.stride()[:3]), n, nq, _ints(lens, "lens", cache),
           _ints(counts, "counts", cache), 1 / math.sqrt(cache.head_dim) if scale is None else scale, out.data_ptr(),
           _c_strides(*out.stride()[:3]), *_rope(rope, cache), ws[0], ws[1])
@@ -252,7 +268,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, counts: 
 
 def kv8_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, pos: torch.Tensor,
                weights: torch.Tensor | None = None, scale: float | None = None, rope=None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """One token per sequence: append ``k``, ``v`` ``[batch, kv_heads, head_dim]``
     at ``pos[b]`` and attend with ``q`` ``[batch, q_heads, head_dim]`` to positions
     ``0 .. pos[b]``.
@@ -260,7 +276,7 @@ def kv8_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV8Cach
     ``weights`` (:meth:`KV8Cache.new_weights`), if given, has each position's
     softmax weights added, summed over the query heads of the kv head.  A
     negative position marks an unused sequence (zero output).  ``rope`` rotates
-    queries and keys.
+    queries and keys; ``workspace`` as in :func:`kv8_attention`.
     """
     if q.dim() != 3:
         raise ValueError("q must be [batch, q_heads, head_dim]")
@@ -268,7 +284,7 @@ def kv8_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KV8Cach
     q = _rows(q, "q", (b, nq, hd), cache)
     k, v = _rows(k, "k", (b, cache.kv_heads, hd), cache), _rows(v, "v", (b, cache.kv_heads, hd), cache)
     out = _output(out, q, cache)
-    ws = _workspace(cache, cache.workspace_bytes(1, nq, weights is not None))
+    ws = _workspace(cache, 1, nq, weights is not None, workspace)
     _call(cache, "pp_kv8_decode", q.data_ptr(), _c_strides(*q.stride()[:2]), nq, k.data_ptr(),
           _c_strides(*k.stride()[:2]), v.data_ptr(), _c_strides(*v.stride()[:2]), _ints(pos, "pos", cache),
           1 / math.sqrt(hd) if scale is None else scale, _weights(weights, "weights", cache), out.data_ptr(),

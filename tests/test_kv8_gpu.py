@@ -460,6 +460,42 @@ def test_streams_and_graph(cuda):
     assert torch.equal(w1, w2)
 
 
+def test_workspaces(cuda):
+    """A given workspace gives the same bits and is left ready for the next
+    call; a graph captured without one owns its scratch, whatever the streams
+    around it do."""
+    from polar_pack_b200.kv8 import kv8_attention, kv8_decode
+    g = _gen(cuda, 41)
+    lens = [700, 64, 0, 131]
+    cache, ref = _new(4, 2, 768, 128, cuda), kr.RefKV(4, 2, 128)
+    _fill(cache, ref, lens, _gen(cuda, 42))
+    q, k, v = _rand(g, 4, 14, 128), _rand(g, 4, 2, 128), _rand(g, 4, 2, 128)
+    pos, n = _ints(lens, cuda), _ints([x + 1 for x in lens], cuda)
+    want = kv8_decode(q, k, v, cache, pos)
+    many = _rand(g, 4, 40, 14, 128)
+    both = _ints([min(x, 40) for x in lens], cuda)
+    prompt = kv8_attention(many, cache, _ints(lens, cuda), both)
+    ws = cache.new_workspace(40, 14)
+    step = cache.new_workspace(1, 14, True)
+    w = cache.new_weights()
+    for _ in range(3):      # the same token again: the cache stays the same
+        assert torch.equal(kv8_decode(q, k, v, cache, pos, weights=w, workspace=step), want)
+        assert torch.equal(kv8_attention(q[:, None], cache, n, workspace=step)[:, 0], want)
+        assert torch.equal(kv8_attention(many, cache, _ints(lens, cuda), both, workspace=ws), prompt)
+    for bad in (step[:-256], step[1:], step.view(torch.int8), step.cpu()):
+        with pytest.raises(ValueError):
+            kv8_decode(q, k, v, cache, pos, weights=w, workspace=bad)
+    torch.cuda.synchronize()
+    s, graph = torch.cuda.Stream(cuda), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        a = kv8_decode(q, k, v, cache, pos)
+        b = kv8_attention(q[:, None], cache, n)[:, 0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)
+
+
 # ------------------------------------------------------------ eviction ----
 @pytest.mark.parametrize("hd,keep,sinks,recent,lens", [
     (128, 100, 4, 10, [300, 100, 101, 0]),
