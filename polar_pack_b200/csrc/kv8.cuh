@@ -102,32 +102,40 @@ __device__ __forceinline__ float kv8_amax8_finite(uint4 x) {
 // Correctly rounded divisions, so that the codes follow from the definition.
 __device__ __forceinline__ float kv8_scale(float amax) { return __fdiv_rn(amax, 127.f); }
 
-// round(x / scale) + 128 in the low byte of the result: adding 1.5 * 2^23 + 128
-// rounds to a whole number, ties to even.  x * (1 / scale) is within 2^-22 of
-// the quotient (both below 128), so only within 1e-4 of a tie can it round
-// otherwise: those few are divided.
-__device__ __forceinline__ uint32_t kv8_code(float x, float scale, float per_scale) {
-  constexpr float kWhole = 12583040.f;
-  float q = x * per_scale;
-  const float y = q + kWhole, off = q - (y - kWhole);
-  if (fabsf(off) > 0.4999f) return __float_as_uint(__fdiv_rn(x, scale) + kWhole);
-  return __float_as_uint(y);
-}
-
-// Codes of eight values.  finite: all of the block's values are.
+// Codes of eight values; finite: all of the block's values are.  The code is
+// the low byte of x / scale + 1.5 * 2^23 + 128: the addition rounds to a whole
+// number, ties to even.  x * (1 / scale) is within 2^-15 of the quotient (both
+// below 128), so only within 4e-5 of a tie can it round otherwise: eight
+// values with one there are divided.  Two values an instruction, one branch
+// for eight.
 __device__ __forceinline__ uint2 kv8_codes8(uint4 x, float scale, float per_scale, bool finite) {
+  constexpr float kWhole = 12583040.f;
+  const uint64_t whole = f32_pair(kWhole, kWhole), minus = f32_pair(-kWhole, -kWhole), per = f32_pair(per_scale, per_scale);
+  float2 f[4];
+  float y[8], off = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = __half22float2(u2h(kv8_word(x, i)));
+    if (!finite) f[i] = make_float2(kv8_finite(f[i].x), kv8_finite(f[i].y));
+    const uint64_t q = f32_mul2(f32_pair(f[i].x, f[i].y), per), r = f32_add2(q, whole), n = f32_add2(r, minus);
+    float q0, q1, n0, n1;
+    f32_split(q, q0, q1);
+    f32_split(n, n0, n1);
+    f32_split(r, y[2 * i], y[2 * i + 1]);
+    off = fmaxf(off, fmaxf(fabsf(q0 - n0), fabsf(q1 - n1)));
+  }
+  if (off > 0.49996f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[2 * i] = __fdiv_rn(f[i].x, scale) + kWhole;
+      y[2 * i + 1] = __fdiv_rn(f[i].y, scale) + kWhole;
+    }
+  }
   uint32_t o[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t c[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float2 f = __half22float2(u2h(kv8_word(x, 2 * h + i)));
-      if (!finite) f = make_float2(kv8_finite(f.x), kv8_finite(f.y));
-      c[2 * i] = kv8_code(f.x, scale, per_scale);
-      c[2 * i + 1] = kv8_code(f.y, scale, per_scale);
-    }
-    o[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    const auto c = [&](int i) { return __float_as_uint(y[4 * h + i]); };
+    o[h] = __byte_perm(__byte_perm(c(0), c(1), 0x0040), __byte_perm(c(2), c(3), 0x0040), 0x5410);
   }
   return make_uint2(o[0], o[1]);
 }
@@ -135,13 +143,16 @@ __device__ __forceinline__ uint2 kv8_codes8(uint4 x, float scale, float per_scal
 // fp16((code - 128) * scale) of eight codes: a byte in the low end of 2^23 is
 // 2^23 + code, exactly.
 __device__ __forceinline__ uint4 kv8_values8(uint2 c, float scale) {
+  const uint64_t zero = f32_pair(-8388736.f, -8388736.f), by = f32_pair(scale, scale);
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = i < 2 ? c.x : c.y;
-    const float a = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7442 : 0x7440)) - 8388736.f;
-    const float b = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7443 : 0x7441)) - 8388736.f;
-    r[i] = h2u(__floats2half2_rn(a * scale, b * scale));
+    const float a = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7442 : 0x7440));
+    const float b = __uint_as_float(__byte_perm(w, 0x4b000000u, i & 1 ? 0x7443 : 0x7441));
+    float x, y;
+    f32_split(f32_mul2(f32_add2(f32_pair(a, b), zero), by), x, y);
+    r[i] = h2u(__floats2half2_rn(x, y));
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -189,12 +200,24 @@ __device__ __forceinline__ Kv8Scale kv8_block_scale(const uint4 (&v)[N], float* 
   return kv8_make_scale(all(m), false);
 }
 
-// Eight stored values of position t of a sequence of `len` tokens, FP16.
-__device__ __forceinline__ uint4 kv8_read8(const Kv8Cache& c, int w, int b, int h, int t, int len, int d0) {
-  if (t / kKvBlock == kv8_last_block(len))
-    return *reinterpret_cast<const uint4*>(c.tail_row(w, b, h, t % kKvBlock) + d0);
-  return kv8_values8(*reinterpret_cast<const uint2*>(c.code_row(w, b, h, t) + d0), *c.scale(w, b, h, t / kKvBlock));
-}
+// One head's keys or values.
+template <int HD>
+struct Kv8Head {
+  uint8_t* codes;  // [capacity][HD]
+  float* scales;   // [capacity / 64]
+  __half* tail;    // [64][HD]
+
+  __device__ __forceinline__ Kv8Head(const Kv8Cache& c, int w, int b, int h)
+      : codes(pick(c.codes, w) + c.head(b, h) * c.cap * HD),
+        scales(pick(c.scales, w) + c.head(b, h) * (c.cap / kKvBlock)),
+        tail(pick(c.tail, w) + c.head(b, h) * (kKvBlock * HD)) {}
+  // Eight stored values of position t, FP16; last: the block in the tail.
+  __device__ __forceinline__ uint4 read8(int t, int last, int d0) const {
+    const int block = (unsigned)t / kKvBlock;
+    if (block == last) return *reinterpret_cast<const uint4*>(tail + t % kKvBlock * HD + d0);
+    return kv8_values8(*reinterpret_cast<const uint2*>(codes + ((int64_t)t * HD + d0)), scales[block]);
+  }
+};
 
 // Checks a descriptor and fills the kernels' view of it.
 int kv8_cache(const char* who, const pp_kv8_cache* c, Kv8Cache* out);

@@ -1,7 +1,11 @@
 // Writing, reading back and evicting from the 8-bit KV cache (kv8.cuh).
+#include <cooperative_groups.h>
+
 #include "kv8.cuh"
 
 namespace pp {
+
+namespace cg = cooperative_groups;
 
 int kv8_cache(const char* who, const pp_kv8_cache* c, Kv8Cache* out) {
   if (!c) {
@@ -86,6 +90,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
   const int len = pos + cnt, last = kv8_last_block(len);
   const int block = pos / kKvBlock + blockIdx.x;
   if (block > last) return;
+  const Kv8Head<HD> to(p.c, w, b, h);
   const __half* x = pick(p.x, w) + b * pick(p.ldb, w) + h * pick(p.ldh, w);
   const int64_t ldt = pick(p.ldt, w);
   auto row8 = [&](int t, int d0) { return kv8_load8(x + (int64_t)(t - pos) * ldt, d0, HD, rope, r0 + t - pos); };
@@ -96,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
     const int t = block * kKvBlock + r;
     v[i] = make_uint4(0, 0, 0, 0);
     if (t < pos)
-      v[i] = *reinterpret_cast<const uint4*>(p.c.tail_row(w, b, h, r) + d0);
+      v[i] = *reinterpret_cast<const uint4*>(to.tail + r * HD + d0);
     else if (t < len)
       v[i] = row8(t, d0);
   }
@@ -104,10 +109,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
     const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      *reinterpret_cast<uint2*>(p.c.code_row(w, b, h, block * kKvBlock + r) + d0) = kv8_codes8(v[i], q);
+      const int e = i * kThreads + threadIdx.x;
+      *reinterpret_cast<uint2*>(to.codes + (int64_t)block * (kKvBlock * HD) + e * 8) = kv8_codes8(v[i], q);
     }
-    if (threadIdx.x == 0) *p.c.scale(w, b, h, block) = q.scale;
+    if (threadIdx.x == 0) to.scales[block] = q.scale;
   }
   if (blockIdx.x != 0) return;
   __syncthreads();  // the tail's old rows have been read
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
     const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
     const int t = last * kKvBlock + r;
     if (t >= pos && t < len)
-      *reinterpret_cast<uint4*>(p.c.tail_row(w, b, h, r) + d0) = last == block ? v[i] : row8(t, d0);
+      *reinterpret_cast<uint4*>(to.tail + r * HD + d0) = last == block ? v[i] : row8(t, d0);
   }
 }
 
@@ -140,19 +145,22 @@ __global__ void __launch_bounds__(kThreads) kv8_restore_kernel(const RestorePara
   const int len = p.lens[b], first = p.start ? p.start[b] : 0;
   const bool ok = len <= p.c.cap;
   if (!ok && blockIdx.x == 0 && h == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, 5);
+  const Kv8Head<HD> head(p.c, w, b, h);
+  const int last = kv8_last_block(len), i0 = blockIdx.x * kKvBlock, n = min(kKvBlock, p.count - i0);
   uint4 v[kVecs];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
-    const int e = k * kThreads + threadIdx.x, i = blockIdx.x * kKvBlock + e / (HD / 8);
-    const int64_t t = (int64_t)first + i;
+    const int e = k * kThreads + threadIdx.x, i = e / (HD / 8);
+    const int64_t t = (int64_t)first + i0 + i;
     v[k] = make_uint4(0, 0, 0, 0);
-    if (ok && i < p.count && t >= 0 && t < len) v[k] = kv8_read8(p.c, w, b, h, (int)t, len, e % (HD / 8) * 8);
+    if (ok && i < n && t >= 0 && t < len) v[k] = head.read8((int)t, last, e % (HD / 8) * 8);
   }
+  const int ld = p.c.nkv * HD;
+  __half* out = pick(p.out, w) + ((int64_t)b * p.count + i0) * ld + h * HD;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
-    const int e = k * kThreads + threadIdx.x, i = blockIdx.x * kKvBlock + e / (HD / 8);
-    if (i < p.count)
-      *reinterpret_cast<uint4*>(pick(p.out, w) + (((int64_t)b * p.count + i) * p.c.nkv + h) * HD + e % (HD / 8) * 8) = v[k];
+    const int e = k * kThreads + threadIdx.x, i = e / (HD / 8);
+    if (i < n) *reinterpret_cast<uint4*>(out + i * ld + e % (HD / 8) * 8) = v[k];
   }
 }
 
@@ -176,66 +184,93 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelThreads = 1024;
-constexpr int kSelRounds = 32;            // of kSelThreads keys, whose kept ones are counted together
-constexpr int kSelCached = 48 * 1024;     // keys that fit shared memory
+constexpr int kSelRounds = 16;         // of kSelThreads keys, whose kept ones are counted together
+constexpr int kSelCached = 48 * 1024;  // keys that fit shared memory
+constexpr int kSelParts = 8;           // CTAs of a cluster, at most
 
-// CTA (head, sequence) finds the keep-th largest key by four passes over the
-// keys' bytes (a histogram each, equal bytes of a warp counted at once), then
-// writes the kept positions in order: those above it, and as many equal to it,
-// lowest first, as there is room.  The keys stay in shared memory where they
-// fit (`cached` keys).
-__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictParams p, int cached) {
-  __shared__ int hist[256];
+__host__ __device__ __forceinline__ int select_part(int len, int parts) {  // positions of a CTA
+  return (int)(((int64_t)len + parts - 1) / parts + 31) & ~31;
+}
+
+// A cluster (head, sequence) finds the keep-th largest key by four passes over
+// the keys' bytes: each CTA counts its stretch of positions (equal bytes of a
+// warp at once), all add the cluster's counts up.  Then each writes its kept
+// positions in order: those above the key, and as many equal to it, lowest
+// first, as there is room.  The keys stay in shared memory where they fit
+// (`cached` of a CTA's).
+__global__ void __launch_bounds__(kSelThreads, 2) kv8_select_kernel(const EvictParams p, int cached) {
+  __shared__ int hist[4][256];  // this CTA's counts, a pass each
+  __shared__ int total[256];
   __shared__ int above_of[kSelRounds * 32 + 1], equal_of[kSelRounds * 32 + 1];  // kept before a round's warp
-  __shared__ int s_digit, s_left;
+  __shared__ int digit[4], s_left, s_above;
   pdl_launch_dependents();
   pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   uint32_t* keys = reinterpret_cast<uint32_t*>(pp_smem);
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.x / parts, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int len = p.lens[b];
   const bool ok = len <= p.c.cap;
   if (!ok && tid == 0 && p.status) atomicExch(p.status, 5);
   len = ok ? max(len, 0) : 0;
   const int m = min(len, p.keep);
-  if (h == 0 && tid == 0) p.new_lens[b] = m;
+  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = m;
   const float* wt = p.weights + p.c.head(b, h) * p.c.cap;
   float* to_wt = p.to_weights + p.to.head(b, h) * p.to.cap;
   int* kept = p.kept + p.c.head(b, h) * p.keep;
-  auto make_key = [&](int t) { return t < p.sinks || t >= len - p.recent ? 0xffffffffu : weight_key(wt[t]); };
-  for (int t = m + tid; t < p.keep; t += kSelThreads) kept[t] = -1;
-  for (int t = m + tid; t < p.to.cap; t += kSelThreads) to_wt[t] = 0.f;
+  const int me = part * kSelThreads + tid, all = parts * kSelThreads;
+  for (int t = m + me; t < p.keep; t += all) kept[t] = -1;
+  for (int t = m + me; t < p.to.cap; t += all) to_wt[t] = 0.f;
   if (m == len) {
-    for (int t = tid; t < len; t += kSelThreads) {
+    for (int t = me; t < len; t += all) {
       kept[t] = t;
       to_wt[t] = wt[t];
     }
     return;
   }
+  const int size = select_part(len, parts), lo = min(len, part * size), hi = min(len, lo + size);
+  auto make_key = [&](int t) { return t < p.sinks || t >= len - p.recent ? 0xffffffffu : weight_key(wt[t]); };
+  for (int i = tid; i < 4 * 256; i += kSelThreads) hist[i >> 8][i & 255] = 0;
+  if (tid == 0) s_above = 0;
 #pragma unroll 4
-  for (int t = tid; t < min(len, cached); t += kSelThreads) keys[t] = make_key(t);
-  auto key = [&](int t) { return t < cached ? keys[t] : make_key(t); };  // a thread reads its own
+  for (int t = lo + tid; t < min(hi, lo + cached); t += kSelThreads) keys[t - lo] = make_key(t);
+  auto key = [&](int t) { return t - lo < cached ? keys[t - lo] : make_key(t); };  // a thread reads its own
+  auto meet = [&] {
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
+  };
+  __syncthreads();
   uint32_t cut = 0;
   int left = m;  // kept positions among the keys that agree with `cut` so far
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
+#pragma unroll 1
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
 #pragma unroll 2
-    for (int t0 = 0; t0 < len; t0 += kSelThreads) {
+    for (int t0 = lo; t0 < hi; t0 += kSelThreads) {
       const int t = t0 + tid;
-      const uint32_t k = t < len ? key(t) : 0;
-      const bool in = t < len && (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8)));
+      const uint32_t k = t < hi ? key(t) : 0;
+      const bool in = t < hi && (pass == 0 || (k >> (shift + 8)) == (cut >> (shift + 8)));
       const uint32_t d = in ? (k >> shift) & 255 : 256;
       if (__any_sync(0xffffffffu, in)) {
         const uint32_t same = __match_any_sync(0xffffffffu, d);
-        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
+        if (in && lane == __ffs(same) - 1) atomicAdd(&hist[pass][d], __popc(same));
       }
     }
-    __syncthreads();
+    meet();
+    if (parts > 1) {
+      if (tid < 256) {
+        int n = 0;
+        for (int c = 0; c < parts; ++c) n += *cluster.map_shared_rank(&hist[pass][tid], c);
+        total[tid] = n;
+      }
+      __syncthreads();
+    }
     if (warp == 0) {
+      const int* count = parts > 1 ? total : hist[pass];
       // the digit at which the count from the top reaches `left`: lane l has digits 255 - 8 l and down
       int n[8], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += n[i] = hist[255 - 8 * lane - i];
+      for (int i = 0; i < 8; ++i) sum += n[i] = count[255 - 8 * lane - i];
       int upto = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -244,23 +279,39 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictPara
       }
       int above = upto - sum;
       if (above < left && upto >= left) {
-        int i = 0;
-        while (above + n[i] < left) above += n[i++];
-        s_digit = 255 - 8 * lane - i;
+        int d = 255 - 8 * lane;
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (d == 255 - 8 * lane - i && above + n[i] < left) {
+            above += n[i];
+            --d;
+          }
+        digit[pass] = d;
         s_left = left - above;
       }
     }
     __syncthreads();
-    cut |= (uint32_t)s_digit << shift;
+    cut |= (uint32_t)digit[pass] << shift;
     left = s_left;
   }
-  int base_gt = 0, base_eq = 0;  // kept above / equal before these rounds
-  for (int r0 = 0; r0 < len; r0 += kSelRounds * kSelThreads) {
-    const int rounds = min(kSelRounds, (len - r0 + kSelThreads - 1) / kSelThreads);
+  int base_gt = 0, base_eq = 0;  // keys above / equal to the cut before these rounds
+  if (parts > 1) {
+    const int d = tid & 255, n = d > digit[tid >> 8] ? hist[tid >> 8][d] : 0;
+    const int sum = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0 && sum) atomicAdd(&s_above, sum);
+    cluster.sync();
+    for (int c = 0; c < part; ++c) {
+      base_gt += *cluster.map_shared_rank(&s_above, c);
+      base_eq += *cluster.map_shared_rank(&hist[3][cut & 255], c);
+    }
+    cluster.sync();  // the others' counts have been read
+  }
+  for (int r0 = lo; r0 < hi; r0 += kSelRounds * kSelThreads) {
+    const int rounds = min(kSelRounds, (hi - r0 + kSelThreads - 1) / kSelThreads);
     for (int i = 0; i < rounds; ++i) {
       const int t = r0 + i * kSelThreads + tid;
-      const uint32_t k = t < len ? key(t) : 0;
-      const uint32_t bg = __ballot_sync(0xffffffffu, t < len && k > cut), be = __ballot_sync(0xffffffffu, t < len && k == cut);
+      const uint32_t k = t < hi ? key(t) : 0;
+      const uint32_t bg = __ballot_sync(0xffffffffu, t < hi && k > cut), be = __ballot_sync(0xffffffffu, t < hi && k == cut);
       if (lane == 0) {
         above_of[i * 32 + warp] = __popc(bg);
         equal_of[i * 32 + warp] = __popc(be);
@@ -286,8 +337,8 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictPara
     __syncthreads();
     for (int i = 0; i < rounds; ++i) {
       const int t = r0 + i * kSelThreads + tid;
-      const uint32_t k = t < len ? key(t) : 0;
-      const bool gt = t < len && k > cut, eq = t < len && k == cut;
+      const uint32_t k = t < hi ? key(t) : 0;
+      const bool gt = t < hi && k > cut, eq = t < hi && k == cut;
       const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq), below = (1u << lane) - 1;
       const int g = base_gt + above_of[i * 32 + warp] + __popc(bg & below);
       const int q = base_eq + equal_of[i * 32 + warp] + __popc(be & below);
@@ -308,44 +359,48 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const EvictPara
 // whole coded block of the old cache is copied, codes and scale, so that
 // repeated evictions do not requantise what does not move apart.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv8_gather_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kThreads, 6) kv8_gather_kernel(const EvictParams p) {
   constexpr int kVecs = kKvBlock * HD / 8 / kThreads;
   __shared__ float red[kThreads / 32];
-  __shared__ int src[kKvBlock];
   pdl_launch_dependents();
   pdl_wait();
   const int block = blockIdx.x, h = blockIdx.y, b = blockIdx.z >> 1, w = blockIdx.z & 1;
-  const int len = p.lens[b], m = p.new_lens[b];
-  if (block * kKvBlock >= m) return;
-  const bool full = (block + 1) * kKvBlock <= m, last = block == kv8_last_block(m);
+  // the positions (-1 past the new length) are read beside the lengths, not after them
   const int* kept = p.kept + p.c.head(b, h) * p.keep + block * kKvBlock;
-  if (threadIdx.x < kKvBlock) src[threadIdx.x] = block * kKvBlock + threadIdx.x < m ? kept[threadIdx.x] : -1;
-  __syncthreads();
-  const int f = src[0];
-  const bool whole = full && f % kKvBlock == 0 && src[kKvBlock - 1] - f == kKvBlock - 1 &&
-                     f / kKvBlock != kv8_last_block(len);
+  const int room = p.keep - block * kKvBlock;
+  int src[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int r = (i * kThreads + threadIdx.x) / (HD / 8);
+    src[i] = r < room ? kept[r] : -1;
+  }
+  const int f = kept[0], g = room >= kKvBlock ? kept[kKvBlock - 1] : -1;
+  const int len = p.lens[b], m = p.new_lens[b];
+  if (f < 0) return;
+  const bool full = g >= 0, last = block == kv8_last_block(m);
+  const bool whole = full && f % kKvBlock == 0 && g - f == kKvBlock - 1 && f / kKvBlock != kv8_last_block(len);
+  const Kv8Head<HD> from(p.c, w, b, h), to(p.to, w, b, h);
+  const int old_last = kv8_last_block(len);
   uint4 v[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    v[i] = src[r] >= 0 ? kv8_read8(p.c, w, b, h, src[r], len, d0) : make_uint4(0, 0, 0, 0);
+    const int d0 = (i * kThreads + threadIdx.x) % (HD / 8) * 8;
+    v[i] = src[i] >= 0 ? from.read8(src[i], old_last, d0) : make_uint4(0, 0, 0, 0);
   }
   if (last) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-      if (src[r] >= 0) *reinterpret_cast<uint4*>(p.to.tail_row(w, b, h, r) + d0) = v[i];
-    }
+    for (int i = 0; i < kVecs; ++i)
+      if (src[i] >= 0) *reinterpret_cast<uint4*>(to.tail + (i * kThreads + threadIdx.x) * 8) = v[i];
   }
   if (!full) return;
   const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
+  uint8_t* out = to.codes + (int64_t)block * (kKvBlock * HD) + threadIdx.x * 8;
+  const uint8_t* same = from.codes + (int64_t)f * HD + threadIdx.x * 8;
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    const uint2 c = whole ? *reinterpret_cast<const uint2*>(p.c.code_row(w, b, h, f + r) + d0) : kv8_codes8(v[i], q);
-    *reinterpret_cast<uint2*>(p.to.code_row(w, b, h, block * kKvBlock + r) + d0) = c;
-  }
-  if (threadIdx.x == 0) *p.to.scale(w, b, h, block) = whole ? *p.c.scale(w, b, h, f / kKvBlock) : q.scale;
+  for (int i = 0; i < kVecs; ++i)
+    *reinterpret_cast<uint2*>(out + i * kThreads * 8) =
+        whole ? *reinterpret_cast<const uint2*>(same + i * kThreads * 8) : kv8_codes8(v[i], q);
+  if (threadIdx.x == 0) to.scales[block] = whole ? from.scales[f / kKvBlock] : q.scale;
 }
 
 bool g_select_attr[64];
@@ -446,11 +501,17 @@ int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int*
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int lim = 0;
   if (int rc = pp::ensure_smem_attr(pp::kv8_select_kernel, pp::g_select_attr, pp::g_select_limit, &lim)) return rc;
-  int cached = p.c.cap < pp::kSelCached ? p.c.cap : pp::kSelCached;
+  // long caches: as many CTAs to a head as find SMs of their own, each with two rounds of positions at least
+  const int sms = pp::device_sm_count(pp::current_device());
+  int parts = 1;
+  while (parts < pp::kSelParts && (int64_t)p.c.nkv * p.c.batch * parts <= sms && p.c.cap >= parts * 4 * pp::kSelThreads)
+    parts *= 2;
+  int cached = pp::select_part(p.c.cap, parts);
+  if (cached > pp::kSelCached) cached = pp::kSelCached;
   if (cached * 4 > lim) cached = lim / 4;
-  if (int rc = pp::launch_kernel("kv8_select_kernel", pp::launch_overlap(), pp::kv8_select_kernel,
-                                 dim3((unsigned)p.c.nkv, (unsigned)p.c.batch), dim3(pp::kSelThreads), (size_t)cached * 4,
-                                 s, p, cached))
+  if (int rc = pp::launch_clusters("kv8_select_kernel", pp::launch_overlap(), parts > 1 ? (unsigned)parts : 0u, pp::kv8_select_kernel,
+                                   dim3((unsigned)(p.c.nkv * parts), (unsigned)p.c.batch), dim3(pp::kSelThreads),
+                                   (size_t)cached * 4, s, p, cached))
     return rc;
   // started early whatever the overlap setting: it waits for the selection itself
   return pp::launch_kernel("kv8_gather_kernel", true,

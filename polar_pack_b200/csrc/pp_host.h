@@ -69,21 +69,28 @@ int ensure_smem_attr(K kernel, bool* done_flags, int* limits, int* max_dynamic) 
 // support it, switched by pp_set_launch_overlap().
 bool launch_overlap();
 
-// cudaLaunchKernelEx with programmatic stream serialisation when
-// `overlap` is set; records launch errors.
+// cudaLaunchKernelEx over clusters of `cluster` CTAs (0: none) with
+// programmatic stream serialisation when `overlap` is set; records launch errors.
 template <typename... KArgs, typename... Args>
-int launch_kernel(const char* what, bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                  cudaStream_t stream, Args&&... args) {
+int launch_clusters(const char* what, bool overlap, unsigned cluster, void (*kernel)(KArgs...), dim3 grid, dim3 block,
+                    size_t smem, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (overlap) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n++].val.clusterDim = {cluster, 1, 1};
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = overlap ? 1 : 0;
+  cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -91,6 +98,12 @@ int launch_kernel(const char* what, bool overlap, void (*kernel)(KArgs...), dim3
     return PP_ERR_CUDA;
   }
   return check_launch(what);
+}
+
+template <typename... KArgs, typename... Args>
+int launch_kernel(const char* what, bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                  cudaStream_t stream, Args&&... args) {
+  return launch_clusters(what, overlap, 0, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

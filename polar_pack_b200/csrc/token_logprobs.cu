@@ -95,30 +95,18 @@ struct Stat {
   }
 };
 
-// Pairs of FP32 values, two operations an instruction.
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void split(uint64_t r, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
-}
-
 // A thread's sums over pairs of logits, beside the maximum m.
 struct PairSums {
   uint64_t z = 0, w = 0;
   __device__ __forceinline__ void add(float a, float b, uint64_t minus_m, uint64_t log2e) {
-    uint64_t d, y;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair(a, b)), "l"(minus_m));
+    uint64_t d = f32_add2(f32_pair(a, b), minus_m);
     float d0, d1, e0, e1;
-    split(d, d0, d1);
-    d = pair(fmaxf(d0, -200.f), fmaxf(d1, -200.f));  // -inf counts nothing
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(d), "l"(log2e));
-    split(y, e0, e1);
-    const uint64_t e = pair(ex2a(e0), ex2a(e1));
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(z) : "l"(e));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(w) : "l"(e), "l"(d));
+    f32_split(d, d0, d1);
+    d = f32_pair(fmaxf(d0, -200.f), fmaxf(d1, -200.f));  // -inf counts nothing
+    f32_split(f32_mul2(d, log2e), e0, e1);
+    const uint64_t e = f32_pair(ex2a(e0), ex2a(e1));
+    z = f32_add2(z, e);
+    w = f32_fma2(e, d, w);
   }
 };
 
@@ -243,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
         if (at < kList) s.list[at] = k;
       }
     };
-    const uint64_t log2e = pair(kLog2e, kLog2e);
+    const uint64_t log2e = f32_pair(kLog2e, kLog2e);
     // this thread's logits of a batch whose vectors may hold listed ones
     auto scan = [&](int b0, auto&& use) {
 #pragma unroll 1
@@ -292,13 +280,13 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
           raise(top);
           if (st.m > -INFINITY) {
             PairSums sums;
-            const uint64_t minus_m = pair(-st.m, -st.m);
+            const uint64_t minus_m = f32_pair(-st.m, -st.m);
 #pragma unroll
             for (int e = 0; e < N; e += 2) sums.add(q[k].get(e), q[k].get(e + 1), minus_m, log2e);
             float a, c;
-            split(sums.z, a, c);
+            f32_split(sums.z, a, c);
             st.z += a + c;
-            split(sums.w, a, c);
+            f32_split(sums.w, a, c);
             st.w += a + c;
           }
           if (TOP && (best_at < 0 || !(top <= best)) && best == best) {
@@ -463,26 +451,10 @@ int launch(const ScoreParams& p, cudaStream_t stream) {
   while (parts < kMaxCluster && p.rows * parts * 2 <= sms &&
          (int64_t)p.vocab * (int)sizeof(T) >= (int64_t)parts * 2 * kThreads * 16)
     parts *= 2;
-  cudaLaunchConfig_t cfg{};
   const int64_t rows = p.rows < (1 << 24) ? p.rows : (1 << 24);
-  cfg.gridDim = dim3((unsigned)(rows * parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = launch_overlap() ? 2 : 1;
-  const cudaError_t e = p.top ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, p)
-                              : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, p);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    set_error("token_logprobs_kernel: %s", cudaGetErrorString(e));
-    return PP_ERR_CUDA;
-  }
-  return check_launch("token_logprobs_kernel");
+  return launch_clusters("token_logprobs_kernel", launch_overlap(), (unsigned)parts,
+                         p.top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
+                         dim3((unsigned)(rows * parts)), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
