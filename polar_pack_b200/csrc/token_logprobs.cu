@@ -12,7 +12,7 @@
 // alternatives logits are whole numbers (value, then lower index), all
 // different; the top-th largest of the best of 64 groups of threads is a bound
 // that at least `top` logits reach, and only the logits of threads whose best
-// reaches it, a few of the 512, are gone through again (by all threads) for a
+// reaches it, a few of the CTA, are gone through again (by all threads) for a
 // list in shared memory, of which the `top` largest are ranked.  A row that lists
 // more than there is room for goes through its logits batch by batch, with a
 // bound that follows the list.  Few rows are spread over clusters of up to
@@ -32,9 +32,18 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kBatch = 4;        // vectors of a thread in flight
+// Threads of a CTA, vectors of a thread in a batch, CTAs of an SM.  Many rows:
+// small CTAs, whose row ends (a chain of barriers) hide behind the others'
+// streams (2048 x 151936 FP16 with top 5: 145 us; 160 with the other shape).
+// Few rows: large ones, a row's chain being the time (4 rows, top 20: 15.2 us;
+// 17.4 with the other shape).
+struct ManyRows {
+  static constexpr int kThreads = 256, kBatch = 4, kResident = 3;
+};
+struct FewRows {
+  static constexpr int kThreads = 512, kBatch = 2, kResident = 2;
+};
+constexpr int kMaxThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;      // of threads, whose best logits give the first bound
 constexpr int kList = 2048;      // keys that the list holds
@@ -97,16 +106,39 @@ struct Stat {
 
 // A thread's sums over pairs of logits, beside the maximum m.
 struct PairSums {
+  float m = -INFINITY;
   uint64_t z = 0, w = 0;
-  __device__ __forceinline__ void add(float a, float b, uint64_t minus_m, uint64_t log2e) {
-    uint64_t d = f32_add2(f32_pair(a, b), minus_m);
-    float d0, d1, e0, e1;
-    f32_split(d, d0, d1);
-    d = f32_pair(fmaxf(d0, -200.f), fmaxf(d1, -200.f));  // -inf counts nothing
-    f32_split(f32_mul2(d, log2e), e0, e1);
+  __device__ __forceinline__ void raise(float top) {
+    if (!(top > m)) return;
+    const float d = m - top, f = m == -INFINITY ? 0.f : ex2a(d * kLog2e);
+    float z0, z1, w0, w1;
+    f32_split(z, z0, z1);
+    f32_split(w, w0, w1);
+    w = f == 0.f ? 0 : f32_pair(f * fmaf(d, z0, w0), f * fmaf(d, z1, w1));
+    z = f == 0.f ? 0 : f32_pair(f * z0, f * z1);
+    m = top;
+  }
+  // after raise: finite a, b
+  __device__ __forceinline__ void add(float a, float b, uint64_t minus_m) {
+    const uint64_t d = f32_add2(f32_pair(a, b), minus_m);
+    float e0, e1;
+    f32_split(f32_mul2(d, f32_pair(kLog2e, kLog2e)), e0, e1);
     const uint64_t e = f32_pair(ex2a(e0), ex2a(e1));
     z = f32_add2(z, e);
     w = f32_fma2(e, d, w);
+  }
+  // any a; -inf counts nothing
+  __device__ __forceinline__ void add(float a) {
+    const float d = fmaxf(a - m, -200.f);
+    const uint64_t e = f32_pair(ex2a(d * kLog2e), 0.f);
+    z = f32_add2(z, e);
+    w = f32_fma2(e, f32_pair(d, 0.f), w);
+  }
+  __device__ __forceinline__ Stat stat() const {
+    float z0, z1, w0, w1;
+    f32_split(z, z0, z1);
+    f32_split(w, w0, w1);
+    return Stat{m, z0 + z1, w0 + w1};
   }
 };
 
@@ -114,9 +146,9 @@ struct Shared {
   Key list[kList];
   Key kept[32];
   Key best[kGroups];
-  uint16_t who[kThreads];  // threads whose best logit reaches the bound
+  uint16_t who[kMaxThreads];  // threads whose best logit reaches the bound
   int interested;
-  Stat stat[kWarps];
+  Stat stat[kMaxThreads / 32];
   Key bound;  // keys below it are not among the row's top
   int count;       // listed keys
   int held;        // of them from earlier batches of a second passage
@@ -131,6 +163,7 @@ struct Result {
 
 // The `top` largest of the first n listed keys, in order, to s.kept.  Every
 // thread of the CTA comes here.
+template <int kThreads>
 __device__ void rank_list(Shared& s, int n, int top) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const Key k = s.list[i];
@@ -143,9 +176,10 @@ __device__ void rank_list(Shared& s, int n, int top) {
 }
 
 // The list becomes its `top` largest, in order.
+template <int kThreads>
 __device__ void prune(Shared& s, int top) {
   const int n = min(s.count, kList);
-  rank_list(s, n, top);
+  rank_list<kThreads>(s, n, top);
   const int left = min(n, top);
   if ((int)threadIdx.x < left) s.list[threadIdx.x] = s.kept[threadIdx.x];
   if (threadIdx.x == 0) {
@@ -167,6 +201,25 @@ struct Vec {
       return __half2float(__ushort_as_half((unsigned short)(word(i >> 1) >> (16 * (i & 1)))));
     else return __uint_as_float(i & 1 ? word(i >> 1) & 0xffff0000u : word(i >> 1) << 16);
   }
+  // The larger of each pair of logits; NaN if one is.
+  __device__ __forceinline__ Vec max(const Vec& o) const {
+    Vec r{v};
+    uint32_t* a = &r.v.x;
+    const uint32_t* b = &o.v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        float y = __uint_as_float(a[i]);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(__uint_as_float(b[i])));
+        a[i] = __float_as_uint(y);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a[i]) : "r"(b[i]));
+      } else {
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a[i]) : "r"(b[i]));
+      }
+    }
+    return r;
+  }
   // The largest; NaN if there is one.
   __device__ __forceinline__ float top() const {
     if constexpr (sizeof(T) == 4) {
@@ -187,13 +240,41 @@ struct Vec {
       return a;
     }
   }
+  static __device__ __forceinline__ Vec nothing() {  // -inf
+    constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return Vec{make_uint4(w, w, w, w)};
+  }
+  // A finite number (a word of one or two) that takes the place of logits
+  // below it, -inf above all: its e^(x - m) is 0, and x - m is finite.
+  // -2^20 for positive m, else the type's lowest; `low` says that m is too
+  // near to that.  NaN becomes it too.
+  static __device__ __forceinline__ uint32_t lowest(float m) {
+    if constexpr (sizeof(T) == 4) return m > 0.f ? 0xc9800000u : 0xff7fffffu;
+    else if constexpr (std::is_same<T, __half>::value) return 0xfbfffbffu;
+    else return m > 0.f ? 0xc980c980u : 0xff7fff7fu;
+  }
+  static __device__ __forceinline__ bool low(float m) {
+    constexpr float lo = std::is_same<T, __half>::value ? -65504.f : sizeof(T) == 4 ? -3.40282347e38f : -3.38953139e38f;
+    return !(m - lo > 200.f);
+  }
+  __device__ __forceinline__ Vec at_least(uint32_t lo) const {
+    Vec r{v};
+    uint32_t* a = &r.v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) a[i] = __float_as_uint(fmaxf(__uint_as_float(a[i]), __uint_as_float(lo)));
+      else if constexpr (std::is_same<T, __half>::value) asm("max.f16x2 %0, %0, %1;" : "+r"(a[i]) : "r"(lo));
+      else asm("max.bf16x2 %0, %0, %1;" : "+r"(a[i]) : "r"(lo));
+    }
+    return r;
+  }
 };
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(const ScoreParams p) {
+template <typename T, bool TOP, typename S>
+__global__ void __launch_bounds__(S::kThreads, S::kResident) token_logprobs_kernel(const ScoreParams p) {
   __shared__ Shared s;
   __shared__ Result mine;
-  constexpr int N = Vec<T>::kN;
+  constexpr int N = Vec<T>::kN, kThreads = S::kThreads, kWarps = kThreads / 32, kBatch = S::kBatch;
   pdl_launch_dependents();
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
@@ -231,7 +312,6 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
         if (at < kList) s.list[at] = k;
       }
     };
-    const uint64_t log2e = f32_pair(kLog2e, kLog2e);
     // this thread's logits of a batch whose vectors may hold listed ones
     auto scan = [&](int b0, auto&& use) {
 #pragma unroll 1
@@ -262,43 +342,61 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
       }
       __syncthreads();
     };
-    float best = -INFINITY;  // this thread's largest logit (a NaN counts as that), and its vector
+    float best = -INFINITY;  // this thread's largest logit (a NaN counts as that), and its batch's first vector
     int best_at = -1;
-#pragma unroll 1
-    for (int b0 = v0; b0 < v1; b0 += kThreads * kBatch) {
-      Vec<T> q[kBatch];
+    PairSums sums;
+    // a batch is loaded while the one before it is summed
+    auto load = [&](Vec<T> (&q)[kBatch], int b0) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int i = b0 + k * kThreads + tid;
+        q[k] = Vec<T>::nothing();
         if (i < v1) q[k].v = ldg_stream(xv + i);
       }
+    };
+    auto take = [&](const Vec<T> (&q)[kBatch], int b0) {
+      Vec<T> m = q[0];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = b0 + k * kThreads + tid;
-        if (i < v1) {
-          const float top = q[k].top();
-          raise(top);
-          if (st.m > -INFINITY) {
-            PairSums sums;
-            const uint64_t minus_m = f32_pair(-st.m, -st.m);
+      for (int k = 1; k < kBatch; ++k) m = m.max(q[k]);
+      const float top = m.top();
+      nan |= top != top;
+      sums.raise(top);
+      if (Vec<T>::low(sums.m)) {
 #pragma unroll
-            for (int e = 0; e < N; e += 2) sums.add(q[k].get(e), q[k].get(e + 1), minus_m, log2e);
-            float a, c;
-            f32_split(sums.z, a, c);
-            st.z += a + c;
-            f32_split(sums.w, a, c);
-            st.w += a + c;
-          }
-          if (TOP && (best_at < 0 || !(top <= best)) && best == best) {
-            best = top;
-            best_at = i;
-          }
+        for (int k = 0; k < kBatch; ++k) {
+#pragma unroll 1
+          for (int e = 0; e < N; ++e) sums.add(q[k].get(e));
+        }
+      } else {
+        const uint64_t minus_m = f32_pair(-sums.m, -sums.m);
+        const uint32_t lo = Vec<T>::lowest(sums.m);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const Vec<T> v = q[k].at_least(lo);
+#pragma unroll
+          for (int e = 0; e < N; e += 2) sums.add(v.get(e), v.get(e + 1), minus_m);
         }
       }
+      if (TOP && b0 + tid < v1 && (best_at < 0 || !(top <= best)) && best == best) {
+        best = top;
+        best_at = b0 + tid;
+      }
+    };
+    constexpr int kStep = kThreads * kBatch;
+    Vec<T> q0[kBatch], q1[kBatch];
+    load(q0, v0);
+#pragma unroll 1
+    for (int b0 = v0; b0 < v1; b0 += 2 * kStep) {
+      load(q1, b0 + kStep);
+      take(q0, b0);
+      if (b0 + kStep >= v1) break;
+      load(q0, b0 + 2 * kStep);
+      take(q1, b0 + kStep);
     }
+    st = sums.stat();
     if constexpr (TOP) {
-      // the bound from the last logits of the best vectors: none is above its vector's best
-      bound_from(best_at < 0 ? 0 : rank_key(best, head + best_at * N + N - 1));
+      // the bound from the last logits of the best batches: none is above its batch's best
+      bound_from(best_at < 0 ? 0 : rank_key(best, head + (best_at + kStep - kThreads) * N + N - 1));
       if (best_at >= 0 && rank_key(best, head + best_at * N) >= s.bound) s.who[atomicAdd(&s.interested, 1)] = tid;
       __syncthreads();
       const int per = (v1 - v0 + kThreads - 1) / kThreads, items = s.interested * per;
@@ -339,14 +437,14 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
             __syncthreads();
             if (s.count <= kList) break;
             // too many: the top-th of those listed is a higher bound; list again
-            rank_list(s, kList, p.top);
+            rank_list<kThreads>(s, kList, p.top);
             if (tid == 0) {
               s.bound = max(s.bound, s.kept[p.top - 1]);
               s.count = s.held;
             }
             __syncthreads();
           }
-          prune(s, p.top);
+          prune<kThreads>(s, p.top);
         }
       }
     }
@@ -370,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
     }
     if (lane == 0) s.stat[warp] = st;
     nan = __syncthreads_or(nan);
-    if (TOP) prune(s, p.top);
+    if (TOP) prune<kThreads>(s, p.top);
     if (warp == 0) {
       st = lane < kWarps ? s.stat[lane] : Stat{-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -409,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
           __syncthreads();
           if (tid == 0) s.count = parts * 32;
           __syncthreads();
-          prune(s, p.top);
+          prune<kThreads>(s, p.top);
         }
       }
       cluster.sync();  // the others' results have been read
@@ -438,6 +536,14 @@ __global__ void __launch_bounds__(kThreads, TOP ? 2 : 3) token_logprobs_kernel(c
   }
 }
 
+template <typename T, typename S>
+int launch(const ScoreParams& p, int parts, cudaStream_t stream) {
+  const int64_t rows = p.rows < (1 << 24) ? p.rows : (1 << 24);
+  return launch_clusters("token_logprobs_kernel", launch_overlap(), (unsigned)parts,
+                         p.top ? token_logprobs_kernel<T, true, S> : token_logprobs_kernel<T, false, S>,
+                         dim3((unsigned)(rows * parts)), dim3(S::kThreads), 0, stream, p);
+}
+
 template <typename T>
 int launch(const ScoreParams& p, cudaStream_t stream) {
   const int sms = device_sm_count(current_device());
@@ -446,15 +552,12 @@ int launch(const ScoreParams& p, cudaStream_t stream) {
     return PP_ERR_CUDA;
   }
   // few rows: as many CTAs to each (a power of two) as keep them all on SMs of
-  // their own, and a batch of vectors to every CTA at least
+  // their own, and 16 KB of logits to every CTA at least
   int parts = 1;
   while (parts < kMaxCluster && p.rows * parts * 2 <= sms &&
-         (int64_t)p.vocab * (int)sizeof(T) >= (int64_t)parts * 2 * kThreads * 16)
+         (int64_t)p.vocab * (int)sizeof(T) >= (int64_t)parts * 2 * (16 << 10))
     parts *= 2;
-  const int64_t rows = p.rows < (1 << 24) ? p.rows : (1 << 24);
-  return launch_clusters("token_logprobs_kernel", launch_overlap(), (unsigned)parts,
-                         p.top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
-                         dim3((unsigned)(rows * parts)), dim3(kThreads), 0, stream, p);
+  return p.rows * kMaxCluster <= sms ? launch<T, FewRows>(p, parts, stream) : launch<T, ManyRows>(p, parts, stream);
 }
 
 }  // namespace
