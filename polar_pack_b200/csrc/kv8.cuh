@@ -117,12 +117,11 @@ __device__ __forceinline__ uint2 kv8_codes8(uint4 x, float scale, float per_scal
   for (int i = 0; i < 4; ++i) {
     f[i] = __half22float2(u2h(kv8_word(x, i)));
     if (!finite) f[i] = make_float2(kv8_finite(f[i].x), kv8_finite(f[i].y));
-    const uint64_t q = f32_mul2(f32_pair(f[i].x, f[i].y), per), r = f32_add2(q, whole), n = f32_add2(r, minus);
-    float q0, q1, n0, n1;
-    f32_split(q, q0, q1);
+    const uint64_t q = f32_mul2(f32_pair(f[i].x, f[i].y), per), r = f32_add2(q, whole), n = f32_fma2(f32_add2(r, minus), f32_pair(-1.f, -1.f), q);
+    float n0, n1;
     f32_split(n, n0, n1);
     f32_split(r, y[2 * i], y[2 * i + 1]);
-    off = fmaxf(off, fmaxf(fabsf(q0 - n0), fabsf(q1 - n1)));
+    off = fmaxf(off, fmaxf(fabsf(n0), fabsf(n1)));
   }
   if (off > 0.49996f) {
 #pragma unroll

@@ -65,13 +65,13 @@ struct AppendParams {
 };
 
 // CTA (j, head, sequence and side) makes block pos / 64 + j of one head's keys
-// or values, each thread HD / 32 vectors of eight in registers: one pass,
+// or values, each thread sixteen dimensions of HD / 64 rows in registers: one pass,
 // rows read once, codes and tail written once.  The CTA of the first block
 // also writes the tail rows of the last one: it alone reads the tail's old
 // rows, so nothing overwrites them before they are read.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
-  constexpr int kVecs = kKvBlock * HD / 8 / kThreads;
+__global__ void __launch_bounds__(kThreads, 5) kv8_append_kernel(const AppendParams p) {
+  constexpr int kRow = HD / 16, kItems = kKvBlock * kRow / kThreads;  // threads of a row, rows of a thread
   __shared__ float red[kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
   if (pos < 0 || cnt == 0) return;
   bool ok = pos <= p.c.cap - cnt;
   Kv8Rope rope = w == 0 ? p.rope : Kv8Rope{};
-  const int r0 = rope.cos ? rope.pos[b] : 0;
-  if (rope.cos && (r0 < 0 || r0 > rope.len - cnt)) ok = false;
+  const int rot = rope.cos ? rope.pos[b] : 0;
+  if (rope.cos && (rot < 0 || rot > rope.len - cnt)) ok = false;
   if (!ok) {
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 5);
     return;
@@ -91,37 +91,47 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
   const int block = pos / kKvBlock + blockIdx.x;
   if (block > last) return;
   const Kv8Head<HD> to(p.c, w, b, h);
+  const int r0 = threadIdx.x / kRow, d0 = threadIdx.x % kRow * 16;
   const __half* x = pick(p.x, w) + b * pick(p.ldb, w) + h * pick(p.ldh, w);
   const int64_t ldt = pick(p.ldt, w);
-  auto row8 = [&](int t, int d0) { return kv8_load8(x + (int64_t)(t - pos) * ldt, d0, HD, rope, r0 + t - pos); };
-  uint4 v[kVecs];
+  auto row = [&](int t, uint4 (&v)[2]) {  // 16 dimensions of a new token
+    const __half* y = x + (int64_t)(t - pos) * ldt;
+    v[0] = kv8_load8(y, d0, HD, rope, rot + t - pos);
+    v[1] = kv8_load8(y, d0 + 8, HD, rope, rot + t - pos);
+  };
+  uint4 v[kItems][2];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    const int t = block * kKvBlock + r;
-    v[i] = make_uint4(0, 0, 0, 0);
-    if (t < pos)
-      v[i] = *reinterpret_cast<const uint4*>(to.tail + r * HD + d0);
-    else if (t < len)
-      v[i] = row8(t, d0);
+  for (int i = 0; i < kItems; ++i) {
+    const int r = r0 + i * (kThreads / kRow), t = block * kKvBlock + r;
+    v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
+    if (t < pos) {
+      const uint4* y = reinterpret_cast<const uint4*>(to.tail + r * HD + d0);
+      v[i][0] = y[0];
+      v[i][1] = y[1];
+    } else if (t < len) {
+      row(t, v[i]);
+    }
   }
   if ((block + 1) * kKvBlock <= len) {
-    const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
+    const Kv8Scale q = kv8_block_scale<2 * kItems, kThreads>(reinterpret_cast<const uint4(&)[2 * kItems]>(v), red);
+    uint8_t* out = to.codes + ((int64_t)(block * kKvBlock + r0) * HD + d0);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int e = i * kThreads + threadIdx.x;
-      *reinterpret_cast<uint2*>(to.codes + (int64_t)block * (kKvBlock * HD) + e * 8) = kv8_codes8(v[i], q);
+    for (int i = 0; i < kItems; ++i) {
+      const uint2 lo = kv8_codes8(v[i][0], q), hi = kv8_codes8(v[i][1], q);
+      *reinterpret_cast<uint4*>(out + i * (kThreads / kRow) * HD) = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
     if (threadIdx.x == 0) to.scales[block] = q.scale;
   }
   if (blockIdx.x != 0) return;
   __syncthreads();  // the tail's old rows have been read
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int e = i * kThreads + threadIdx.x, r = e / (HD / 8), d0 = e % (HD / 8) * 8;
-    const int t = last * kKvBlock + r;
-    if (t >= pos && t < len)
-      *reinterpret_cast<uint4*>(to.tail + r * HD + d0) = last == block ? v[i] : row8(t, d0);
+  for (int i = 0; i < kItems; ++i) {
+    const int r = r0 + i * (kThreads / kRow), t = last * kKvBlock + r;
+    if (t < pos || t >= len) continue;
+    if (last != block) row(t, v[i]);
+    uint4* y = reinterpret_cast<uint4*>(to.tail + r * HD + d0);
+    y[0] = v[i][0];
+    y[1] = v[i][1];
   }
 }
 
@@ -360,47 +370,69 @@ __global__ void __launch_bounds__(kSelThreads, 2) kv8_select_kernel(const EvictP
 // repeated evictions do not requantise what does not move apart.
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 6) kv8_gather_kernel(const EvictParams p) {
-  constexpr int kVecs = kKvBlock * HD / 8 / kThreads;
+  constexpr int kRow = HD / 16, kItems = kKvBlock * kRow / kThreads;  // threads of a row, rows of a thread
   __shared__ float red[kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int block = blockIdx.x, h = blockIdx.y, b = blockIdx.z >> 1, w = blockIdx.z & 1;
   // the positions (-1 past the new length) are read beside the lengths, not after them
   const int* kept = p.kept + p.c.head(b, h) * p.keep + block * kKvBlock;
-  const int room = p.keep - block * kKvBlock;
-  int src[kVecs];
+  const int room = p.keep - block * kKvBlock, r0 = threadIdx.x / kRow, d0 = threadIdx.x % kRow * 16;
+  int src[kItems];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int r = (i * kThreads + threadIdx.x) / (HD / 8);
+  for (int i = 0; i < kItems; ++i) {
+    const int r = r0 + i * (kThreads / kRow);
     src[i] = r < room ? kept[r] : -1;
   }
   const int f = kept[0], g = room >= kKvBlock ? kept[kKvBlock - 1] : -1;
-  const int len = p.lens[b], m = p.new_lens[b];
+  const int len = p.lens[b], m = p.new_lens[b], old_last = kv8_last_block(len);
   if (f < 0) return;
-  const bool full = g >= 0, last = block == kv8_last_block(m);
-  const bool whole = full && f % kKvBlock == 0 && g - f == kKvBlock - 1 && f / kKvBlock != kv8_last_block(len);
+  const bool full = g >= 0;
   const Kv8Head<HD> from(p.c, w, b, h), to(p.to, w, b, h);
-  const int old_last = kv8_last_block(len);
-  uint4 v[kVecs];
+  uint4 v[2 * kItems];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int d0 = (i * kThreads + threadIdx.x) % (HD / 8) * 8;
-    v[i] = src[i] >= 0 ? from.read8(src[i], old_last, d0) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kItems; ++i) {
+    v[2 * i] = v[2 * i + 1] = make_uint4(0, 0, 0, 0);
+    if (src[i] < 0) continue;
+    const int at = src[i] / kKvBlock;
+    if (at == old_last) {
+      const uint4* x = reinterpret_cast<const uint4*>(from.tail + src[i] % kKvBlock * HD + d0);
+      v[2 * i] = x[0];
+      v[2 * i + 1] = x[1];
+    } else {
+      const uint4 c = *reinterpret_cast<const uint4*>(from.codes + ((int64_t)src[i] * HD + d0));
+      const float scale = from.scales[at];
+      v[2 * i] = kv8_values8(make_uint2(c.x, c.y), scale);
+      v[2 * i + 1] = kv8_values8(make_uint2(c.z, c.w), scale);
+    }
   }
-  if (last) {
+  if (block == kv8_last_block(m)) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (src[i] >= 0) *reinterpret_cast<uint4*>(to.tail + (i * kThreads + threadIdx.x) * 8) = v[i];
+    for (int i = 0; i < kItems; ++i)
+      if (src[i] >= 0) {
+        uint4* x = reinterpret_cast<uint4*>(to.tail + (r0 + i * (kThreads / kRow)) * HD + d0);
+        x[0] = v[2 * i];
+        x[1] = v[2 * i + 1];
+      }
   }
   if (!full) return;
-  const Kv8Scale q = kv8_block_scale<kVecs, kThreads>(v, red);
-  uint8_t* out = to.codes + (int64_t)block * (kKvBlock * HD) + threadIdx.x * 8;
-  const uint8_t* same = from.codes + (int64_t)f * HD + threadIdx.x * 8;
+  uint8_t* out = to.codes + ((int64_t)(block * kKvBlock + r0) * HD + d0);
+  constexpr int kStep = kThreads / kRow * HD;
+  if (f % kKvBlock == 0 && g - f == kKvBlock - 1 && f / kKvBlock != old_last) {
+    const uint8_t* same = from.codes + ((int64_t)(f + r0) * HD + d0);
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i)
-    *reinterpret_cast<uint2*>(out + i * kThreads * 8) =
-        whole ? *reinterpret_cast<const uint2*>(same + i * kThreads * 8) : kv8_codes8(v[i], q);
-  if (threadIdx.x == 0) to.scales[block] = whole ? from.scales[f / kKvBlock] : q.scale;
+    for (int i = 0; i < kItems; ++i)
+      *reinterpret_cast<uint4*>(out + i * kStep) = *reinterpret_cast<const uint4*>(same + i * kStep);
+    if (threadIdx.x == 0) to.scales[block] = from.scales[f / kKvBlock];
+    return;
+  }
+  const Kv8Scale q = kv8_block_scale<2 * kItems, kThreads>(v, red);
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const uint2 lo = kv8_codes8(v[2 * i], q), hi = kv8_codes8(v[2 * i + 1], q);
+    *reinterpret_cast<uint4*>(out + i * kStep) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+  if (threadIdx.x == 0) to.scales[block] = q.scale;
 }
 
 bool g_select_attr[64];

@@ -235,7 +235,8 @@ def kv8_restore(cache: KV8Cache, lens: torch.Tensor, start: torch.Tensor | None 
     n = cache.capacity if count is None else int(count)
     if n < 0:
         raise ValueError("count must not be negative")
-    k, v = torch.empty(2, cache.batch, n, cache.kv_heads, cache.head_dim, dtype=torch.float16, device=cache.device)
+    k = torch.empty(cache.batch, n, cache.kv_heads, cache.head_dim, dtype=torch.float16, device=cache.device)
+    v = torch.empty_like(k)
     _call(cache, "pp_kv8_restore", _ints(lens, "lens", cache), _ints(start, "start", cache), n, k.data_ptr(),
           v.data_ptr())
     return k, v
