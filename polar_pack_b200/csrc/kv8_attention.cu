@@ -12,8 +12,7 @@ constexpr int kMaxGroup = 16;
 
 // How a call with `rows` query rows per kv head runs on kv8_decode_kernel:
 // tiles of 8 rows while one is enough, else of 16.
-constexpr int kDecodeRows = 64;
-constexpr int kDecodeBatch = 512;
+constexpr int kDecodeBatch = 512;  // sequences of a launch
 
 struct DecodePlan {
   int nt, tiles, ctas;
@@ -51,6 +50,30 @@ PromptPlan plan_prompt(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
   d.splits = s > 1 ? (int)s : 1;
   d.bytes = d.splits > 1 ? (size_t)d.splits * c.batch * c.nkv * rows * (c.hd + 2) * sizeof(float) : 0;
   return d;
+}
+
+// Whether kv8_decode_kernel takes a call: a single row tile always, more than
+// 256 rows never.  Between, the times that the two kernels would take at full
+// caches, in ns, as measured on 148 SMs (16 query heads on 2 kv heads of 128):
+// decode 12 us and one for 300 blocks of 16 rows, a segment counting eight
+// more; prompt 9 us, 1.45 for a CTA's block, 4 for joining parts.
+//   sequences, positions, rows   decode  prompt (us)
+//   1, 512, 256                  13.3    18.8
+//   4, 4096, 96                  19.4    24.7
+//   4, 4096, 128                 25.0    23.7
+//   32, 512, 32                  13.6    21.1
+//   32, 512, 64                  33.2    21.3
+//   32, 4096, 32                 32.3    60.1
+//   32, 4096, 64                 63.9    60.4
+bool decode_takes(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
+  const int64_t rows = n * (nq / c.nkv);
+  if (rows <= 16 || rows > 256) return rows <= 16;
+  const PromptPlan pr = plan_prompt(c, n, nq, ctas);
+  const int64_t heads = (int64_t)c.nkv * c.batch, blocks = c.cap / kKvBlock;
+  const int64_t decode = 12000 + heads * cdiv(rows, 16) * (blocks + 8) * 10 / 3;
+  const int64_t prompt = 9000 + 1450 * cdiv(blocks, pr.splits) * cdiv(heads * pr.tiles * pr.splits, ctas) +
+                         (pr.splits > 1 ? 4000 : 0);
+  return decode <= prompt;
 }
 
 bool g_attr[6][64];
@@ -202,9 +225,9 @@ int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64
     pp::set_error("pp_kv8_attention_workspace_bytes: no current CUDA device");
     return PP_ERR_CUDA;
   }
-  *bytes = n * (nq / c.nkv) <= pp::kDecodeRows ? pp::plan_decode(c, n, nq, weights != 0, ctas).bytes
-                                               : pp::align_up(ctas * sizeof(int), 256) +
-                                                     pp::plan_prompt(c, n, nq, ctas).bytes;
+  *bytes = pp::decode_takes(c, n, nq, ctas)
+               ? pp::plan_decode(c, n, nq, weights != 0, ctas).bytes
+               : pp::align_up(ctas * sizeof(int), 256) + pp::plan_prompt(c, n, nq, ctas).bytes;
   return PP_OK;
 }
 
@@ -220,7 +243,12 @@ int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_s
     return rc;
   if (empty) return PP_OK;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (n * (nq / p.c.nkv) <= pp::kDecodeRows) {
+  const int ctas = pp::device_sm_count(pp::current_device());
+  if (ctas < 1) {
+    pp::set_error("pp_kv8_attention: no current CUDA device");
+    return PP_ERR_CUDA;
+  }
+  if (pp::decode_takes(p.c, n, nq, ctas)) {
     p.q = reinterpret_cast<const __half*>(q);
     p.ldqb = q_strides[0];
     p.ldqt = q_strides[1];
@@ -236,11 +264,6 @@ int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_s
     p.scale2 = scale * 1.44269504088896341f;
     p.status = status;
     return pp::run_decode("pp_kv8_attention", p, nullptr, workspace, workspace_bytes, s);
-  }
-  const int ctas = pp::device_sm_count(pp::current_device());
-  if (ctas < 1) {
-    pp::set_error("pp_kv8_attention: no current CUDA device");
-    return PP_ERR_CUDA;
   }
   const pp::PromptPlan d = pp::plan_prompt(p.c, n, nq, ctas);
   const size_t counters = pp::align_up(ctas * sizeof(int), 256);  // of the other kernel's calls on this workspace

@@ -70,26 +70,6 @@ struct Kv8PromptSmem {
   static constexpr int kBytes = kBar + 256;
 };
 
-// Pairs of FP32 values, two operations an instruction.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // Row r of a call's n * group rows: query r / group, head r % group.
 __device__ __forceinline__ int kv8_row_stop(int i, int len, int cnt) { return i < cnt ? len - cnt + i + 1 : 0; }
 
@@ -275,7 +255,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         }
       }
       const float shift = (m == -INFINITY ? 0.f : -m) + kPrLift + log_f;
-      const uint64_t k2 = pack2(k, k), shift2 = pack2(shift, shift);
+      const uint64_t k2 = f32_pair(k, k), shift2 = f32_pair(shift, shift);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -289,16 +269,16 @@ __global__ void __launch_bounds__(kPrThreads, 1)
 #pragma unroll
         for (int u = 0; u < 32; u += 2) {
           float x, y;
-          unpack2(fma2(pack2(__uint_as_float(s[u]), __uint_as_float(s[u + 1])), k2, shift2), x, y);
+          f32_split(f32_fma2(f32_pair(__uint_as_float(s[u]), __uint_as_float(s[u + 1])), k2, shift2), x, y);
           x = ex2(x);
           y = ex2(y);
-          sum[u / 2 & 1] = add2(sum[u / 2 & 1], pack2(x, y));
+          sum[u / 2 & 1] = f32_add2(sum[u / 2 & 1], f32_pair(x, y));
           w[u / 2] = h2u(__floats2half2_rn(x, y));
         }
         tc_st16(s_cols + 16 * c, w);
       }
       float sx, sy;
-      unpack2(add2(sum[0], sum[1]), sx, sy);
+      f32_split(f32_add2(sum[0], sum[1]), sx, sy);
       l = fmaf(sx + sy, ex2(-log_f), l);
       tc_wait_st();
       tc_fence_before();
@@ -356,140 +336,141 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       reinterpret_cast<float2*>(p.part + (int64_t)p.splits * p.c.batch * p.c.nkv * rows * HD)
           [(((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r] = make_float2(empty ? -INFINITY : m, empty ? 0.f : l);
   } else {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-   if (warp < 16) {
-    // --------------------------------------------------------------- unpack
-    // warps 8-11 values, 12-15 keys; rows 32 (w & 1) + lane, sixteen-dimension
-    // chunks of parity w >> 1
-    const int w = warp & 3, side = warp < 12 ? 1 : 0;
-    const int r = (w & 1) * 32 + lane;
-    constexpr int kChunks = HD / 32;
-    const uint32_t full = side ? v_full : k_full, empty = side ? v_empty : k_empty;
-    const uint32_t src = base + S::kCodes + side * S::kCode, dst = base + (side ? S::kV : S::kK) + r * 128;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < 16) {
+      // --------------------------------------------------------------- unpack
+      // warps 8-11 values, 12-15 keys; rows 32 (w & 1) + lane, sixteen-dimension
+      // chunks of parity w >> 1
+      const int w = warp & 3, side = warp < 12 ? 1 : 0;
+      const int r = (w & 1) * 32 + lane;
+      constexpr int kChunks = HD / 32;
+      const uint32_t full = side ? v_full : k_full, empty = side ? v_empty : k_empty;
+      const uint32_t src = base + S::kCodes + side * S::kCode, dst = base + (side ? S::kV : S::kK) + r * 128;
 #pragma unroll 1
-    for (int j = 0; j < J; ++j) {
-      const int st = j % kPrCodeStages, buf = j & 1;
-      const bool is_tail = j0 + j >= coded;
-      uint4 lo[kChunks], hi[kChunks];
-      bool fine = true;
-      if (!is_tail) {
-        fine = wait(code_full + 8 * st, (j / kPrCodeStages) & 1);
-        uint4 x[kChunks];
+      for (int j = 0; j < J; ++j) {
+        const int st = j % kPrCodeStages, buf = j & 1;
+        const bool is_tail = j0 + j >= coded;
+        uint4 lo[kChunks], hi[kChunks];
+        bool fine = true;
+        if (!is_tail) {
+          fine = wait(code_full + 8 * st, (j / kPrCodeStages) & 1);
+          uint4 x[kChunks];
 #pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc)
-          x[cc] = lds128(src + 2 * st * S::kCode + tile_off<HD>(r, 2 * cc + (w >> 1)));
+          for (int cc = 0; cc < kChunks; ++cc)
+            x[cc] = lds128(src + 2 * st * S::kCode + tile_off<HD>(r, 2 * cc + (w >> 1)));
 #pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc) {
-          lo[cc] = make_uint4(codes2<0x4140>(x[cc].x), codes2<0x4342>(x[cc].x), codes2<0x4140>(x[cc].y),
-                              codes2<0x4342>(x[cc].y));
-          hi[cc] = make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w),
-                              codes2<0x4342>(x[cc].w));
-        }
-      } else {  // FP16 rows from memory, zero past the end
+          for (int cc = 0; cc < kChunks; ++cc) {
+            lo[cc] = make_uint4(codes2<0x4140>(x[cc].x), codes2<0x4342>(x[cc].x), codes2<0x4140>(x[cc].y),
+                                codes2<0x4342>(x[cc].y));
+            hi[cc] = make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w),
+                                codes2<0x4342>(x[cc].w));
+          }
+        } else {  // FP16 rows from memory, zero past the end
 #pragma unroll
-        for (int cc = 0; cc < kChunks; ++cc) {
-          lo[cc] = hi[cc] = make_uint4(0, 0, 0, 0);
-          if ((j0 + j) * kKvBlock + r < len) {
-            const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * (2 * cc + (w >> 1)));
-            lo[cc] = g[0];
-            hi[cc] = g[1];
+          for (int cc = 0; cc < kChunks; ++cc) {
+            lo[cc] = hi[cc] = make_uint4(0, 0, 0, 0);
+            if ((j0 + j) * kKvBlock + r < len) {
+              const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * (2 * cc + (w >> 1)));
+              lo[cc] = g[0];
+              hi[cc] = g[1];
+            }
           }
         }
-      }
-      if (j > 1) fine = fine && wait(empty + 8 * buf, ((j >> 1) - 1) & 1);
-      if (!fine) break;
+        if (j > 1) fine = fine && wait(empty + 8 * buf, ((j >> 1) - 1) & 1);
+        if (!fine) break;
 #pragma unroll
-      for (int cc = 0; cc < kChunks; ++cc) {
-        const int c = 2 * cc + (w >> 1), ch = 2 * (c & 3);
-        const uint32_t to = dst + buf * S::kKv + c / 4 * (kKvBlock * 128);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(lo[cc].x),
-                     "r"(lo[cc].y), "r"(lo[cc].z), "r"(lo[cc].w) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(hi[cc].x),
-                     "r"(hi[cc].y), "r"(hi[cc].z), "r"(hi[cc].w) : "memory");
+        for (int cc = 0; cc < kChunks; ++cc) {
+          const int c = 2 * cc + (w >> 1), ch = 2 * (c & 3);
+          const uint32_t to = dst + buf * S::kKv + c / 4 * (kKvBlock * 128);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + ((ch ^ (r & 7)) << 4)), "r"(lo[cc].x),
+                       "r"(lo[cc].y), "r"(lo[cc].z), "r"(lo[cc].w) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((ch + 1) ^ (r & 7)) << 4)), "r"(hi[cc].x),
+                       "r"(hi[cc].y), "r"(hi[cc].z), "r"(hi[cc].w) : "memory");
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(full + 8 * buf);
+          if (!is_tail) mbar_arrive(code_empty + 8 * st);
+        }
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(full + 8 * buf);
-        if (!is_tail) mbar_arrive(code_empty + 8 * st);
-      }
-    }
   } else if (warp == 16) {
-    // ------------------------------------------------------------- S = Q K^T
-    // Two blocks ahead of the second product, into the buffer whose weights it
-    // has read.  Descriptors' offsets within a tile add to their address field.
-    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
-    const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
-    bool fine = J == 0 || wait(q_full, 0);
+      // ------------------------------------------------------------- S = Q K^T
+      // Two blocks ahead of the second product, into the buffer whose weights it
+      // has read.  Descriptors' offsets within a tile add to their address field.
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kKvBlock >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+      const uint64_t q_desc = sw128_desc(base + S::kQ, 16, 1024), k_desc = sw128_desc(base + S::kK, 16, 1024);
+      bool fine = J == 0 || wait(q_full, 0);
 #pragma unroll 1
-    for (int j = 0; j < J && fine; ++j) {
-      const int buf = j & 1;
-      const uint64_t kd = k_desc + (uint32_t)(buf * (S::kKv >> 4));
-      fine = wait(k_full + 8 * buf, (j >> 1) & 1);
+      for (int j = 0; j < J && fine; ++j) {
+        const int buf = j & 1;
+        const uint64_t kd = k_desc + (uint32_t)(buf * (S::kKv >> 4));
+        fine = wait(k_full + 8 * buf, (j >> 1) & 1);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (j > 1) fine = fine && wait(o_full + 8 * (2 * t + buf), ((j >> 1) - 1) & 1);
-        if (!fine) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t qd = q_desc + (uint32_t)(t * (S::kQTile >> 4));
-          const uint32_t dst = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
+        for (int t = 0; t < 2; ++t) {
+          if (j > 1) fine = fine && wait(o_full + 8 * (2 * t + buf), ((j >> 1) - 1) & 1);
+          if (!fine) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t qd = q_desc + (uint32_t)(t * (S::kQTile >> 4));
+            const uint32_t dst = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
 #pragma unroll
-          for (int d = 0; d < HD / 16; ++d)
-            tc_mma(dst, qd + (d / 4 * (kPrTile * 128) + d % 4 * 32 >> 4), kd + (d / 4 * (kKvBlock * 128) + d % 4 * 32 >> 4),
-                   idesc, d > 0);
-          tc_commit(s_full + 8 * (2 * t + buf));
-          if (t == 1) tc_commit(k_empty + 8 * buf);
+            for (int d = 0; d < HD / 16; ++d)
+              tc_mma(dst, qd + (d / 4 * (kPrTile * 128) + d % 4 * 32 >> 4),
+                     kd + (d / 4 * (kKvBlock * 128) + d % 4 * 32 >> 4),
+                     idesc, d > 0);
+            tc_commit(s_full + 8 * (2 * t + buf));
+            if (t == 1) tc_commit(k_empty + 8 * buf);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    if (J > 0) wait(done, 0);  // no product outlives the tensor memory
+      if (J > 0) wait(done, 0);  // no product outlives the tensor memory
   } else if (warp == 18) {
-    // --------------------------------------------------------------- O += P V
-    constexpr uint32_t idesc =
-        (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
-    const uint64_t v_desc = sw128_desc(base + S::kV, kKvBlock * 128, 1024);
-    bool fine = true;
+      // --------------------------------------------------------------- O += P V
+      constexpr uint32_t idesc =
+          (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
+      const uint64_t v_desc = sw128_desc(base + S::kV, kKvBlock * 128, 1024);
+      bool fine = true;
 #pragma unroll 1
-    for (int j = 0; j < J && fine; ++j) {
-      const int buf = j & 1;
-      const uint64_t vd = v_desc + (uint32_t)(buf * (S::kKv >> 4));
-      fine = wait(v_full + 8 * buf, (j >> 1) & 1);
+      for (int j = 0; j < J && fine; ++j) {
+        const int buf = j & 1;
+        const uint64_t vd = v_desc + (uint32_t)(buf * (S::kKv >> 4));
+        fine = wait(v_full + 8 * buf, (j >> 1) & 1);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        fine = fine && wait(p_full + 8 * (2 * t + buf), (j >> 1) & 1);
-        if (!fine) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t pa = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
+        for (int t = 0; t < 2; ++t) {
+          fine = fine && wait(p_full + 8 * (2 * t + buf), (j >> 1) & 1);
+          if (!fine) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t pa = tmem + 256u + (uint32_t)((2 * t + buf) * kKvBlock);
 #pragma unroll
-          for (int x = 0; x < kKvBlock / 16; ++x)
-            tc_mma_ta(tmem + (uint32_t)(t * HD), pa + 8 * x, vd + (x * 2048 >> 4), idesc, j > 0 || x > 0);
-          tc_commit(o_full + 8 * (2 * t + buf));
-          if (t == 1) tc_commit(v_empty + 8 * buf);
+            for (int x = 0; x < kKvBlock / 16; ++x)
+              tc_mma_ta(tmem + (uint32_t)(t * HD), pa + 8 * x, vd + (x * 2048 >> 4), idesc, j > 0 || x > 0);
+            tc_commit(o_full + 8 * (2 * t + buf));
+            if (t == 1) tc_commit(v_empty + 8 * buf);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    if (elect_one()) tc_commit(done);
-    __syncwarp();
-    wait(done, 0);
+      if (elect_one()) tc_commit(done);
+      __syncwarp();
+      wait(done, 0);
   } else if (warp == 17 && lane == 0) {
-    // ------------------------------------------------------------ code boxes
-    const int n = min(j1, coded) - j0;
-    int issued = 0;
-    for (int j = 0; j < n; ++j, ++issued) {
-      const int st = j % kPrCodeStages;
-      if (j >= kPrCodeStages && !mbar_wait_bounded(code_empty + 8 * st, (j / kPrCodeStages - 1) & 1, p.status)) break;
-      const int y = (int)(p.c.head(b, kvh) * p.c.cap) + (j0 + j) * kKvBlock;
-      mbar_expect_tx(code_full + 8 * st, 2 * S::kCode);
-      tma_load_2d(base + S::kCodes + 2 * st * S::kCode, &tk, 0, y, code_full + 8 * st);
-      tma_load_2d(base + S::kCodes + (2 * st + 1) * S::kCode, &tv, 0, y, code_full + 8 * st);
+      // ------------------------------------------------------------ code boxes
+      const int n = min(j1, coded) - j0;
+      int issued = 0;
+      for (int j = 0; j < n; ++j, ++issued) {
+        const int st = j % kPrCodeStages;
+        if (j >= kPrCodeStages && !mbar_wait_bounded(code_empty + 8 * st, (j / kPrCodeStages - 1) & 1, p.status)) break;
+        const int y = (int)(p.c.head(b, kvh) * p.c.cap) + (j0 + j) * kKvBlock;
+        mbar_expect_tx(code_full + 8 * st, 2 * S::kCode);
+        tma_load_2d(base + S::kCodes + 2 * st * S::kCode, &tk, 0, y, code_full + 8 * st);
+        tma_load_2d(base + S::kCodes + (2 * st + 1) * S::kCode, &tv, 0, y, code_full + 8 * st);
+      }
+      for (int j = max(0, issued - kPrCodeStages); j < issued; ++j)  // none stays in flight
+        mbar_wait_bounded(code_full + 8 * (j % kPrCodeStages), (j / kPrCodeStages) & 1, p.status);
     }
-    for (int j = max(0, issued - kPrCodeStages); j < issued; ++j)  // none stays in flight
-      mbar_wait_bounded(code_full + 8 * (j % kPrCodeStages), (j / kPrCodeStages) & 1, p.status);
-   }
   }
   tc_fence_before();
   __syncthreads();

@@ -86,7 +86,8 @@ class KV8Cache:
         return torch.zeros(self.batch, self.kv_heads, self.capacity, dtype=torch.float32, device=self.device)
 
     def new_workspace(self, n: int, q_heads: int, weights: bool = False) -> torch.Tensor:
-        """Scratch for attention calls of at most these sizes on this cache's shape."""
+        """Scratch for attention calls of ``n`` query tokens and ``q_heads`` heads on this cache's
+        shape (other sizes may need more, and refuse it then)."""
         return torch.zeros(self.workspace_bytes(n, q_heads, weights), dtype=torch.uint8, device=self.device)
 
     def nbytes(self) -> int:

@@ -238,6 +238,22 @@ def test_prompt_over_long_cache(cuda, nq, nkv, hd, scale):
     assert int(cache.status) == 0
 
 
+@pytest.mark.parametrize("nq,nkv,hd,n", [(8, 1, 128, 3), (8, 1, 128, 17), (4, 2, 64, 100), (7, 1, 128, 36)])
+def test_small_and_large_capacity(cuda, nq, nkv, hd, n):
+    """17 to 256 rows per kv head: the capacity decides which kernel they run on; both are right."""
+    from polar_pack_b200.kv8 import kv8_attention
+    g = _gen(cuda, n)
+    lens, counts = [n + 70, n, 400, 5], [n, n, min(n, 9), min(n, 5)]
+    q = _rand(g, 4, n, nq, hd, spread=2.0)
+    for cap in (448, 16384):
+        cache, ref = _new(4, nkv, cap, hd, cuda), kr.RefKV(4, nkv, hd)
+        _fill(cache, ref, lens, _gen(cuda, 50))
+        out = kv8_attention(q, cache, _ints(lens, cuda), counts=_ints(counts, cuda))
+        want, _ = kr.attention(ref, q, counts)
+        _check_out(out, want, ref)
+        assert int(cache.status) == 0
+
+
 def test_prompt_rows_do_not_mix(cuda):
     """A query of NaN changes its own row only; value blocks of very different scale."""
     from polar_pack_b200.kv8 import kv8_append, kv8_attention
