@@ -19,6 +19,11 @@
 // of a lane's word as its k elements, values by transposed ldmatrix, whose
 // word holds two dimensions at two positions: both orders cost nothing, since
 // the queries and the outputs take the same permutation.
+//
+// Measured: 4 sequences of 1024, 16 query heads on 2 kv heads of 128: 11 us, a
+// chain of launch, lengths, boxes, products and join; 64 ragged sequences up
+// to 8190, 28 heads on 4, 244 MB: 64 us, 3.8 TB/s, bound by the warps' issue
+// slots (about 1200 instructions a block).
 #pragma once
 
 #include "kv8.cuh"

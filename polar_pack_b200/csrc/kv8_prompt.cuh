@@ -24,6 +24,13 @@
 // K and V tiles have the same layout, positions x dimensions in 128-byte
 // swizzled rows: K-major for the first product, MN-major for the second.
 // Every wait is bounded; tensor memory is released on every path.
+//
+// Measured: 4 prompts of 2048, 28 query heads on 4 kv heads of 128, causal: 182
+// us, 660 TFLOP/s of the pairs that count; 4 chunks of 509 after up to 3492, 16
+// heads on 2: 86 us.  A block takes 1.1 us of both tiles, where its products
+// need 0.68: the chain S -> softmax -> P -> O of a tile is longer than the other
+// tile's products (a copy without the exponentials, or without the unpacking,
+// was hardly faster).
 #pragma once
 
 #include "kv8.cuh"

@@ -153,3 +153,26 @@ def test_side_stream(cuda):
     s.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_equal_terms(cuda, dtype):
+    """Many equal logits below the maximum: their sum's roundings must not add up."""
+    x = torch.full((4, 150001), -0.3, device=cuda, dtype=dtype)
+    x[:, 1::512] = 0.25
+    x[1] *= 3
+    x[2, ::7] = -math.inf
+    _check(x, torch.tensor([0, 1, 5, 513], dtype=torch.int32, device=cuda), 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_lowest_beside_nothing(cuda, dtype):
+    """Rows of the type's lowest value and -inf, in any order, odd lengths and starts."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(11)
+    wide = torch.full((6, 20011), torch.finfo(dtype).min, device=cuda).to(dtype)
+    wide[torch.rand(wide.shape, generator=g, device=cuda) < 0.5] = -math.inf
+    wide[3:, 7000] = torch.tensor([1.0, 1e4, -5.0], device=cuda).to(dtype)
+    for x in (wide, wide[:, 3:10002]):
+        t = torch.tensor([int(torch.isfinite(r).nonzero()[0]) for r in x], dtype=torch.int32, device=cuda)
+        _check(x, t, 0)
