@@ -886,16 +886,34 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const Kv8WeightsParams
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.z, kvh = blockIdx.y, group = p.nq / p.nkv;
-  const int len = p.lens[b] + p.extra;
   const int t = blockIdx.x * 256 + threadIdx.x;
-  if (len > p.cap || t >= len) return;
-  if (p.rope.cos && (p.rope.pos[b] < 0 || p.rope.pos[b] >= p.rope.len)) return;
+  if (t >= p.cap) return;
+  // everything is read side by side, whatever the length turns out to be
   const float* s = p.scores + ((int64_t)b * p.nq + kvh * group) * p.cap + t;
   const float* l = p.lse + b * p.nq + kvh * group;
+  float* out = p.weights + ((int64_t)b * p.nkv + kvh) * p.cap + t;
+  constexpr int kChunk = 8;
+  float x[kChunk], y[kChunk];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int h = 0; h < kChunk; ++h) {
+      const bool in = h0 + h < group;
+      x[h] = in ? s[(int64_t)(h0 + h) * p.cap] : -INFINITY;
+      y[h] = in ? l[h0 + h] : 0.f;
+    }
+  };
+  load(0);
+  const float before = *out;
+  const int len = p.lens[b] + p.extra, rot = p.rope.cos ? p.rope.pos[b] : 0;
+  if (len > p.cap || t >= len || (p.rope.cos && (rot < 0 || rot >= p.rope.len))) return;
   float w = 0.f;
-#pragma unroll 4
-  for (int h = 0; h < group; ++h) w += ex2(s[(int64_t)h * p.cap] - l[h]);
-  p.weights[((int64_t)b * p.nkv + kvh) * p.cap + t] += w;
+  for (int h0 = 0;;) {
+#pragma unroll
+    for (int h = 0; h < kChunk; ++h) w += ex2(x[h] - y[h]);
+    if ((h0 += kChunk) >= group) break;
+    load(h0);
+  }
+  *out = before + w;
 }
 
 }  // namespace pp
