@@ -441,8 +441,8 @@ PP_API int pp_kv8_restore(const pp_kv8_cache* cache, const int* lens, const int*
  * (1: a copy never arrived).  FP32 scores, softmax and sums; the softmax
  * weights are rounded to FP16 for the value product.  Workspace:
  * pp_kv8_attention_workspace_bytes on the device that is current (weights: for
- * pp_kv8_decode with weights), 256-byte aligned, zero-filled once, shared only
- * with other calls of these two functions. */
+ * pp_kv8_decode with weights; another n may need more), 256-byte aligned,
+ * zero-filled once, shared only with other calls of these two functions. */
 PP_API int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64_t nq, int weights,
                                             size_t* bytes);
 

@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
           if (!is_tail) mbar_arrive(code_empty + 8 * st);
         }
       }
-  } else if (warp == 16) {
+    } else if (warp == 16) {
       // ------------------------------------------------------------- S = Q K^T
       // Two blocks ahead of the second product, into the buffer whose weights it
       // has read.  Descriptors' offsets within a tile add to their address field.
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
         }
       }
       if (J > 0) wait(done, 0);  // no product outlives the tensor memory
-  } else if (warp == 18) {
+    } else if (warp == 18) {
       // --------------------------------------------------------------- O += P V
       constexpr uint32_t idesc =
           (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPrTile >> 4) << 24);
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       if (elect_one()) tc_commit(done);
       __syncwarp();
       wait(done, 0);
-  } else if (warp == 17 && lane == 0) {
+    } else if (warp == 17 && lane == 0) {
       // ------------------------------------------------------------ code boxes
       const int n = min(j1, coded) - j0;
       int issued = 0;
