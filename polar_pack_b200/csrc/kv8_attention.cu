@@ -33,22 +33,27 @@ DecodePlan plan_decode(const Kv8Cache& c, int64_t n, int64_t nq, bool weights, i
 }
 
 // More rows go to kv8_prompt_kernel.  With few tiles for the SMs, a tile's
-// positions are split into parts of at least eight blocks (by the capacity: the
-// lengths are on the device).
+// positions may be split into parts of at least eight blocks: as many of them
+// here as the lengths, which are on the device, can make use of
+// (kv8_part_blocks).
 struct PromptPlan {
+  int64_t base;  // tiles of all heads
   int tiles, splits;
-  size_t bytes;
+  size_t join, part, bytes;  // of the workspace, after the other kernel's counters
 };
 
 PromptPlan plan_prompt(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
   PromptPlan d{};
   const int64_t rows = n * (nq / c.nkv);
   d.tiles = (int)cdiv(rows, kPrRows);
-  const int64_t base = (int64_t)d.tiles * c.nkv * c.batch;
-  int64_t s = ctas / base;
+  d.base = (int64_t)d.tiles * c.nkv * c.batch;
+  int64_t s = c.batch <= kPrSplitBatch ? 2 * ctas / d.base : 1;
   if (s > c.cap / kKvBlock / 8) s = c.cap / kKvBlock / 8;
+  if (s > kPrMaxSplits) s = kPrMaxSplits;
   d.splits = s > 1 ? (int)s : 1;
-  d.bytes = d.splits > 1 ? (size_t)d.splits * c.batch * c.nkv * rows * (c.hd + 2) * sizeof(float) : 0;
+  d.join = align_up((size_t)ctas * sizeof(int), 256);
+  d.part = d.join + 256;
+  d.bytes = d.splits > 1 ? d.part + (size_t)d.splits * c.batch * c.nkv * rows * (c.hd + 2) * sizeof(float) : 0;
   return d;
 }
 
@@ -71,9 +76,9 @@ bool decode_takes(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
   const PromptPlan pr = plan_prompt(c, n, nq, ctas);
   const int64_t heads = (int64_t)c.nkv * c.batch, blocks = c.cap / kKvBlock;
   const int64_t decode = 12000 + heads * cdiv(rows, 16) * (blocks + 8) * 10 / 3;
-  const int64_t prompt = 9000 + 1450 * cdiv(blocks, pr.splits) * cdiv(heads * pr.tiles * pr.splits, ctas) +
-                         (pr.splits > 1 ? 4000 : 0);
-  return decode <= prompt;
+  for (int64_t k = 1; k <= pr.splits; ++k)  // parts of a tile's positions
+    if (decode > 9000 + 1450 * cdiv(blocks, k) * cdiv(pr.base * k, ctas) + (k > 1 ? 4000 : 0)) return false;
+  return true;
 }
 
 bool g_attr[6][64];
@@ -124,7 +129,8 @@ int launch_prompt(const Kv8PromptParams& p, cudaStream_t s) {
                              p, tm[0], tm[1]))
     return rc;
   if (p.splits == 1) return PP_OK;
-  const Kv8JoinParams j{p.part, p.out, p.ldob, p.ldot, p.ldoh, p.c.batch, p.c.nkv, p.n, p.nq, p.splits};
+  const Kv8JoinParams j{p.part, p.out, p.ldob, p.ldot, p.ldoh, p.lens, p.part_blocks, p.c.batch, p.c.nkv, p.n, p.nq,
+                        p.splits, p.c.cap};
   const int64_t rows = (int64_t)p.c.batch * p.c.nkv * p.n * (p.nq / p.c.nkv);
   // started early whatever the overlap setting: it waits for the attention itself
   return launch_kernel("kv8_join_kernel", true, kv8_join_kernel<HD>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, s, j);
@@ -227,7 +233,7 @@ int pp_kv8_attention_workspace_bytes(const pp_kv8_cache* cache, int64_t n, int64
   }
   *bytes = pp::decode_takes(c, n, nq, ctas)
                ? pp::plan_decode(c, n, nq, weights != 0, ctas).bytes
-               : pp::align_up(ctas * sizeof(int), 256) + pp::plan_prompt(c, n, nq, ctas).bytes;
+               : pp::plan_prompt(c, n, nq, ctas).bytes;
   return PP_OK;
 }
 
@@ -266,9 +272,8 @@ int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_s
     return pp::run_decode("pp_kv8_attention", p, nullptr, workspace, workspace_bytes, s);
   }
   const pp::PromptPlan d = pp::plan_prompt(p.c, n, nq, ctas);
-  const size_t counters = pp::align_up(ctas * sizeof(int), 256);  // of the other kernel's calls on this workspace
-  if (d.bytes && (!workspace || workspace_bytes < counters + d.bytes || !pp::aligned(workspace, 256))) {
-    pp::set_error("pp_kv8_attention: workspace of %zu bytes (256-byte aligned) required", counters + d.bytes);
+  if (d.bytes && (!workspace || workspace_bytes < d.bytes || !pp::aligned(workspace, 256))) {
+    pp::set_error("pp_kv8_attention: workspace of %zu bytes (256-byte aligned) required", d.bytes);
     return PP_ERR_WORKSPACE;
   }
   pp::Kv8PromptParams a{};
@@ -290,7 +295,11 @@ int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int64_t q_s
   a.rope = p.rope;
   a.tiles = d.tiles;
   a.splits = d.splits;
-  a.part = d.bytes ? reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + counters) : nullptr;
+  a.ctas = ctas;
+  if (d.bytes) {
+    a.part_blocks = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + d.join);
+    a.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + d.part);
+  }
   a.status = status;
   return p.c.hd == 128 ? pp::launch_prompt<128>(a, s) : pp::launch_prompt<64>(a, s);
 }

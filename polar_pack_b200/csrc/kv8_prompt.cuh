@@ -26,11 +26,14 @@
 // Every wait is bounded; tensor memory is released on every path.
 //
 // Measured: 4 prompts of 2048, 28 query heads on 4 kv heads of 128, causal: 182
-// us, 660 TFLOP/s of the pairs that count; 4 chunks of 509 after up to 3492, 16
-// heads on 2: 86 us.  A block takes 1.1 us of both tiles, where its products
-// need 0.68: the chain S -> softmax -> P -> O of a tile is longer than the other
-// tile's products (a copy without the exponentials, or without the unpacking,
-// was hardly faster).
+// us, 660 TFLOP/s of the pairs that count; ragged chunks of 509 of 0, 2040, 2332
+// and 4001, 16 heads on 2: 69 us (86 with the longest in one part).  A block
+// takes 1.1 us of both tiles, where its products need 0.68.  Copies that left
+// work out: without the unpacking, the exponentials or all but one step of
+// either product hardly faster, without products and softmax together 0.65 us;
+// so a block is bound by the softmax warps' own chain, one row to a thread, two
+// such warps to a scheduler.  A single pass over the scores with the maximum so far,
+// repeated where it grows, took 188 us.
 #pragma once
 
 #include "kv8.cuh"
@@ -58,8 +61,10 @@ struct Kv8PromptParams {
   float scale2;       // |scale| * log2(e)
   uint32_t q_sign;    // 0x80008000 for a negative scale
   Kv8Rope rope;
-  int tiles, splits;  // row tiles per (sequence, kv head); parts of each tile's positions
+  int tiles, splits;  // row tiles per (sequence, kv head); parts of a tile's positions, at most
+  int ctas;           // that run at a time
   float* part;        // splits > 1: [splits][batch][kv head][rows][hd] sums, then the same rows' (maximum, sum)
+  int* part_blocks;   // splits > 1: blocks of a part, for the join
   int* status;
 };
 
@@ -77,6 +82,59 @@ struct Kv8PromptSmem {
   static constexpr int kBytes = kBar + 256;
 };
 
+// Blocks of a sequence of the call, and into how many parts they are split (a
+// sequence without queries may be longer than all that count: at most `most`).
+__device__ __forceinline__ int kv8_seq_blocks(int len, int cap) {
+  return len > 0 && len <= cap ? (len + kKvBlock - 1) / kKvBlock : 0;
+}
+__device__ __forceinline__ int kv8_seq_parts(int blocks, int part_blocks, int most) {
+  return min(most, max(1, (blocks + part_blocks - 1) / part_blocks));
+}
+
+// Blocks of a part (splits > 1), from the lengths: of 512 sizes up to the
+// longest sequence's the one with which all tiles' parts, run `ctas` at a time,
+// take the least time.  A CTA's start and end cost as much as 14 blocks (15 us),
+// the join's start 4 and each of its parts 1/20 (its sums in FP32, written and
+// read).
+constexpr int kPrSplitBatch = 256;  // sequences of a call that may be split
+constexpr int kPrMaxSplits = 256;
+
+__device__ __forceinline__ int kv8_part_blocks(const Kv8PromptParams& p) {
+  __shared__ int s_blocks[kPrSplitBatch], s_tiles[kPrSplitBatch], s_max;
+  __shared__ unsigned s_best;
+  const int tid = threadIdx.x, group = p.nq / p.c.nkv;
+  if (tid == 0) {
+    s_max = 1;
+    s_best = ~0u;
+  }
+  __syncthreads();
+  if (tid < p.c.batch) {
+    const int cnt = p.counts ? min(max(p.counts[tid], 0), p.n) : p.n;
+    const int blocks = kv8_seq_blocks(p.lens[tid], p.c.cap);
+    s_blocks[tid] = blocks;
+    s_tiles[tid] = (cnt * group + kPrRows - 1) / kPrRows;
+    if (cnt > 0) atomicMax(&s_max, blocks);
+  }
+  __syncthreads();
+  constexpr int kSizes = 512;
+  auto size = [&](int i) { return (int)(((int64_t)s_max * (kSizes - i) + kSizes - 1) / kSizes); };
+  if (tid < kSizes) {
+    int n = 0, joined = 0;
+    for (int b = 0; b < p.c.batch; ++b) {
+      const int parts = kv8_seq_parts(s_blocks[b], size(tid), 0x7fffffff);
+      n += s_tiles[b] * parts;
+      if (parts > 1) joined += s_tiles[b] * parts;
+    }
+    const int64_t rounds = (n * p.c.nkv + p.ctas - 1) / p.ctas;
+    const int64_t time = rounds * (14 + size(tid)) * 20 + (joined ? 80 + joined * p.c.nkv : 0);
+    const bool fits = size(tid) * (int64_t)p.splits >= s_max;
+    const unsigned best = __reduce_min_sync(0xffffffffu, fits ? (unsigned)min(time, (int64_t)0x3fffff) << 9 | tid : ~0u);
+    if ((tid & 31) == 0) atomicMin(&s_best, best);
+  }
+  __syncthreads();
+  return size((int)(s_best & 511));
+}
+
 // Row r of a call's n * group rows: query r / group, head r % group.
 __device__ __forceinline__ int kv8_row_stop(int i, int len, int cnt) { return i < cnt ? len - cnt + i + 1 : 0; }
 
@@ -90,8 +148,17 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
   // long tiles first, of all heads: the last rows attend the most positions
-  const int tile = p.tiles - 1 - blockIdx.y / p.splits, split = blockIdx.y % p.splits;
+  const int tile = p.tiles - 1 - blockIdx.y % p.tiles, split = blockIdx.y / p.tiles;
   const int kvh = blockIdx.x % p.c.nkv, b = blockIdx.x / p.c.nkv;
+  int splits = 1;  // parts of this sequence's tiles; the CTAs past them have no work
+  if (p.splits > 1) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int size = kv8_part_blocks(p);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.part_blocks = size;
+    splits = kv8_seq_parts(kv8_seq_blocks(p.lens[b], p.c.cap), size, p.splits);
+    if (split >= splits) return;
+  }
   const int group = p.nq / p.c.nkv, rows = p.n * group, row0 = tile * kPrRows;
   // barriers
   const uint32_t bar = base + S::kBar;
@@ -142,7 +209,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const int i_first = row0 / group, i_last = min((min(row0 + kPrRows, rows) - 1) / group, cnt - 1);
   const int max_stop = i_last >= i_first ? max(0, kv8_row_stop(i_last, len, cnt)) : 0;
   const int blocks = len > 0 ? (max_stop + kKvBlock - 1) / kKvBlock : 0;
-  const int j0 = (int)((int64_t)blocks * split / p.splits), j1 = (int)((int64_t)blocks * (split + 1) / p.splits);
+  const int j0 = (int)((int64_t)blocks * split / splits), j1 = (int)((int64_t)blocks * (split + 1) / splits);
   const int J = j1 - j0;
   const int coded = kv8_last_block(len);  // the block after them is the tail
   const float *k_scale = p.c.scale(0, b, kvh, 0), *v_scale = p.c.scale(1, b, kvh, 0);
@@ -298,7 +365,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     const float inv = empty || l == 0.f ? 0.f : vref / l;
     // The results leave by way of shared memory, which nothing else uses any
     // more, so that a row's bytes go out side by side (a thread has a whole row).
-    const bool parts = p.splits > 1;
+    const bool parts = splits > 1;
     char* mine = reinterpret_cast<char*>(pp_smem) + warp * (32 * HD * 4);  // this warp's 32 rows
     char* to = nullptr;  // where row `lane` goes
     if (r < rows)
@@ -492,7 +559,9 @@ struct Kv8JoinParams {
   const float* part;
   __half* out;
   int64_t ldob, ldot, ldoh;
-  int batch, nkv, n, nq, splits;
+  const int* lens;
+  const int* part_blocks;
+  int batch, nkv, n, nq, splits, cap;
 };
 
 template <int HD>
@@ -504,19 +573,21 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8JoinParams p) {
   const int64_t at = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
   if (at >= all) return;
   const int lane = threadIdx.x & 31, r = (int)(at % rows), kvh = (int)(at / rows % p.nkv), b = (int)(at / rows / p.nkv);
+  const int splits = kv8_seq_parts(kv8_seq_blocks(p.lens[b], p.cap), *p.part_blocks, p.splits);
+  if (splits == 1) return;  // written by its only part
   constexpr int kPer = HD / 32;
   const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.splits * all * HD);
   float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 4) {  // four parts' loads at a time
+  for (int s0 = 0; s0 < splits; s0 += 4) {  // four parts' loads at a time
     float2 v[4], x[4][kPer / 2];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       v[s] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int e = 0; e < kPer / 2; ++e) x[s][e] = make_float2(0.f, 0.f);
-      if (s0 + s < p.splits) {
+      if (s0 + s < splits) {
         v[s] = ml[(s0 + s) * all + at];
 #pragma unroll
         for (int e = 0; e < kPer / 2; ++e)

@@ -124,7 +124,8 @@ def _workspace(cache: KV8Cache, n: int, q_heads: int, weights: bool, given) -> t
                              f"bytes on {cache.device}")
         return given.data_ptr(), given.numel(), given
     if torch.cuda.is_current_stream_capturing():
-        new = torch.zeros(nbytes, dtype=torch.uint8, device=cache.device)
+        new = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
+        new[:4096].zero_()  # the counters
         return new.data_ptr(), nbytes, new
     key = (cache.index, _lib.stream_handle(cache.device))
     buf = _scratch.get(key)

@@ -238,6 +238,35 @@ def test_prompt_over_long_cache(cuda, nq, nkv, hd, scale):
     assert int(cache.status) == 0
 
 
+@pytest.mark.parametrize("nq,nkv,hd,n,lens,counts", [
+    (4, 1, 128, 300, [6000, 300, 2500, 0], [300, 299, 10, 0]),      # split by the longest
+    (16, 2, 64, 70, [3000, 9000], [70, 70]),
+    (10, 2, 128, 60, [1, 60, 8100], [1, 60, 60]),
+    (2, 2, 64, 257, [9001, 9000, 8999], [257, 256, 0]),
+    (8, 1, 128, 90, [30000, 700, 2000], [0, 90, 90]),              # the longest has no queries
+])
+def test_split_positions(cuda, nq, nkv, hd, n, lens, counts):
+    """Chunks of prompts over long caches, whose positions are split where that pays."""
+    from polar_pack_b200.kv8 import kv8_attention
+    g = _gen(cuda, n)
+    B = len(lens)
+    cap = -(-max(lens) // 64) * 64 + 64
+    cache, ref = _new(B, nkv, cap, hd, cuda), kr.RefKV(B, nkv, hd)
+    _fill(cache, ref, lens, g)
+    q = _rand(g, B, n, nq, hd, spread=2.0)
+    out = kv8_attention(q, cache, _ints(lens, cuda), counts=_ints(counts, cuda))
+    want, _ = kr.attention(ref, q, counts)
+    _check_out(out, want, ref)
+    again = kv8_attention(q, cache, _ints(lens, cuda), counts=_ints(counts, cuda))
+    assert torch.equal(out, again) and int(cache.status) == 0
+    # lengths past the capacity: refused on the device, the others as before
+    bad = list(lens)
+    bad[0] = cap + 1
+    out = kv8_attention(q, cache, _ints(bad, cuda), counts=_ints(counts, cuda))
+    _check_out(out[1:], want[1:], ref)
+    assert not out[0].any() and int(cache.status) == 5
+
+
 @pytest.mark.parametrize("nq,nkv,hd,n", [(8, 1, 128, 3), (8, 1, 128, 17), (4, 2, 64, 100), (7, 1, 128, 36)])
 def test_small_and_large_capacity(cuda, nq, nkv, hd, n):
     """17 to 256 rows per kv head: the capacity decides which kernel they run on; both are right."""
