@@ -46,6 +46,19 @@ struct ManyRows {
 struct FewRows {
   static constexpr int kThreads = 512, kBatch = 2, kResident = 2;
 };
+// Short rows: two warps, ten rows to an SM.  Which rows count as short
+// (short_rows) by measurement of both (us, 256 threads against 64):
+//   FP16 1001 x 31968, top 0 / 5 / 32    443 -> 96, 694 -> 211, 5113 -> 235
+//   FP16 4001 x 7998                     75 -> 31, 142 -> 61, 159 -> 130
+//   FP16 16001 x 1999                    26 -> 18, 45 -> 34, 61 -> 126
+//   FP16 1001 x 200                      8.2 -> 5.3, 11 -> 8.2, 77 -> 10.5
+//   FP16 4001 x 200                      6.1 -> 5.4, 9.5 -> 8.8, 10 -> 21
+struct ShortRows {
+  static constexpr int kThreads = 64, kBatch = 4, kResident = 10;
+};
+constexpr bool short_rows(int64_t rows, int64_t row_bytes, int top, int sms) {
+  return row_bytes <= (rows < 8 * sms ? 4 << 10 : top > 8 ? 8 << 10 : 32 << 10);
+}
 constexpr int kMaxThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 64;      // of threads, whose best logits give the first bound
@@ -563,6 +576,7 @@ int launch(const ScoreParams& p, cudaStream_t stream) {
   while (parts < kMaxCluster && p.rows * parts * 2 <= sms &&
          (int64_t)p.vocab * (int)sizeof(T) >= (int64_t)parts * 2 * (16 << 10))
     parts *= 2;
+  if (short_rows(p.rows, (int64_t)p.vocab * (int)sizeof(T), p.top, sms)) return launch<T, ShortRows>(p, 1, stream);
   return p.rows * kMaxCluster <= sms ? launch<T, FewRows>(p, parts, stream) : launch<T, ManyRows>(p, parts, stream);
 }
 

@@ -176,3 +176,17 @@ def test_lowest_beside_nothing(cuda, dtype):
     for x in (wide, wide[:, 3:10002]):
         t = torch.tensor([int(torch.isfinite(r).nonzero()[0]) for r in x], dtype=torch.int32, device=cuda)
         _check(x, t, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,top", [(1300, 1001, 32), (1300, 4001, 5), (1300, 9000, 32), (40, 300, 32),
+                                            (3, 2047, 32), (1200, 31, 31), (2000, 1, 1), (1250, 16383, 8)])
+def test_short_rows(cuda, dtype, rows, vocab, top):
+    """Rows of a few KB, of which a CTA of two warps takes one; ties and rows of nothing among them."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(rows * 7 + vocab)
+    x = (torch.randn(rows, vocab, generator=g, device=cuda) * 3).to(dtype)
+    x[1::3] = (x[1::3] * 2).round() / 2
+    x[2] = torch.finfo(dtype).min if dtype == torch.float16 else -1.0
+    t = torch.randint(0, vocab, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    _check(x, t, top)
