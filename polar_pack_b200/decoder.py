@@ -518,6 +518,7 @@ class QuadDecoder:
         pos0 = self.pos.clone()
         kept = [] if self.kv8 is None else [(x, x.clone()) for x in (self.held, self.rot, *self.kv8_weights)
                                             if x is not None]
+        stream.wait_stream(torch.cuda.current_stream(self.device))   # steps still queued there, and the copies above
         with torch.cuda.stream(stream):
             self._run(stream.cuda_stream)       # warm-up outside the graph (argument caches)
             self._advance()

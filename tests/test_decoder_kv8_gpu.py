@@ -150,3 +150,27 @@ def test_refusals(cuda, parts):
         dec.step(t)
     with pytest.raises(ValueError):
         dec.capture(torch.cuda.Stream(cuda))
+
+
+def test_capture_behind_queued_steps(cuda, parts):
+    """A capture directly behind steps that the GPU has not reached yet."""
+    cfg = parts[0]
+    a, b = (_decoder(parts, kv_budget=90, kv_slack=40, kv_recent=16, kv_sinks=3) for _ in "ab")
+    toks = _tokens(cfg, 30, 10)
+    for t in toks[:20]:
+        a.step(t)
+    weights = [w.clone() for w in a.kv8_weights]
+    x = torch.randn(8192, 8192, device=cuda)
+    s = torch.cuda.Stream(cuda)
+    torch.cuda.synchronize()
+    for _ in range(10):                      # some 100 ms
+        x = torch.mm(x, x) * 1e-4
+    for t in toks[:20]:
+        b.step(t)
+    b.capture(s)
+    assert b.held.tolist() == [20] * 4 and b.rot.tolist() == [20] * 4 and b.pos.item() == 20
+    for u, w in zip(weights, b.kv8_weights):
+        assert torch.equal(u, w)
+    for t in toks[20:]:
+        assert torch.equal(a.step(t), b.step(t))
+    assert int(b.status.item()) == 0

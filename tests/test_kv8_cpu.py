@@ -65,3 +65,33 @@ def test_arguments(lib):
                                    None) == lib.PP_ERR_INVALID
     assert L.pp_token_logprobs(257, 0, 100, 1, 100, 256, 0, 256, 256, 256, 256, None, None) == lib.PP_ERR_INVALID
     assert L.pp_token_logprobs(256, 0, 100, 0, 100, 256, 0, 256, 256, 256, 256, None, None) == 0
+
+
+def test_capture_waits_for_the_current_stream(monkeypatch):
+    """The step that a capture warms up with runs behind the work that the
+    current stream holds: it shares the decoder's buffers and position."""
+    import contextlib
+
+    import torch
+    from polar_pack_b200.decoder import QuadDecoder
+    log = []
+
+    class Stream:
+        cuda_stream = 0
+
+        def wait_stream(self, other):
+            log.append(("wait", other))
+
+        def synchronize(self):
+            log.append("synchronize")
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: "current")
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "graph", lambda g, stream=None, **kw: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", object)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    dec = QuadDecoder.__new__(QuadDecoder)
+    dec.kv8, dec.device, dec.pos = None, torch.device("cpu"), torch.zeros(1, dtype=torch.int32)
+    dec._run = lambda s: log.append("run")
+    dec.capture(Stream())
+    assert log[:3] == [("wait", "current"), "run", "synchronize"] and int(dec.pos) == 0
