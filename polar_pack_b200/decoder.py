@@ -516,8 +516,12 @@ class QuadDecoder:
         if self.kv8 is not None and self.n_held == self.kv_room:
             raise ValueError("the caches are full: take a step or evict before a capture")
         pos0 = self.pos.clone()
-        kept = [] if self.kv8 is None else [(x, x.clone()) for x in (self.held, self.rot, *self.kv8_weights)
-                                            if x is not None]
+        kept = []
+        if self.kv8 is not None:
+            # where the caches hold whole blocks, the warm-up's token takes the
+            # place of the last block's first row, which is still read from there
+            tails = [t for c in self.kv8 for t in (c.k_tail, c.v_tail)]
+            kept = [(x, x.clone()) for x in (self.held, self.rot, *self.kv8_weights, *tails) if x is not None]
         stream.wait_stream(torch.cuda.current_stream(self.device))   # steps still queued there, and the copies above
         with torch.cuda.stream(stream):
             self._run(stream.cuda_stream)       # warm-up outside the graph (argument caches)

@@ -174,3 +174,26 @@ def test_capture_behind_queued_steps(cuda, parts):
     for t in toks[20:]:
         assert torch.equal(a.step(t), b.step(t))
     assert int(b.status.item()) == 0
+
+
+@pytest.mark.parametrize("held", [64, 128])
+def test_capture_at_a_blocks_end(cuda, parts, held):
+    """A capture leaves the rows of the last block, also where the step it
+    warms up with would open the next one."""
+    from polar_pack_b200.kv8 import kv8_restore
+    cfg = parts[0]
+    a, b = (_decoder(parts, kv_budget=40, kv_slack=150, kv_recent=8, kv_sinks=2) for _ in "ab")
+    toks = _tokens(cfg, held + 10, 9)
+    for t in toks[:held]:
+        a.step(t)
+        b.step(t)
+    torch.cuda.synchronize()
+    b.capture(torch.cuda.Stream(cuda))
+    for x, y in zip(a.kv8, b.kv8):
+        for u, w in zip(kv8_restore(x, a.held, count=held), kv8_restore(y, b.held, count=held)):
+            assert torch.equal(u, w)
+    a.evict()
+    b.evict()
+    for t in toks[held:]:
+        assert torch.equal(a.step(t), b.step(t))
+    assert int(b.status.item()) == 0
