@@ -69,8 +69,14 @@ __device__ __forceinline__ uint16_t ldg_u16(const void* p) {
 }
 
 // Coherent loads for data that the previous kernel of the stream may have
-// written while this one was already running (launch overlap): activations
-// and the plug correction.  The read-only path above is for weights only.
+// written while this one was already running (launch overlap): activations,
+// logits and the plug correction.  The read-only path above is for weights only.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {  // as ldg_stream
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint2 ld_u2(const void* p) { return *reinterpret_cast<const uint2*>(p); }
 __device__ __forceinline__ uint32_t ld_u32(const void* p) { return *reinterpret_cast<const uint32_t*>(p); }
 __device__ __forceinline__ uint16_t ld_u16(const void* p) { return *reinterpret_cast<const uint16_t*>(p); }

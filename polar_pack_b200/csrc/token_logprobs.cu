@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) token_logprobs_kern
       for (int k = 0; k < kBatch; ++k) {
         const int i = b0 + k * kThreads + tid;
         q[k] = Vec<T>::nothing();
-        if (i < v1) q[k].v = ldg_stream(xv + i);
+        if (i < v1) q[k].v = ld_stream(xv + i);  // coherent: the logits may be new
       }
     };
     auto take = [&](const Vec<T> (&q)[kBatch], int b0) {

@@ -197,3 +197,32 @@ def test_capture_at_a_blocks_end(cuda, parts, held):
     for t in toks[held:]:
         assert torch.equal(a.step(t), b.step(t))
     assert int(b.status.item()) == 0
+
+
+def test_launch_overlap(cuda, parts):
+    """Steps, evictions, a replayed step and scores, each kernel started while
+    the one before it runs: the same bits as one after another."""
+    from polar_pack_b200 import _lib
+    cfg = parts[0]
+    toks = _tokens(cfg, 150, 11)
+    runs = []
+    old = _lib.set_launch_overlap(False)
+    try:
+        for on in (False, True):
+            _lib.set_launch_overlap(on)
+            dec = _decoder(parts, kv_budget=90, kv_slack=20, kv_recent=16, kv_sinks=3)
+            got = []
+            for t in toks[:100]:
+                got.append(dec.step(t).clone())
+                r = dec.logprobs(t, top=7)
+                got += [r.logprob, r.entropy, r.top_ids, r.top_logprobs]
+            got.append(dec.score(toks[100:].T))
+            dec.capture(torch.cuda.Stream(cuda))
+            got.append(dec.score(toks[100:130].T))
+            got += [w.clone() for w in dec.kv8_weights]
+            assert int(dec.status.item()) == 0
+            runs.append(got)
+    finally:
+        _lib.set_launch_overlap(old)
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)

@@ -95,3 +95,16 @@ def test_capture_waits_for_the_current_stream(monkeypatch):
     dec._run = lambda s: log.append("run")
     dec.capture(Stream())
     assert log[:3] == [("wait", "current"), "run", "synchronize"] and int(dec.pos) == 0
+
+
+def test_coherent_loads():
+    """With launch overlap a kernel runs while the one before it writes its
+    inputs: none of these operators reads through the read-only path, which
+    need not see such writes."""
+    import re
+    from pathlib import Path
+
+    import polar_pack_b200
+    src = Path(polar_pack_b200.__file__).parent / "csrc"
+    for f in (*src.glob("kv8*"), src / "token_logprobs.cu"):
+        assert not re.search(r"\bldg_\w+\(|__ldg\(|\.nc\b", f.read_text()), f.name
