@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kResident) token_logprobs_kern
         p.top_logprobs[r * p.top + lane] = to_f(x[i]) - lse;
       }
     }
-    if (TOP) __syncthreads();  // the list has been read
+    __syncthreads();  // the warps' sums and the list have been read
   }
 }
 

@@ -190,3 +190,25 @@ def test_short_rows(cuda, dtype, rows, vocab, top):
     x[2] = torch.finfo(dtype).min if dtype == torch.float16 else -1.0
     t = torch.randint(0, vocab, (rows,), generator=g, device=cuda, dtype=torch.int32)
     _check(x, t, top)
+
+
+@pytest.mark.parametrize("top", [0, 2])
+def test_more_rows_than_a_grid(cuda, top):
+    """More rows than a launch has CTAs for (2^24): a CTA takes one row after another."""
+    from polar_pack_b200.scoring import token_logprobs
+    rows, vocab = (1 << 24) + 5001, 6
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GB of device memory")
+    g = torch.Generator(device=cuda)
+    g.manual_seed(21)
+    x = (torch.randn(rows, vocab, generator=g, device=cuda) * 3).half()
+    t = torch.randint(0, vocab, (rows,), generator=g, device=cuda, dtype=torch.int32)
+    r = token_logprobs(x, t, top=top)
+    some = torch.cat([torch.arange(0, 6000, device=cuda), torch.arange(rows - 6000, rows, device=cuda)])
+    lp = torch.log_softmax(x[some].double(), 1)
+    tol = 2e-6 + 2.5e-7 * float(x.abs().max())
+    assert ((r.logprob[some] - lp.gather(1, t[some].long()[:, None])[:, 0]).abs() <= tol).all()
+    assert ((r.entropy[some] + (lp.exp() * lp).sum(1)).abs() <= 1e-5 * (1 + math.log(vocab))).all()
+    order = torch.sort(x[some].double(), dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(r.top_ids[some].long(), order)
+    assert ((r.top_logprobs[some] - lp.gather(1, order)).abs() <= tol).all()
