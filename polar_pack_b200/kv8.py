@@ -138,12 +138,21 @@ def _workspace(cache: KV8Cache, n: int, q_heads: int, weights: bool, given) -> t
 
 
 def _c_strides(*s: int):
+    """Row strides of a checked tensor for the C call.  Only a dimension of one
+    can have a stride there that is no multiple of 8 (_rows, _output): it
+    addresses nothing."""
     a = _strides.get(s)
     if a is None:
         if len(_strides) >= 1024:
             _strides.clear()
-        a = _strides[s] = (ctypes.c_int64 * len(s))(*s)
+        a = _strides[s] = (ctypes.c_int64 * len(s))(*(0 if x & 7 else x for x in s))
     return a
+
+
+def _odd_rows(t: torch.Tensor) -> bool:
+    """Rows that the kernels cannot read: strided, or not 16-byte aligned."""
+    st = t.stride()
+    return st[-1] != 1 or t.data_ptr() & 15 != 0 or any(s & 7 and n > 1 for s, n in zip(st[:-1], t.shape))
 
 
 def _rows(t: torch.Tensor, name: str, shape: tuple, cache: KV8Cache) -> torch.Tensor:
@@ -151,10 +160,8 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, cache: KV8Cache) -> torch.Te
     if t.dtype is not torch.float16 or t.shape != shape or t.get_device() != cache.index:
         raise ValueError(f"{name} must be FP16 {list(shape)} on {cache.device}, "
                          f"got {t.dtype} {list(t.shape)} on {t.device}")
-    if t.data_ptr() & 15 or not t.is_contiguous():
-        st = t.stride()
-        if st[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for s in st[:-1]):
-            t = t.clone(memory_format=torch.contiguous_format)
+    if (t.data_ptr() & 15 or not t.is_contiguous()) and _odd_rows(t):
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -195,9 +202,8 @@ def _output(out, q, cache: KV8Cache):
         if q.is_contiguous():
             return torch.empty_like(q)
         return torch.empty(q.shape, dtype=torch.float16, device=cache.device)
-    st = out.stride()
-    if (out.dtype is not torch.float16 or out.get_device() != cache.index or out.shape != q.shape or st[-1] != 1
-            or out.data_ptr() & 15 or any(s & 7 for s in st[:-1])):
+    if (out.dtype is not torch.float16 or out.get_device() != cache.index or out.shape != q.shape
+            or _odd_rows(out)):
         raise ValueError(f"out must be FP16 {list(q.shape)} on {cache.device} with 16-byte aligned contiguous rows")
     return out
 

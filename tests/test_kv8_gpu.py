@@ -643,3 +643,30 @@ def test_refusals(cuda):
         kv8_evict(c, KV8Cache.empty(2, 1, 128, 128, cuda), pos, w, 64, 0, 0)
     assert kv8_attention(z(2, 0, 4, 128), c, pos).shape == (2, 0, 4, 128)
     kv8_append(c, z(2, 0, 2, 128), z(2, 0, 2, 128), pos)
+
+
+# ----------------------------------------------- what a call must accept ----
+def _odd_ones(x):
+    """x with strides of its size-1 dimensions that mean nothing, and are odd."""
+    return x.as_strided(x.shape, [s if n > 1 else 8 * s + 1 + 2 * i for i, (n, s) in enumerate(zip(x.shape, x.stride()))])
+
+
+def test_strides_of_single_rows(cuda):
+    """The stride of a dimension of one is nobody's business: batch 1, one token, one head."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_attention, kv8_decode
+    g = _gen(cuda, 61)
+    k, v, q = _rand(g, 1, 3, 1, 64), _rand(g, 1, 3, 1, 64), _rand(g, 1, 1, 2, 64)
+    pos = _ints([0], cuda)
+    got = []
+    for odd in (lambda x: x, _odd_ones):
+        c = _new(1, 1, 64, 64, cuda)
+        kv8_append(c, odd(k[:, :2]), odd(v[:, :2]), pos)
+        kv8_append(c, odd(k[:, 2:]), odd(v[:, 2:]), pos + 2)
+        out = torch.zeros_like(q)
+        res = [kv8_attention(odd(q), c, pos + 3, out=odd(out)), kv8_attention(odd(q), c, pos + 3)]
+        out = torch.zeros_like(q[:, 0])
+        res += [kv8_decode(odd(q[:, 0]), odd(k[:, 0]), odd(v[:, 0]), c, pos + 3, out=odd(out)), out]
+        got.append(res + [c.k_tail[:, :, :4], c.v_tail[:, :, :4]])
+        assert int(c.status) == 0
+    for a, b in zip(*got):
+        assert a.any() and torch.equal(a, b)
