@@ -56,7 +56,9 @@ class KV8Cache:
             if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
                 raise ValueError(f"cache tensors must be contiguous; expected {shape} {dtype}, "
                                  f"got {tuple(t.shape)} {t.dtype}")
-        self.device = _lib.require_cuda(*(t for t, _, _ in want))
+        self.device = _lib.require_cuda(*(t for t, _, _ in want), status)
+        if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
+            raise ValueError("status must be an int32 tensor")
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.k_tail, self.v_tail = k_tail, v_tail
         self.batch, self.kv_heads, self.capacity, self.head_dim = b, h, cap, hd

@@ -670,3 +670,13 @@ def test_strides_of_single_rows(cuda):
         assert int(c.status) == 0
     for a, b in zip(*got):
         assert a.any() and torch.equal(a, b)
+
+
+def test_status_is_checked(cuda):
+    """The status word is written by the device: another place or type is refused."""
+    from polar_pack_b200.kv8 import KV8Cache
+    KV8Cache.empty(1, 1, 64, 64, cuda, status=torch.zeros(1, dtype=torch.int32, device=cuda))
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, device=cuda),
+                torch.zeros(1, dtype=torch.int64, device=cuda), torch.zeros(0, dtype=torch.int32, device=cuda)):
+        with pytest.raises((ValueError, RuntimeError)):
+            KV8Cache.empty(1, 1, 64, 64, cuda, status=bad)
