@@ -338,9 +338,9 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     const int r = e / (HD / 8), d0 = e % (HD / 8) * 8;
     const int i = p.n == 1 ? 0 : (row0 + r) / group, h = row0 + r - i * group;
     if (r >= NT * 8 || i >= p.n || h >= group) return make_uint4(0, 0, 0, 0);
-    const int t = p.rope.cos ? p.rope.pos[b] + i : 0;
-    if (p.rope.cos && (t < 0 || t >= p.rope.len)) return make_uint4(0, 0, 0, 0);
-    return kv8_load8(p.q + b * p.ldqb + i * p.ldqt + (int64_t)(kvh * group + h) * p.ldqh, d0, HD, p.rope, t);
+    const int t0 = p.rope.cos ? p.rope.pos[b] : 0;
+    if (p.rope.cos && (t0 < 0 || t0 >= p.rope.len - i)) return make_uint4(0, 0, 0, 0);
+    return kv8_load8(p.q + b * p.ldqb + i * p.ldqt + (int64_t)(kvh * group + h) * p.ldqh, d0, HD, p.rope, t0 + i);
   };
   auto token_row8 = [&](int b, int kvh, int e) {  // the token's key, then its value
     const int w = e / (HD / 8), d0 = e % (HD / 8) * 8;
@@ -367,9 +367,10 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
   // lengths and the units before each sequence; every warp for itself while a
   // warp's lanes hold them all (all write the same), else the CTA together
   auto length = [&](int b) {
-    const int len = p.lens[b] + p.extra;
+    const int held = p.lens[b];
     const int cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
-    bool ok = len <= p.c.cap;
+    bool ok = held <= p.c.cap - p.extra;  // held + extra may pass the type's end
+    const int len = ok ? held + p.extra : 1;
     if (p.rope.cos && len > 0 && cnt > 0) {
       const int r = p.rope.pos[b];
       ok = ok && r >= 0 && r <= p.rope.len - cnt;
@@ -905,8 +906,8 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const Kv8WeightsParams
   };
   load(0);
   const float before = *out;
-  const int len = p.lens[b] + p.extra, rot = p.rope.cos ? p.rope.pos[b] : 0;
-  if (len > p.cap || t >= len || (p.rope.cos && (rot < 0 || rot >= p.rope.len))) return;
+  const int held = p.lens[b], rot = p.rope.cos ? p.rope.pos[b] : 0;
+  if (held > p.cap - p.extra || t >= held + p.extra || (p.rope.cos && (rot < 0 || rot >= p.rope.len))) return;
   float w = 0.f;
   for (int h0 = 0;;) {
 #pragma unroll

@@ -680,3 +680,18 @@ def test_status_is_checked(cuda):
                 torch.zeros(1, dtype=torch.int64, device=cuda), torch.zeros(0, dtype=torch.int32, device=cuda)):
         with pytest.raises((ValueError, RuntimeError)):
             KV8Cache.empty(1, 1, 64, 64, cuda, status=bad)
+
+
+def test_positions_at_the_end_of_the_type(cuda):
+    """A position of 2^31 - 1 is past every capacity, not an unused sequence."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_decode
+    g = _gen(cuda, 62)
+    q, k, v = _rand(g, 2, 4, 128), _rand(g, 2, 1, 128), _rand(g, 2, 1, 128)
+    pos = _ints([2 ** 31 - 1, 3], cuda)
+    c = _new(2, 1, 64, 128, cuda, stale=False)
+    w = c.new_weights()
+    out = kv8_decode(q, k, v, c, pos, weights=w)
+    assert int(c.status) == 5 and not out[0].any() and out[1].any() and not w[0].any() and w[1].any()
+    c.status.zero_()
+    kv8_append(c, k[:, None], v[:, None], pos)
+    assert int(c.status) == 5
