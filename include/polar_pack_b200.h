@@ -473,7 +473,8 @@ PP_API int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t
  * which is one whole coded block of the old cache is copied unchanged.
  * into_weights ([batch][kv_heads][into->capacity]) receives the kept tokens'
  * weights, zero past them; new_lens[b] = min(lens[b], keep); kept
- * [batch][kv_heads][keep] the old positions, -1 past new_lens[b]. */
+ * [batch][kv_heads][keep] the old positions, -1 past new_lens[b].  No array
+ * that is written may share bytes with another one of the call. */
 PP_API int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int* lens, const float* weights,
                         float* into_weights, int* new_lens, int* kept, int64_t keep, int64_t sinks, int64_t recent,
                         int* status, void* stream);

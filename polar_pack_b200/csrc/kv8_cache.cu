@@ -440,6 +440,38 @@ __global__ void __launch_bounds__(kThreads, 6) kv8_gather_kernel(const EvictPara
   if (threadIdx.x == 0) to.scales[block] = q.scale;
 }
 
+// Whether an array that an eviction writes shares bytes with another of its
+// arrays: the kernels read the old cache while they write the new one.
+bool evict_overlaps(const EvictParams& p, const int* lens, const float* weights, const float* to_weights,
+                    const int* new_lens, const int* kept, int64_t keep) {
+  struct Range {
+    uintptr_t at;
+    uint64_t bytes;
+  } r[17];
+  int n = 0;
+  auto add = [&](const void* at, int64_t bytes) { r[n++] = Range{reinterpret_cast<uintptr_t>(at), (uint64_t)bytes}; };
+  const int64_t heads = (int64_t)p.c.batch * p.c.nkv;
+  auto cache = [&](const Kv8Cache& c) {
+    for (int w = 0; w < 2; ++w) {
+      add(c.codes[w], heads * c.cap * c.hd);
+      add(c.scales[w], heads * (c.cap / kKvBlock) * (int64_t)sizeof(float));
+      add(c.tail[w], heads * kKvBlock * c.hd * (int64_t)sizeof(__half));
+    }
+  };
+  cache(p.to);
+  add(to_weights, heads * p.to.cap * (int64_t)sizeof(float));
+  add(new_lens, p.c.batch * (int64_t)sizeof(int));
+  add(kept, heads * keep * (int64_t)sizeof(int));
+  const int written = n;
+  cache(p.c);
+  add(weights, heads * p.c.cap * (int64_t)sizeof(float));
+  add(lens, p.c.batch * (int64_t)sizeof(int));
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (r[i].at < r[j].at + r[j].bytes && r[j].at < r[i].at + r[i].bytes) return true;
+  return false;
+}
+
 bool g_select_attr[64];
 int g_select_limit[64];
 
@@ -519,13 +551,11 @@ int pp_kv8_evict(const pp_kv8_cache* cache, const pp_kv8_cache* into, const int*
                   "sinks + recent at most keep");
     return PP_ERR_INVALID;
   }
-  for (int w = 0; w < 2; ++w)
-    for (int u = 0; u < 2; ++u)
-      if (p.c.codes[w] == p.to.codes[u] || p.c.tail[w] == p.to.tail[u] || p.c.scales[w] == p.to.scales[u] ||
-          weights == into_weights) {
-        pp::set_error("pp_kv8_evict: the new cache must not be the old one");
-        return PP_ERR_INVALID;
-      }
+  if (pp::evict_overlaps(p, lens, weights, into_weights, new_lens, kept, keep)) {
+    pp::set_error("pp_kv8_evict: the arrays that are written must not overlap the old cache, its weights and lengths "
+                  "or one another");
+    return PP_ERR_INVALID;
+  }
   p.lens = lens;
   p.weights = weights;
   p.to_weights = into_weights;

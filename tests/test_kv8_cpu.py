@@ -108,3 +108,28 @@ def test_coherent_loads():
     src = Path(polar_pack_b200.__file__).parent / "csrc"
     for f in (*src.glob("kv8*"), src / "token_logprobs.cu"):
         assert not re.search(r"\bldg_\w+\(|__ldg\(|\.nc\b", f.read_text()), f.name
+
+
+def test_evict_refuses_what_overlaps(lib):
+    """Arrays that are written may share no byte with another one."""
+    L, M = lib.load(), 1 << 20
+    pair = lambda a, step: (ctypes.c_void_p * 2)(a, a + step)
+    old = dict(codes=pair(M, M), scales=pair(3 * M, M), tail=pair(5 * M, M), batch=1, kv_heads=1, capacity=256)
+    into = dict(codes=pair(11 * M, M), scales=pair(13 * M, M), tail=pair(15 * M, M), batch=1, kv_heads=1, capacity=256)
+    args = dict(lens=20 * M, weights=21 * M, into_weights=22 * M, new_lens=23 * M, kept=24 * M)
+
+    def call(new=into, **kw):
+        a = {**args, **kw}
+        return L.pp_kv8_evict(_cache(lib, **old), _cache(lib, **new), a["lens"], a["weights"], a["into_weights"],
+                              a["new_lens"], a["kept"], 64, 0, 0, None, None)
+
+    codes, tail, wts = 256 * 128, 64 * 128 * 2, 256 * 4
+    for at in (M + codes - 16, 2 * M + 64, 12 * M - codes + 16):            # old keys, old values, the new values
+        assert call({**into, "codes": (ctypes.c_void_p * 2)(at, 12 * M)}) == lib.PP_ERR_INVALID
+    assert call({**into, "tail": (ctypes.c_void_p * 2)(5 * M + tail - 16, 16 * M)}) == lib.PP_ERR_INVALID
+    assert call({**into, "scales": (ctypes.c_void_p * 2)(3 * M + 12, 14 * M)}) == lib.PP_ERR_INVALID
+    assert call(into_weights=21 * M + wts - 4) == lib.PP_ERR_INVALID
+    assert call(into_weights=21 * M - wts + 4) == lib.PP_ERR_INVALID
+    assert call(new_lens=20 * M) == lib.PP_ERR_INVALID
+    assert call(kept=20 * M - 63 * 4) == lib.PP_ERR_INVALID
+    assert call(kept=22 * M + 4) == lib.PP_ERR_INVALID
