@@ -437,7 +437,7 @@ PP_API int pp_kv8_restore(const pp_kv8_cache* cache, const int* lens, const int*
  * over positions 0 .. lens[b] - counts[b] + i of kv head h / (nq / kv_heads):
  * the queries are the last counts[b] (NULL: n) of the sequence's lens[b]
  * tokens, appended before.  Rows i >= counts[b], and rows that attend nothing,
- * are zero.  At most 16 query heads per kv head; status must not be NULL here
+ * are zero; infinities and NaN reach only the rows that attend them.  At most 16 query heads per kv head; status must not be NULL here
  * (1: a copy never arrived).  FP32 scores, softmax and sums; the softmax
  * weights are rounded to FP16 for the value product.  Workspace:
  * pp_kv8_attention_workspace_bytes on the device that is current (weights: for

@@ -80,6 +80,20 @@ __device__ __forceinline__ float kv8_finite(float x) { return x != x ? 0.f : fmi
 
 __device__ __forceinline__ uint32_t kv8_word(uint4 x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
+// Sets values of a word (two of them) that are infinite or NaN to zero; tells
+// which, by all bits of theirs.  The value products take masked positions by a
+// weight of 0, which such values would turn into NaN: the open block's go in
+// without them, and the rows that attend them have them added afterwards (a
+// softmax weight is positive, so it does not change them).
+__device__ __forceinline__ uint32_t kv8_drop_odd(uint32_t& x) {
+  const uint32_t odd = __vcmpeq2(x & 0x7c007c00u, 0x7c007c00u);
+  x &= ~odd;
+  return odd;
+}
+__device__ __forceinline__ uint32_t kv8_drop_odd(uint4& x) {
+  return kv8_drop_odd(x.x) | kv8_drop_odd(x.y) | kv8_drop_odd(x.z) | kv8_drop_odd(x.w);
+}
+
 // Largest magnitude of eight values; not finite if one is not.
 __device__ __forceinline__ float kv8_amax8(uint4 x) {
   __half2 m = __hmax2_nan(__hmax2_nan(__habs2(u2h(x.x)), __habs2(u2h(x.y))),

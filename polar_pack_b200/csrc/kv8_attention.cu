@@ -81,8 +81,8 @@ bool decode_takes(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
   return true;
 }
 
-bool g_attr[6][64];
-int g_limit[6][64];
+bool g_attr[10][64];
+int g_limit[10][64];
 
 int encode_codes(const Kv8Cache& c, CUtensorMap (&tm)[2]) {
   const uint64_t rows = (uint64_t)c.batch * c.nkv * c.cap;
@@ -93,11 +93,11 @@ int encode_codes(const Kv8Cache& c, CUtensorMap (&tm)[2]) {
   return PP_OK;
 }
 
-template <int NT, int HD>
+template <int NT, int HD, bool MANY>
 int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
-  constexpr int kv = (NT - 1) * 2 + (HD == 128);
+  constexpr int kv = (NT - 1) * 4 + MANY * 2 + (HD == 128);
   using S = Kv8DecodeSmem<NT, HD>;
-  auto kern = kv8_decode_kernel<NT, HD>;
+  auto kern = kv8_decode_kernel<NT, HD, MANY>;
   int lim = 0;
   if (int rc = ensure_smem_attr(kern, g_attr[kv], g_limit[kv], &lim)) return rc;
   const int smem = S::bytes(p.c.batch);
@@ -111,10 +111,16 @@ int launch_decode(const Kv8DecodeParams& p, int ctas, cudaStream_t s) {
                        (size_t)smem, s, p, tm[0], tm[1]);
 }
 
+template <bool MANY>
+int launch_decode(const Kv8DecodeParams& p, int nt, int ctas, cudaStream_t s) {
+  if (p.c.hd == 128) return nt == 1 ? launch_decode<1, 128, MANY>(p, ctas, s) : launch_decode<2, 128, MANY>(p, ctas, s);
+  return nt == 1 ? launch_decode<1, 64, MANY>(p, ctas, s) : launch_decode<2, 64, MANY>(p, ctas, s);
+}
+
 template <int HD>
 int launch_prompt(const Kv8PromptParams& p, cudaStream_t s) {
   using S = Kv8PromptSmem<HD>;
-  constexpr int kv = 4 + (HD == 128);
+  constexpr int kv = 8 + (HD == 128);
   auto kern = kv8_prompt_kernel<HD>;
   int lim = 0;
   if (int rc = ensure_smem_attr(kern, g_attr[kv], g_limit[kv], &lim)) return rc;
@@ -200,9 +206,7 @@ int run_decode(const char* who, Kv8DecodeParams& p, float* weights, void* worksp
       p.lse = all.lse + (int64_t)b0 * all.nq;
       p.scores = all.scores + (int64_t)b0 * all.nq * all.c.cap;
     }
-    if (int rc = p.c.hd == 128 ? (d.nt == 1 ? launch_decode<1, 128>(p, ctas, s) : launch_decode<2, 128>(p, ctas, s))
-                               : (d.nt == 1 ? launch_decode<1, 64>(p, ctas, s) : launch_decode<2, 64>(p, ctas, s)))
-      return rc;
+    if (int rc = p.n > 1 ? launch_decode<true>(p, d.nt, ctas, s) : launch_decode<false>(p, d.nt, ctas, s)) return rc;
   }
   if (!weights) return PP_OK;
   const Kv8WeightsParams w{all.scores, all.lse, weights, all.lens, all.rope, all.extra, all.nq, all.c.nkv, all.c.cap};

@@ -216,6 +216,31 @@ __device__ __forceinline__ void kv8_softmax(Kv8Acc<NT, HD>& a, float (&s)[MT][NT
   }
 }
 
+// The first n rows of a tail unit's values, at v in shared memory, without those
+// that are infinite or NaN (kv8_drop_odd); whether there were any.
+template <int HD>
+__device__ __forceinline__ bool kv8_drop_odd_rows(uint32_t v, int n) {
+  const int lane = threadIdx.x & 31;
+  __half2 top = __float2half2_rn(0.f);
+#pragma unroll
+  for (int k = 0; k < kDecTailUnit * HD / 8 / 32; ++k) {
+    const int e = k * 32 + lane;
+    const uint4 x = lds128(v + e * 16);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(u2h(x.x)), __habs2(u2h(x.y))),
+                                  __hmax2_nan(__habs2(u2h(x.z)), __habs2(u2h(x.w))));
+    if (e < n * (HD / 8)) top = __hmax2_nan(top, m);
+  }
+  const float2 f = __half22float2(top);
+  if (__all_sync(0xffffffffu, f.x <= 65504.f && f.y <= 65504.f)) return false;
+#pragma unroll 1
+  for (int e = lane; e < n * (HD / 2); e += 32) {
+    uint32_t x = lds_u32(v + e * 4);
+    kv8_drop_odd(x);
+    sts_u32(v + e * 4, x);
+  }
+  return true;
+}
+
 // What a CTA knows of the launch's work: effective lengths and unit counts.
 // A segment counts kDecSegmentUnits more units than it has, at its end, for
 // the time between two segments of a CTA (about 3 us, which at the memory's
@@ -304,7 +329,37 @@ struct Kv8Part {
   int b, kvh, row0, rows, seg0, first, contrib, last;
 };
 
+// Adds the values of the tail rows u0 to u1 that are infinite or NaN to the
+// results of the rows that attend them, in rec or (NULL) in the output.
 template <int NT, int HD>
+__device__ __noinline__ void kv8_add_odd(const Kv8DecodeParams& p, int b, int kvh, int row0, int rows, int cnt, int len,
+                                         int u0, int u1, float* rec) {
+  const int group = p.nq / p.c.nkv, t0 = kv8_last_block(len) * kKvBlock;
+  for (int e = threadIdx.x; e < HD / 16 * NT * 2 * 32; e += kv8_warps(NT) * 32) {
+    const int el = e & 31, r = (e >> 6) % NT * 8 + 2 * (el & 3) + ((e >> 5) & 1);
+    const int d = 16 * ((e >> 6) / NT) + 2 * (el >> 2), i = (row0 + r) / group, h = row0 + r - i * group;
+    if (r >= rows || i >= cnt) continue;
+    float x = 0.f, y = 0.f;
+    for (int t = u0; t < min(u1, len - cnt + i + 1 - t0); ++t) {
+      uint32_t v = *reinterpret_cast<const uint32_t*>(p.c.tail_row(1, b, kvh, t) + d), rest = v;
+      v &= kv8_drop_odd(rest);
+      x += __low2float(u2h(v));
+      y += __high2float(u2h(v));
+    }
+    if (x == 0.f && y == 0.f) continue;
+    if (rec) {
+      rec[r * HD + d] += x;
+      rec[r * HD + d + 1] += y;
+    } else {
+      __half2* o = reinterpret_cast<__half2*>(p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh + d);
+      *o = __floats2half2_rn(__low2float(*o) + x, __high2float(*o) + y);
+    }
+  }
+}
+
+// MANY: the call has several query tokens (a single one attends all of the
+// tail).  Its own kernel, as the other is 2 to 4% slower with its code.
+template <int NT, int HD, bool MANY>
 __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
     kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
@@ -312,6 +367,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
   constexpr int kWarps = S::kWarps, kThreads = kWarps * 32, kPartFloats = kv8_part_floats(NT, HD);
   __shared__ float red[kWarps];
   __shared__ int s_max;
+  __shared__ int s_odd;  // the last segment with values in the tail that are infinite or NaN
   __shared__ Kv8Part s_part[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
@@ -319,6 +375,7 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
   const uint32_t k_bar = base + S::kBar + warp * 16, v_bar = k_bar + 8;
   int* s_len = reinterpret_cast<int*>(pp_smem + S::kLens);
   int* s_pre = s_len + p.c.batch;
+  if (tid == 0) s_odd = -1;
   if (lane == 0) {
     mbar_init(k_bar, 1);
     mbar_init(v_bar, 1);
@@ -702,6 +759,10 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       uint32_t pb[1][NT][2];
       kv8_softmax<NT, HD, 1>(acc, s, gain, pb);
       await_values(more);
+      if (MANY && kv8_drop_odd_rows<HD>(v_slot, min(len - t0, kDecTailUnit))) {  // one query attends all rows
+        __syncwarp();
+        if (lane == 0) s_odd = segment;
+      }
       const uint32_t v0 = row(1, 2 * t4) + 4 * g, v1 = row(1, 2 * t4 + 1) + 4 * g;
       const uint32_t v2 = row(1, 2 * t4 + 8) + 4 * g, v3 = row(1, 2 * t4 + 9) + 4 * g;
       const int left = len - t0 - 2 * t4;  // rows past the end count as zero: their contents may be anything
@@ -798,6 +859,11 @@ __global__ void __launch_bounds__(kv8_warps(NT) * 32, 1)
       }
     }
 
+    if (MANY && s_odd == segment) {  // the same for all threads
+      __syncthreads();               // the results are written
+      kv8_add_odd<NT, HD>(p, b, kvh, row0, rows, cnt, len, (max(at - seg0, coded) - coded) * kDecTailUnit,
+                          (u_end - coded) * kDecTailUnit, whole ? nullptr : rec);
+    }
     if (!whole) {
       if (tid == 0) {
         const int first = aligned ? segment * each : seg0 / per;

@@ -78,7 +78,8 @@ struct Kv8PromptSmem {
   static constexpr int kK = 2 * kQTile;                          // two buffers each
   static constexpr int kV = kK + 2 * kKv;
   static constexpr int kCodes = kV + 2 * kKv;
-  static constexpr int kBar = kCodes + kPrCodeStages * 2 * kCode;
+  static constexpr int kTail = kCodes + kPrCodeStages * 2 * kCode;  // the open block's values, plain rows
+  static constexpr int kBar = kTail + kKvBlock * HD * 2;
   static constexpr int kBytes = kBar + 256;
 };
 
@@ -138,6 +139,36 @@ __device__ __forceinline__ int kv8_part_blocks(const Kv8PromptParams& p) {
 // Row r of a call's n * group rows: query r / group, head r % group.
 __device__ __forceinline__ int kv8_row_stop(int i, int len, int cnt) { return i < cnt ? len - cnt + i + 1 : 0; }
 
+// Adds the values of the open block that are infinite or NaN to the results of
+// this CTA's rows that attend them: to the output, or to the part's sums in
+// FP32.  The softmax warps' threads come here, a row each; everything is worked
+// out again, as the kernel has no registers to keep it in.
+template <int HD>
+__device__ __noinline__ void kv8_prompt_add_odd(const Kv8PromptParams& p, bool parts) {
+  const int tile = p.tiles - 1 - blockIdx.y % p.tiles, split = blockIdx.y / p.tiles;
+  const int kvh = blockIdx.x % p.c.nkv, b = blockIdx.x / p.c.nkv, group = p.nq / p.c.nkv, rows = p.n * group;
+  const int r = tile * kPrRows + threadIdx.x, i = r / group, h = r - i * group;
+  if (r >= rows) return;
+  const int len = p.lens[b], cnt = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+  const int open = kv8_last_block(len) * kKvBlock, stop = kv8_row_stop(i, len, cnt);
+  __half* out = p.out + b * p.ldob + i * p.ldot + (int64_t)(kvh * group + h) * p.ldoh;
+  float* sums = p.part + ((((int64_t)split * p.c.batch + b) * p.c.nkv + kvh) * rows + r) * HD;
+  for (int t = open; t < stop; ++t)
+    for (int d = 0; d < HD; d += 2) {
+      uint32_t v = *reinterpret_cast<const uint32_t*>(p.c.tail_row(1, b, kvh, t - open) + d), rest = v;
+      v &= kv8_drop_odd(rest);
+      if (v == 0) continue;
+      const float2 f = __half22float2(u2h(v));
+      if (parts) {
+        sums[d] += f.x;
+        sums[d + 1] += f.y;
+      } else {
+        __half2* o = reinterpret_cast<__half2*>(out + d);
+        *o = __floats2half2_rn(__low2float(*o) + f.x, __high2float(*o) + f.y);
+      }
+    }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kPrThreads, 1)
     kv8_prompt_kernel(const __grid_constant__ Kv8PromptParams p, const __grid_constant__ CUtensorMap tk,
@@ -145,6 +176,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   using S = Kv8PromptSmem<HD>;
   __shared__ float s_red[8];
   __shared__ uint32_t s_tmem;
+  __shared__ int s_odd;  // values of the open block are infinite or NaN
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(pp_smem);
   // long tiles first, of all heads: the last rows attend the most positions
@@ -168,7 +200,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   const uint32_t s_full = bar + 128;                               // [tile][2]
   const uint32_t p_full = bar + 160;                               // [tile][2]
   const uint32_t o_full = bar + 192;                               // [tile][2]
-  const uint32_t done = bar + 224, q_full = bar + 232;
+  const uint32_t done = bar + 224, q_full = bar + 232, tail_full = bar + 240;
   if (tid == 0) {
     for (int i = 0; i < kPrCodeStages; ++i) {
       mbar_init(code_full + 8 * i, 1);
@@ -187,6 +219,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     }
     mbar_init(done, 1);
     mbar_init(q_full, 8);
+    mbar_init(tail_full, 8);
+    s_odd = 0;
     fence_mbar_init();
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
@@ -252,6 +286,26 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
       for (int j = j0 + tid; j < min(j1, coded); j += 256) vref = fmaxf(vref, v_scale[j]);
+      if (j1 > coded) {  // the open block's values, zero past the end and where they are infinite or NaN
+        constexpr int kTailItems = kKvBlock * (HD / 8) / 256;
+        uint4 x[kTailItems];
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < kTailItems; ++k) {
+          const int e = k * 256 + tid, row = e / (HD / 8);
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (coded * kKvBlock + row < len)
+            x[k] = *reinterpret_cast<const uint4*>(p.c.tail_row(1, b, kvh, row) + e % (HD / 8) * 8);
+        }
+#pragma unroll
+        for (int k = 0; k < kTailItems; ++k) {
+          odd |= kv8_drop_odd(x[k]);
+          *reinterpret_cast<uint4*>(pp_smem + S::kTail + (k * 256 + tid) * 16) = x[k];
+        }
+        if (odd) s_odd = 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tail_full);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
@@ -439,12 +493,15 @@ __global__ void __launch_bounds__(kPrThreads, 1)
             hi[cc] = make_uint4(codes2<0x4140>(x[cc].z), codes2<0x4342>(x[cc].z), codes2<0x4140>(x[cc].w),
                                 codes2<0x4342>(x[cc].w));
           }
-        } else {  // FP16 rows from memory, zero past the end
+        } else {  // FP16 rows, zero past the end
+          if (side) fine = wait(tail_full, 0);
+          const __half* tail =
+              side ? reinterpret_cast<const __half*>(pp_smem + S::kTail + r * HD * 2) : p.c.tail_row(0, b, kvh, r);
 #pragma unroll
           for (int cc = 0; cc < kChunks; ++cc) {
             lo[cc] = hi[cc] = make_uint4(0, 0, 0, 0);
             if ((j0 + j) * kKvBlock + r < len) {
-              const uint4* g = reinterpret_cast<const uint4*>(p.c.tail_row(side, b, kvh, r) + 16 * (2 * cc + (w >> 1)));
+              const uint4* g = reinterpret_cast<const uint4*>(tail + 16 * (2 * cc + (w >> 1)));
               lo[cc] = g[0];
               hi[cc] = g[1];
             }
@@ -548,6 +605,7 @@ __global__ void __launch_bounds__(kPrThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (tid < kPrRows && s_odd) kv8_prompt_add_odd<HD>(p, splits > 1);  // the results are written
   if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

@@ -695,3 +695,48 @@ def test_positions_at_the_end_of_the_type(cuda):
     c.status.zero_()
     kv8_append(c, k[:, None], v[:, None], pos)
     assert int(c.status) == 5
+
+
+@pytest.mark.parametrize("nq,nkv,hd,n,lens,counts", [
+    (4, 2, 64, 4, [40, 2, 70], [4, 4, 1]),          # one tile of rows
+    (16, 2, 128, 10, [30, 90, 128], [10, 7, 9]),     # 80 rows to a kv head
+    (2, 1, 128, 200, [250, 200, 60], [200, 199, 60]),   # more than 256
+    (14, 2, 64, 60, [100, 4100, 0], [60, 60, 0]),    # positions split
+])
+def test_values_that_are_not_numbers(cuda, nq, nkv, hd, n, lens, counts):
+    """Values of NaN and infinity in the open block: rows that attend them get
+    what the formula gives, all others are as if they were not there."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_attention
+    g = _gen(cuda, 63 + n)
+    B = len(lens)
+    cap = -(-max(lens) // 64) * 64 + 64
+    k, v = (_rand(g, B, max(lens), nkv, hd) for _ in "kv")
+    q = _rand(g, B, n, nq, hd, spread=2.0)
+    bad = v.clone()
+    late = [max(l - max(c // 2, 1), 0) for l, c in zip(lens, counts)]      # the first position that is not finite
+    late = [max(t, (l - 1) // 64 * 64) for t, l in zip(late, lens)]
+    for b, (t, l) in enumerate(zip(late, lens)):
+        if l:
+            bad[b, t, :, 3], bad[b, t, 0, 9], bad[b, l - 1, :, 3], bad[b, l - 1, 0, 20] = (
+                float("inf"), float("nan"), -float("inf"), -float("inf"))
+    outs, want = [], None
+    for x in (v, bad):
+        cache = _new(B, nkv, cap, hd, cuda)
+        kv8_append(cache, k, x, _ints([0] * B, cuda), counts=_ints(lens, cuda))
+        outs.append(kv8_attention(q, cache, _ints(lens, cuda), counts=_ints(counts, cuda)))
+        assert int(cache.status) == 0
+    ref = kr.RefKV(B, nkv, hd)
+    ref.append(k, bad, lens)
+    want, _ = kr.attention(ref, q, counts)
+    plain, out = outs
+    vmax = float(v.abs().max())
+    for b, (l, c) in enumerate(zip(lens, counts)):
+        for i in range(n):
+            if i >= c or l - c + i < late[b]:
+                assert torch.equal(out[b, i], plain[b, i]), (b, i)
+                assert not (i >= c or l - c + i < 0) or not out[b, i].any()
+                continue
+            x, y = out[b, i].cpu().double(), want[b, i]
+            same = (x == y) | (x.isnan() & y.isnan())
+            assert (same | ((x - y).abs() <= OUT_TOL * vmax)).all(), (b, i)
+            assert not torch.isfinite(x[:, 3]).any()
