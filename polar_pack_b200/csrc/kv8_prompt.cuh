@@ -3,11 +3,14 @@
 //
 // Mathematics as in kv8_decode.cuh, with the running maximum moved only when a
 // row outgrows it by 2^4 and the block scale of the values folded into the
-// weights: with f = s_v / v_ref, v_ref the largest s_v of the range, the tensor
-// core accumulates P' (c_v - 128) for P' = fp16(2^11 f exp(S - m)), and
-// out = v_ref sum P' (c_v - 128) / (2^11 sum exp(S - m)).  2^11 leaves 2^4 for the
-// lagging maximum below FP16's largest number, and keeps weights down to
-// 2^-25 / f of the maximum at full precision.
+// weights: with f = s_v / v_ref, v_ref the power of two above the largest s_v of
+// the range, the tensor core accumulates P' (c_v - 128) for
+// P' = fp16(2^11 f exp(S - m)), and
+// out = v_ref sum P' (c_v - 128) / (2^11 sum exp(S - m)).  The open block's rows
+// are divided by v_ref instead (which is at least 2^-15 of their largest, so
+// that they stay FP16 numbers).  2^11 leaves 2^4 for the lagging maximum below
+// FP16's largest number, and keeps weights down to 2^-25 / f of the maximum at
+// full precision.
 //
 // Bound: the matrix products; next to them the 16 exponentials a clock of an
 // SM, which take about as long.  A CTA has 256 rows (query x head of the kv
@@ -258,8 +261,10 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");  // 256 x 144 + 384 x 64 = 640 x 96 registers
     // -------------------------------------------------------------- softmax
     // the query rows to their tiles, K-major, while the first blocks are on their
-    // way: sixteen loads at a time; and the largest value scale of the blocks
-    float vref = j1 > coded ? 1.f : 0.f;  // the tail's rows count as they are
+    // way: sixteen loads at a time; and the reference of the value scales
+    float vref = 0.f;
+    constexpr int kTailItems = kKvBlock * (HD / 8) / 256;
+    uint4 open[kTailItems];
     if (J > 0) {
       constexpr int kItems = kPrRows * (HD / 8) / 256, kBatch = 16 < kItems ? 16 : kItems;
 #pragma unroll 1
@@ -287,24 +292,20 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       if (lane == 0) mbar_arrive(q_full);
       for (int j = j0 + tid; j < min(j1, coded); j += 256) vref = fmaxf(vref, v_scale[j]);
       if (j1 > coded) {  // the open block's values, zero past the end and where they are infinite or NaN
-        constexpr int kTailItems = kKvBlock * (HD / 8) / 256;
-        uint4 x[kTailItems];
         uint32_t odd = 0;
 #pragma unroll
         for (int k = 0; k < kTailItems; ++k) {
           const int e = k * 256 + tid, row = e / (HD / 8);
-          x[k] = make_uint4(0, 0, 0, 0);
+          open[k] = make_uint4(0, 0, 0, 0);
           if (coded * kKvBlock + row < len)
-            x[k] = *reinterpret_cast<const uint4*>(p.c.tail_row(1, b, kvh, row) + e % (HD / 8) * 8);
+            open[k] = *reinterpret_cast<const uint4*>(p.c.tail_row(1, b, kvh, row) + e % (HD / 8) * 8);
         }
 #pragma unroll
         for (int k = 0; k < kTailItems; ++k) {
-          odd |= kv8_drop_odd(x[k]);
-          *reinterpret_cast<uint4*>(pp_smem + S::kTail + (k * 256 + tid) * 16) = x[k];
+          odd |= kv8_drop_odd(open[k]);
+          vref = fmaxf(vref, kv8_amax8(open[k]) * 0x1p-15f);
         }
         if (odd) s_odd = 1;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tail_full);
       }
     }
 #pragma unroll
@@ -312,15 +313,30 @@ __global__ void __launch_bounds__(kPrThreads, 1)
     if (lane == 0) s_red[warp] = vref;
     asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps, all of which come here
     for (int k = 0; k < 8; ++k) vref = fmaxf(vref, s_red[k]);
+    vref = __uint_as_float((__float_as_uint(vref) + 0x7fffffu) & 0xff800000u);
     if (!(vref > 0.f)) vref = 1.f;  // every value is zero
+    const float per_vref = 1.f / vref;
+    if (J > 0 && j1 > coded) {
+#pragma unroll
+      for (int k = 0; k < kTailItems; ++k) {
+        uint32_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(u2h(kv8_word(open[k], i)));
+          y[i] = h2u(__floats2half2_rn(f.x * per_vref, f.y * per_vref));
+        }
+        *reinterpret_cast<uint4*>(pp_smem + S::kTail + (k * 256 + tid) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tail_full);
+    }
     const int t = warp >> 2, r = row0 + t * kPrTile + (warp & 3) * 32 + lane;
     const int i = r / group, h = r - i * group;
     const int stop = r < rows ? kv8_row_stop(i, len, cnt) : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_cols = tmem + lanes + (uint32_t)(t * HD);
     float m = -INFINITY, l = 0.f;
-    const float per_vref = 1.f / vref;
-    float ks = 1.f, vs = 1.f;  // of the next block
+    float ks = 1.f, vs = vref;  // of the next block
     if (J > 0 && j0 < coded) {
       ks = k_scale[j0];
       vs = v_scale[j0];
@@ -331,7 +347,8 @@ __global__ void __launch_bounds__(kPrThreads, 1)
       const int blk = j0 + j, buf = j & 1;
       const float k = fmaxf(ks * p.scale2, 1e-30f);  // positive: a masked score stays -inf
       const float log_f = vs == 0.f ? 0.f : __log2f(vs * per_vref);
-      ks = vs = 1.f;
+      ks = 1.f;
+      vs = vref;
       if (blk + 1 < min(j1, coded)) {
         ks = k_scale[blk + 1];
         vs = v_scale[blk + 1];

@@ -740,3 +740,40 @@ def test_values_that_are_not_numbers(cuda, nq, nkv, hd, n, lens, counts):
             same = (x == y) | (x.isnan() & y.isnan())
             assert (same | ((x - y).abs() <= OUT_TOL * vmax)).all(), (b, i)
             assert not torch.isfinite(x[:, 3]).any()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size,tail", [(1.0, 1.0), (1e-2, 1e-2), (1e-3, 1e-3), (1e-4, 1e-4), (1e-3, 30.0), (1.0, 1e-3),
+                                       (100.0, 100.0)])
+def test_small_values_beside_a_sink(cuda, hd, size, tail):
+    """Values of any size, where a first position takes most of the weight and
+    the rest of it is spread over all the others; positions not split."""
+    from polar_pack_b200.kv8 import kv8_append, kv8_attention
+    g = _gen(cuda, hd)
+    heads, n, L = 90, 270, 3000
+    last = (L - 1) // 64 * 64
+    for gap in (8.0, 11.0, 13.0):
+        q = torch.zeros(1, n, heads, hd, device=cuda)
+        q[..., 0] = 8
+        k = torch.zeros(1, L, heads, hd, device=cuda)
+        k[:, 0, :, 0] = gap / 8 * hd ** 0.5
+        v = 1 + 0.1 * torch.rand(1, L, heads, hd, generator=g, device=cuda)
+        v[:, 0] *= -1
+        v[:, :last] *= size
+        v[:, last:] *= tail
+        k, v, q = k.half(), v.half(), q.half()
+        cache = _new(1, heads, 3008, hd, cuda, stale=False)
+        kv8_append(cache, k, v, _ints([0], cuda))
+        out = kv8_attention(q, cache, _ints([L], cuda))
+        x = []
+        for codes, scales, rows in ((cache.k_codes, cache.k_scales, cache.k_tail),
+                                    (cache.v_codes, cache.v_scales, cache.v_tail)):
+            y = (codes[0].double() - 128) * scales[0].double().repeat_interleave(64, 1)[..., None]
+            x.append(torch.cat([y[:, :last], rows[0, :, :L - last].double()], 1))
+        for i in (n - 1, n // 2, 0):
+            end = L - n + i + 1
+            p = torch.softmax((x[0][:, :end] @ q[0, i, :, :, None].double())[..., 0] / hd ** 0.5, -1)
+            want = (p[:, None] @ x[1][:, :end])[:, 0]
+            bound = OUT_TOL * x[1][:, :end].abs().amax((1, 2))[:, None] + 2.0 ** -24
+            assert ((out[0, i].double() - want).abs() <= bound).all(), (gap, i)
+        assert int(cache.status) == 0
