@@ -777,3 +777,40 @@ def test_small_values_beside_a_sink(cuda, hd, size, tail):
             bound = OUT_TOL * x[1][:, :end].abs().amax((1, 2))[:, None] + 2.0 ** -24
             assert ((out[0, i].double() - want).abs() <= bound).all(), (gap, i)
         assert int(cache.status) == 0
+
+
+def test_launch_overlap(cuda):
+    """Each kernel started while the one before it runs: the same bits as one after another."""
+    from polar_pack_b200 import _lib
+    from polar_pack_b200.kv8 import kv8_append, kv8_attention, kv8_decode, kv8_evict, kv8_restore
+    runs = []
+    old = _lib.set_launch_overlap(False)
+    try:
+        for on in (False, True):
+            _lib.set_launch_overlap(on)
+            g = _gen(cuda, 71)
+            got = []
+            for nq, nkv, hd, n, lens in ((16, 2, 128, 150, [4000, 150, 0]), (6, 3, 64, 5, [700, 64, 5]),
+                                         (7, 1, 128, 1, [63, 1, 2000])):
+                counts = [min(n, l) for l in lens]
+                k, v = (_rand(g, 3, max(lens), nkv, hd) for _ in "kv")
+                q, q1 = _rand(g, 3, n, nq, hd, spread=2.0), _rand(g, 4, 3, nq, hd, spread=2.0)
+                k1, v1 = (_rand(g, 4, 3, nkv, hd) for _ in "kv")
+                a, b = (_new(3, nkv, 4100, hd, cuda, stale=False) for _ in "ab")
+                pos, new, w = _ints(lens, cuda), _ints([l + 4 for l in lens], cuda), a.new_weights()
+                steps = [pos + i for i in range(4)]
+                for _ in range(3):           # the caches are written again while they may still be read
+                    kv8_append(a, k, v, pos * 0, counts=pos)
+                    got.append(kv8_attention(q, a, pos, counts=_ints(counts, cuda)))
+                    for i in range(4):
+                        got.append(kv8_decode(q1[i], k1[i], v1[i], a, steps[i], weights=w))
+                    got += kv8_evict(a, b, new, w, 100, sinks=2, recent=30)
+                    got += kv8_restore(b, got[-2], count=100)
+                    got.append(kv8_attention(q, b, got[-4], counts=_ints(counts, cuda).clamp(max=100)))
+                got.append(w)
+                assert int(a.status) == 0 and int(b.status) == 0
+            runs.append(got)
+    finally:
+        _lib.set_launch_overlap(old)
+    for x, y in zip(*runs):
+        assert torch.equal(x, y)
