@@ -399,6 +399,8 @@ PP_API int pp_swiglu_rows(const void* gate_up, int64_t ldg, int64_t I, void* y, 
  * as 0, infinities as +-65504).  The block that holds a sequence's last token
  * is read from the FP16 tail; its codes are written by the call that completes
  * it, so the cache does not depend on how its tokens were split into calls.
+ * Lengths grow: the first token of a block takes the place of the block before
+ * it in the tail, after which no call may go back to that block's end.
  * capacity is a multiple of 64, head_dim 64 or 128, all arrays 16-byte aligned.
  * Lengths, positions and counts are int32 in device memory, one per sequence;
  * the caller advances them.  A sequence that would pass the capacity (or its
@@ -454,7 +456,8 @@ PP_API int pp_kv8_attention(const pp_kv8_cache* cache, const void* q, const int6
 /* The single-token form: appends one token per sequence at pos[b] (as
  * pp_kv8_append) and attends to positions 0 .. pos[b] (as pp_kv8_attention).
  * weights (optional, NULL: none): float [batch][kv_heads][capacity];
- * weights[b][g][t] += sum of head group g's softmax weights at position t.
+ * weights[b][g][t] += sum of head group g's softmax weights at position t
+ * (pp_kv8_attention adds none).
  * Strides are those of (sequence, head).  Calls at the same position rewrite
  * the same token. */
 PP_API int pp_kv8_decode(const pp_kv8_cache* cache, const void* q, const int64_t q_strides[2], int64_t nq, const void* k,

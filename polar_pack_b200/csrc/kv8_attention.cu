@@ -61,15 +61,16 @@ PromptPlan plan_prompt(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
 // 256 rows never.  Between, the times that the two kernels would take at full
 // caches, in ns, as measured on 148 SMs (16 query heads on 2 kv heads of 128):
 // decode 12 us and one for 300 blocks of 16 rows, a segment counting eight
-// more; prompt 9 us, 1.45 for a CTA's block, 4 for joining parts.
+// more; prompt 9 us, 1.45 for a CTA's block, 4 for joining parts.  The lengths
+// are on the device, so the estimate is by the capacity.
 //   sequences, positions, rows   decode  prompt (us)
-//   1, 512, 256                  13.3    18.8
-//   4, 4096, 96                  19.4    24.7
-//   4, 4096, 128                 25.0    23.7
-//   32, 512, 32                  13.6    21.1
-//   32, 512, 64                  33.2    21.3
-//   32, 4096, 32                 32.3    60.1
-//   32, 4096, 64                 63.9    60.4
+//   1, 512, 256                  13.0    19.8
+//   4, 4096, 96                  19.5    27.2
+//   4, 4096, 128                 25.2    26.5 (taken, by 5% the slower)
+//   32, 512, 32                  14.0    22.0
+//   32, 512, 64                  34.4    22.1
+//   32, 4096, 32                 32.6    63.7
+//   32, 4096, 64                 64.8    65.1
 bool decode_takes(const Kv8Cache& c, int64_t n, int64_t nq, int ctas) {
   const int64_t rows = n * (nq / c.nkv);
   if (rows <= 16 || rows > 256) return rows <= 16;

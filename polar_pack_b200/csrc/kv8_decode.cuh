@@ -21,7 +21,7 @@
 // the queries and the outputs take the same permutation.
 //
 // Measured: 4 sequences of 1024, 16 query heads on 2 kv heads of 128: 11 us, a
-// chain of launch, lengths, boxes, products and join; 64 ragged sequences up
+// chain of launch, lengths, boxes, products and join (13 us with two tokens each); 64 ragged sequences up
 // to 8190, 28 heads on 4, 244 MB: 64 us, 3.8 TB/s, bound by the warps' chains
 // of instructions (about 1200 a block; three warps to a scheduler keep 39% of
 // its slots busy) and by the barriers where segments end.

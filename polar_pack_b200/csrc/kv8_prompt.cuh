@@ -28,15 +28,16 @@
 // swizzled rows: K-major for the first product, MN-major for the second.
 // Every wait is bounded; tensor memory is released on every path.
 //
-// Measured: 4 prompts of 2048, 28 query heads on 4 kv heads of 128, causal: 182
-// us, 660 TFLOP/s of the pairs that count; ragged chunks of 509 of 0, 2040, 2332
-// and 4001, 16 heads on 2: 69 us (86 with the longest in one part).  A block
+// Measured: 4 prompts of 2048, 28 query heads on 4 kv heads of 128, causal: 185
+// us, 649 TFLOP/s of the pairs that count; ragged chunks of 509 of 0, 2040, 2332
+// and 4001, 16 heads on 2: 70 us (86 with the longest in one part).  A block
 // takes 1.1 us of both tiles, where its products need 0.68.  Copies that left
 // work out: without the unpacking, the exponentials or all but one step of
 // either product hardly faster, without products and softmax together 0.65 us;
 // so a block is bound by the softmax warps' own chain, one row to a thread, two
 // such warps to a scheduler.  A single pass over the scores with the maximum so far,
-// repeated where it grows, took 188 us.
+// repeated where it grows, took 188 us where this took 182.  The unpacking roles
+// keep some values in local memory (52 bytes at head_dim 128).
 #pragma once
 
 #include "kv8.cuh"

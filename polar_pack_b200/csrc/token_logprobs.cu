@@ -7,9 +7,10 @@
 // Bound: the logits' bytes for many rows; next to them one exponential per
 // logit, 16 a clock and SM, which at the measured memory rate are three
 // quarters of the time for 2-byte logits.  Measured: 2048 rows of 151936 FP16
-// with the 5 likeliest, 622 MB: 134 us, 4.6 TB/s, about 9 instructions a logit; 301
-// rows of 32003 FP32: 12 us, 3.2 TB/s; 4 rows with the 20 likeliest: 15 us, a chain
-// of barriers.  One pass: a thread keeps its own (maximum, Z, W = sum e^(x - m)
+// with the 5 likeliest, 622 MB: 134 us back to back, 4.6 TB/s, about 9 instructions a logit
+// (109 us without alternatives); 301 rows of 32003 FP32: 12 us, 3.2 TB/s; 4 rows
+// with the 20 likeliest: 14 to 16 us, 6.7 without: the rest are the bound, the second
+// look and the ranking at a row's end.  One pass: a thread keeps its own (maximum, Z, W = sum e^(x - m)
 // (x - m)), moved to a new maximum when a batch of its logits exceeds it, and
 // the place of its largest logit.  For the
 // alternatives logits are whole numbers (value, then lower index), all

@@ -21,6 +21,9 @@ strides are free (views whose rows are not 16-byte aligned are copied first).
 ``cache.status`` is a device int that becomes 5 when a sequence would pass the
 cache's capacity or its rotation tables; such a sequence is left unwritten and
 its outputs are zero.
+
+Lengths grow: the first token of a block takes the place of the block before it
+in the tail, so after it no call may go back to a length up to that block's end.
 """
 from __future__ import annotations
 
@@ -84,7 +87,8 @@ class KV8Cache:
         return cls(*codes, *scales, *tails, status=status)
 
     def new_weights(self) -> torch.Tensor:
-        """Zeroed attention weights for :func:`kv8_decode` to accumulate."""
+        """Zeroed attention weights for :func:`kv8_decode` to accumulate (what the queries of
+        :func:`kv8_attention` look at is not added)."""
         return torch.zeros(self.batch, self.kv_heads, self.capacity, dtype=torch.float32, device=self.device)
 
     def new_workspace(self, n: int, q_heads: int, weights: bool = False) -> torch.Tensor:
